@@ -14,7 +14,9 @@ CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libtef_hip.so")
 
 # -ffp-contract=off: keep the reference's (unfused) fp32 op order on the parity-sensitive paths.
-FLAGS = ["--offload-arch=gfx950", "-O3", "-ffp-contract=off", "-fPIC", "-std=c++17"]
+# -packed-fp32-ops: scalar fp32 instructions only; some forms of the packed ones have given wrong results on this hardware.
+FLAGS = ["--offload-arch=gfx950", "-O3", "-ffp-contract=off", "-fPIC", "-std=c++17",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 # -munsafe-fp-atomics (hardware floating-point atomic adds instead of compare-and-swap loops) only where a unit HAS
 # floating-point atomics, and what they are.  None of them is on the integer paths whose results are bitwise reproducible
