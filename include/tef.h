@@ -533,6 +533,34 @@ int tef_adam_clip_step(float *p, float *g, float *m, float *v, size_t n, const f
 int tef_adam_clip_step_hp(float *p, float *g, float *m, float *v, size_t n, const float *norm, const double *hp,
                           const float *step, void *stream);
 
+/* ---- layer normalisation over one axis (csrc/tef_norm.hip) ---------------------------------------------------------
+ * x is [outer][channels][inner], normalised over `channels` (inner = 1: rows; inner = H * W: feature maps):
+ *   y = act((x - mean) * rstd * weight[c] + bias[c] + residual)
+ * weight, bias, residual may each be NULL.  x, residual, y, dy, dx, dresidual have type `dtype`; weight, bias and their
+ * gradients `wdtype`, which is TEF_F32 or dtype.  Statistics and sums are fp32.  Pointers need the alignment of their element
+ * type only.  Forward: mean, rstd [outer * inner] are written for the backward pass (both NULL: not kept).
+ * Backward: any of dx, dresidual, dweight, dbias may be NULL; they are WRITTEN, not accumulated.  `bias` and `residual` are
+ * the forward pass's (read only when act is not TEF_ACT_NONE).  The workspace is needed for dweight / dbias; results do not depend on
+ * the order in which workgroups run. */
+#define TEF_F32  0
+#define TEF_F16  1
+#define TEF_BF16 2
+typedef struct tef_norm_desc {
+    long outer;
+    long inner;
+    int channels;
+    int dtype;
+    int wdtype;
+    int act;
+    float eps;
+} tef_norm_desc;
+int tef_layer_norm_forward(const tef_norm_desc *d, const void *x, const void *weight, const void *bias, const void *residual,
+                           void *y, float *mean, float *rstd, void *stream);
+size_t tef_layer_norm_workspace_bytes(const tef_norm_desc *d);
+int tef_layer_norm_backward(const tef_norm_desc *d, const void *x, const void *weight, const void *bias, const void *residual,
+                            const float *mean, const float *rstd, const void *dy, void *dx, void *dresidual, void *dweight,
+                            void *dbias, void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- validation metrics (loss/flow_val.py; evaluation only, batch 1, no gradients) ---------------------------------
  * Flow maps are planar [H][W] (fx, fy separately); event lists are loc [N][2] = (y, x), ts [N], mask [N][2]. */
 /* one warping step: flow lookup at loc (flow_out [N][2] = (f_y, f_x) if not NULL); if do_warp: loc += (tref - ts) * flow,

@@ -90,6 +90,14 @@ class NetPlan(ctypes.Structure):
         ("copy_batch", ctypes.c_int), ("wgrad_ws", _fp), ("wgrad_ws_bytes", ctypes.c_size_t),
     ]
 
+
+class NormDesc(ctypes.Structure):
+    """struct tef_norm_desc (include/tef.h)"""
+
+    _fields_ = [("outer", ctypes.c_long), ("inner", ctypes.c_long), ("channels", ctypes.c_int), ("dtype", ctypes.c_int),
+                ("wdtype", ctypes.c_int), ("act", ctypes.c_int), ("eps", ctypes.c_float)]
+
+
 # name -> (restype, argtypes); every symbol include/tef.h declares
 SIGNATURES = {
     "tef_version": (ctypes.c_int, []),
@@ -215,6 +223,9 @@ SIGNATURES = {
     "tef_adam_clip_step": (ctypes.c_int, [_fp, _fp, _fp, _fp, ctypes.c_size_t, _fp, ctypes.c_float, ctypes.c_double,
                                           ctypes.c_double, ctypes.c_double, ctypes.c_double, _fp, _fp]),
     "tef_adam_clip_step_hp": (ctypes.c_int, [_fp, _fp, _fp, _fp, ctypes.c_size_t, _fp, _fp, _fp, _fp]),
+    "tef_layer_norm_forward": (ctypes.c_int, [ctypes.POINTER(NormDesc)] + [_fp] * 8),
+    "tef_layer_norm_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(NormDesc)]),
+    "tef_layer_norm_backward": (ctypes.c_int, [ctypes.POINTER(NormDesc)] + [_fp] * 12 + [ctypes.c_size_t, _fp]),
     "tef_gru_blend": (ctypes.c_int, [_fp, _fp, _fp, ctypes.c_size_t, _fp, _fp]),
     "tef_gru_blend_backward": (ctypes.c_int, [_fp, _fp, _fp, _fp, ctypes.c_size_t, _fp, _fp, _fp, _fp]),
     "tef_val_event_step": (ctypes.c_int, [_fp, _fp, ctypes.c_int, ctypes.c_int, _fp, _fp, _fp, ctypes.c_int,

@@ -1,0 +1,689 @@
+// tef_norm.hip — layer normalisation over one axis, fused with what follows it in a normalised layer:
+//
+//   mean = sum_c x / C,  rstd = 1 / sqrt(sum_c (x - mean)^2 / C + eps),  u = (x - mean) * rstd
+//   z = u * weight[c] + bias[c] (+ residual),  y = act(z)
+//
+// and the gradients, with g = dy * act'(z), h = g * weight:
+//
+//   dx = rstd * (h - sum_c h / C - u * sum_c (h * u) / C),  dresidual = g
+//   dweight[c] = sum_rows g * u,  dbias[c] = sum_rows g
+//
+// x is [outer][C][inner], normalised over C: inner = 1 are rows (tokens, channels-last maps), inner > 1 the feature maps of
+// this package's networks.  Bound by memory: the forward pass reads x (and residual) once and writes y once, the backward
+// pass reads x, dy (and residual where the activation needs z) once and writes dx (and dresidual) once; a row's values stay
+// in registers between its sums and its results.  Sums and statistics are fp32: a lane adds its own elements, then lanes
+// and waves are joined in a fixed order.  The variance is taken of (x - mean), not as a difference of large moments.  z is
+// formed again in the backward pass instead of being derived from the rounded y: 1 - y^2 of a half-precision y near 1 has
+// no correct digit.  The sums over rows (dweight, dbias) go through one partial row per workgroup and a second launch that
+// adds those in a fixed order: bit-for-bit reproducible, no atomics.
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "tef.h"
+#include "tef_common.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxBlocks = 1024;       // persistent workgroups of a backward pass = partial rows of dweight / dbias
+
+template <typename T> __device__ inline float to_f(T v);
+template <> __device__ inline float to_f<float>(float v) { return v; }
+template <> __device__ inline float to_f<__half>(__half v) { return __half2float(v); }
+template <> __device__ inline float to_f<__hip_bfloat16>(__hip_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ inline T from_f(float v);
+template <> __device__ inline float from_f<float>(float v) { return v; }
+template <> __device__ inline __half from_f<__half>(float v) { return __float2half(v); }                          // nearest even
+template <> __device__ inline __hip_bfloat16 from_f<__hip_bfloat16>(float v) { return __float2bfloat16(v); }      // nearest even
+
+// V consecutive elements; the address is a multiple of the ELEMENT's size only (views, odd row lengths): gfx950's global
+// loads take that, in one instruction.
+template <typename T, int V> struct __attribute__((packed, aligned(sizeof(T)))) Pack { T v[V]; };
+template <typename T, int V> __device__ inline void load(const T *p, float (&f)[V])
+{
+    const Pack<T, V> q = *reinterpret_cast<const Pack<T, V> *>(p);
+#pragma unroll
+    for (int k = 0; k < V; ++k) f[k] = to_f<T>(q.v[k]);
+}
+template <typename T, int V> __device__ inline void store(T *p, const float (&f)[V])
+{
+    Pack<T, V> q;
+#pragma unroll
+    for (int k = 0; k < V; ++k) q.v[k] = from_f<T>(f[k]);
+    *reinterpret_cast<Pack<T, V> *>(p) = q;
+}
+// the first n of V elements (n >= V: all of them; n <= 0: none), the rest 0
+template <typename T, int V> __device__ inline void load_n(const T *p, int n, float (&f)[V])
+{
+    if (n >= V) return load<T, V>(p, f);
+#pragma unroll
+    for (int k = 0; k < V; ++k) f[k] = k < n ? to_f<T>(p[k]) : 0.0f;
+}
+template <typename T, int V> __device__ inline void store_n(T *p, int n, const float (&f)[V])
+{
+    if (n >= V) return store<T, V>(p, f);
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+        if (k < n) p[k] = from_f<T>(f[k]);
+}
+
+struct Vecs {            // weight and bias (either may be missing) in one of the three types
+    const void *w, *b;
+    int dtype;
+};
+__device__ inline float vec_at(const void *p, int dtype, int c, float missing)
+{
+    if (!p) return missing;
+    if (dtype == TEF_F32) return reinterpret_cast<const float *>(p)[c];
+    if (dtype == TEF_F16) return __half2float(reinterpret_cast<const __half *>(p)[c]);
+    return __bfloat162float(reinterpret_cast<const __hip_bfloat16 *>(p)[c]);
+}
+__device__ inline void vec_put(void *p, int dtype, int c, float v)
+{
+    if (dtype == TEF_F32) reinterpret_cast<float *>(p)[c] = v;
+    else if (dtype == TEF_F16) reinterpret_cast<__half *>(p)[c] = __float2half(v);
+    else reinterpret_cast<__hip_bfloat16 *>(p)[c] = __float2bfloat16(v);
+}
+
+__device__ inline float act(int a, float z)
+{
+    if (a == TEF_ACT_NONE) return z;
+    if (a == TEF_ACT_RELU) return z > 0.0f || z != z ? z : 0.0f;      // (NaN stays NaN)
+    if (a == TEF_ACT_TANH) return tanhf(z);
+    return 1.0f / (1.0f + expf(-z));
+}
+__device__ inline float act_slope(int a, float z)
+{
+    if (a == TEF_ACT_NONE) return 1.0f;
+    if (a == TEF_ACT_RELU) return z > 0.0f ? 1.0f : z != z ? z : 0.0f;
+    if (a == TEF_ACT_TANH) { const float y = tanhf(z); return 1.0f - y * y; }
+    const float y = 1.0f / (1.0f + expf(-z));
+    return y * (1.0f - y);
+}
+
+struct Args {
+    const void *x, *res, *dy;
+    void *y, *dx, *dres;
+    float *mean, *rstd, *part;       // part: [workgroups][2][C] partial sums of dweight, dbias
+    Vecs v;
+    long rows;                       // outer * inner
+    long inner;
+    int C, act;
+    float eps;
+};
+
+// ---- rows: C contiguous --------------------------------------------------------------------------------------------------
+// A row belongs to L lanes (a power of two, at most one wave: no barrier, several short rows a wave) or, WG, to the whole
+// workgroup.  Lane l holds the elements V * (l + L * i) .. + V - 1, i < NV, in registers.
+constexpr int V = 4;
+
+template <bool WG> __device__ inline float row_sum(float s, int L, float *red)
+{
+    for (int o = (WG ? 64 : L) >> 1; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if (WG) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+        __syncthreads();
+        s = (red[0] + red[1]) + (red[2] + red[3]);
+    }
+    return s;
+}
+
+template <typename T, int NV, bool WG> __global__ __launch_bounds__(kThreads) void rows_fwd(Args a, int L)
+{
+    __shared__ float red[kThreads / 64];
+    const int l = WG ? threadIdx.x : threadIdx.x & (L - 1), per = WG ? 1 : kThreads / L;
+    const float inv = 1.0f / (float)a.C;
+    for (long r0 = (long)blockIdx.x * per; r0 < a.rows; r0 += (long)gridDim.x * per) {
+        const long r = WG ? r0 : r0 + threadIdx.x / L;
+        const bool live = r < a.rows;
+        const T *x = reinterpret_cast<const T *>(a.x) + (live ? r : 0) * a.C;
+        float f[NV][V], s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = V * (l + L * i);
+            load_n<T, V>(x + c, live ? a.C - c : 0, f[i]);
+            s += (f[i][0] + f[i][1]) + (f[i][2] + f[i][3]);
+        }
+        const float mean = row_sum<WG>(s, L, red) * inv;
+        float q = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                f[i][k] -= mean;
+                if (V * (l + L * i) + k < a.C) q += f[i][k] * f[i][k];
+            }
+        const float rstd = 1.0f / sqrtf(row_sum<WG>(q, L, red) * inv + a.eps);
+        if (live && l == 0 && a.mean) { a.mean[r] = mean; a.rstd[r] = rstd; }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = V * (l + L * i), n = live ? a.C - c : 0;
+            if (n <= 0) continue;
+            float e[V] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (a.res) load_n<T, V>(reinterpret_cast<const T *>(a.res) + r * a.C + c, n, e);
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+                if (k < n) e[k] = act(a.act, f[i][k] * rstd * vec_at(a.v.w, a.v.dtype, c + k, 1.0f) + vec_at(a.v.b, a.v.dtype, c + k, 0.0f) + e[k]);
+            store_n<T, V>(reinterpret_cast<T *>(a.y) + r * a.C + c, n, e);
+        }
+    }
+}
+
+template <typename T, int NV, bool WG> __global__ __launch_bounds__(kThreads) void rows_bwd(Args a, int L)
+{
+    __shared__ float red[kThreads / 64];
+    __shared__ float cols[WG ? 1 : kThreads * V];
+    const int l = WG ? threadIdx.x : threadIdx.x & (L - 1), per = WG ? 1 : kThreads / L;
+    const float inv = 1.0f / (float)a.C;
+    const bool need_z = a.act != TEF_ACT_NONE;
+    float w[NV][V], b[NV][V], dw[NV][V], db[NV][V];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const int c = V * (l + L * i) + k;
+            w[i][k] = c < a.C ? vec_at(a.v.w, a.v.dtype, c, 1.0f) : 0.0f;
+            b[i][k] = c < a.C && need_z ? vec_at(a.v.b, a.v.dtype, c, 0.0f) : 0.0f;
+            dw[i][k] = db[i][k] = 0.0f;
+        }
+    for (long r0 = (long)blockIdx.x * per; r0 < a.rows; r0 += (long)gridDim.x * per) {
+        const long r = WG ? r0 : r0 + threadIdx.x / L;
+        const bool live = r < a.rows;
+        const long at = (live ? r : 0) * a.C;
+        const float mean = live ? a.mean[r] : 0.0f, rstd = live ? a.rstd[r] : 0.0f;
+        float u[NV][V], h[NV][V], s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = V * (l + L * i), n = live ? a.C - c : 0;
+            load_n<T, V>(reinterpret_cast<const T *>(a.x) + at + c, n, u[i]);
+            load_n<T, V>(reinterpret_cast<const T *>(a.dy) + at + c, n, h[i]);
+            float e[V] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (need_z && a.res) load_n<T, V>(reinterpret_cast<const T *>(a.res) + at + c, n, e);
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                u[i][k] = k < n ? (u[i][k] - mean) * rstd : 0.0f;
+                float g = h[i][k];
+                if (need_z && k < n) g *= act_slope(a.act, u[i][k] * w[i][k] + b[i][k] + e[k]);
+                e[k] = g;
+                dw[i][k] += g * u[i][k];
+                db[i][k] += g;
+                h[i][k] = g * w[i][k];
+                s1 += h[i][k];
+                s2 += h[i][k] * u[i][k];
+            }
+            if (a.dres) store_n<T, V>(reinterpret_cast<T *>(a.dres) + at + c, n, e);
+        }
+        if (!a.dx) continue;
+        s1 = row_sum<WG>(s1, L, red) * inv;
+        s2 = row_sum<WG>(s2, L, red) * inv;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = V * (l + L * i), n = live ? a.C - c : 0;
+            float e[V];
+#pragma unroll
+            for (int k = 0; k < V; ++k) e[k] = rstd * (h[i][k] - s1 - u[i][k] * s2);
+            store_n<T, V>(reinterpret_cast<T *>(a.dx) + at + c, n, e);
+        }
+    }
+    if (!a.part) return;
+    float *part = a.part + (long)blockIdx.x * 2 * a.C;
+    for (int which = 0; which < 2; ++which)
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float *acc = which ? db[i] : dw[i];
+            const int c = V * (l + L * i);
+            if (WG) {
+#pragma unroll
+                for (int k = 0; k < V; ++k)
+                    if (c + k < a.C) part[which * a.C + c + k] = acc[k];
+            } else {      // the row groups of the workgroup, in order
+                __syncthreads();
+#pragma unroll
+                for (int k = 0; k < V; ++k) cols[threadIdx.x * V + k] = acc[k];
+                __syncthreads();
+                if ((int)threadIdx.x < L)
+#pragma unroll
+                    for (int k = 0; k < V; ++k) {
+                        float s = 0.0f;
+                        for (int g = 0; g < per; ++g) s += cols[(g * L + l) * V + k];
+                        if (c + k < a.C) part[which * a.C + c + k] = s;
+                    }
+            }
+        }
+}
+
+// ---- maps: the channels of a position lie `inner` elements apart --------------------------------------------------------
+// A workgroup takes LX * P neighbouring positions (P per lane: 4 when inner is a multiple of 4, so that a lane's positions
+// are one load; else 1) and all channels: lane group g of G = 256 / LX holds the channels g, g + G, ... in registers.
+template <int P> __device__ inline void map_sum(float (&s)[P], int LX, float *red)      // over the lane groups
+{
+    const int lx = threadIdx.x & (LX - 1), wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int k = 0; k < P; ++k)
+        for (int o = 32; o >= LX; o >>= 1) s[k] += __shfl_xor(s[k], o, 64);
+    __syncthreads();
+    if ((int)(threadIdx.x & 63) < LX)
+#pragma unroll
+        for (int k = 0; k < P; ++k) red[(wave * LX + lx) * P + k] = s[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < P; ++k)
+        s[k] = (red[lx * P + k] + red[(LX + lx) * P + k]) + (red[(2 * LX + lx) * P + k] + red[(3 * LX + lx) * P + k]);
+}
+
+template <typename T, int NC, int P> __global__ __launch_bounds__(kThreads) void maps_fwd(Args a, int LX)
+{
+    __shared__ float red[4 * 64 * P];
+    const int lx = threadIdx.x & (LX - 1), g = threadIdx.x / LX, G = kThreads / LX;
+    const float inv = 1.0f / (float)a.C;
+    const long tile = (long)LX * P;
+    for (long t = blockIdx.x; t * tile < a.rows; t += gridDim.x) {
+        const long pos = t * tile + (long)lx * P;
+        const bool live = pos < a.rows;
+        const long o = live ? pos / a.inner : 0, at = live ? o * a.C * a.inner + (pos - o * a.inner) : 0;
+        const T *x = reinterpret_cast<const T *>(a.x) + at;
+        float f[NC][P], s[P], q[P];
+#pragma unroll
+        for (int k = 0; k < P; ++k) s[k] = q[k] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const int c = g + G * i;
+            load_n<T, P>(x + (long)c * a.inner, live && c < a.C ? P : 0, f[i]);
+#pragma unroll
+            for (int k = 0; k < P; ++k) s[k] += f[i][k];
+        }
+        map_sum<P>(s, LX, red);
+#pragma unroll
+        for (int k = 0; k < P; ++k) s[k] *= inv;
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+#pragma unroll
+            for (int k = 0; k < P; ++k) {
+                f[i][k] -= s[k];
+                if (g + G * i < a.C) q[k] += f[i][k] * f[i][k];
+            }
+        map_sum<P>(q, LX, red);
+#pragma unroll
+        for (int k = 0; k < P; ++k) q[k] = 1.0f / sqrtf(q[k] * inv + a.eps);
+        if (!live) continue;
+        if (a.mean && g == 0) { store<float, P>(a.mean + pos, s); store<float, P>(a.rstd + pos, q); }
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const int c = g + G * i;
+            if (c >= a.C) continue;
+            const float w = vec_at(a.v.w, a.v.dtype, c, 1.0f), b = vec_at(a.v.b, a.v.dtype, c, 0.0f);
+            float e[P];
+#pragma unroll
+            for (int k = 0; k < P; ++k) e[k] = 0.0f;
+            if (a.res) load<T, P>(reinterpret_cast<const T *>(a.res) + at + (long)c * a.inner, e);
+#pragma unroll
+            for (int k = 0; k < P; ++k) e[k] = act(a.act, f[i][k] * q[k] * w + b + e[k]);
+            store<T, P>(reinterpret_cast<T *>(a.y) + at + (long)c * a.inner, e);
+        }
+    }
+}
+
+template <typename T, int NC, int P> __global__ __launch_bounds__(kThreads) void maps_bwd(Args a, int LX)
+{
+    __shared__ float red[4 * 64 * P];
+    const int lx = threadIdx.x & (LX - 1), g = threadIdx.x / LX, G = kThreads / LX;
+    const float inv = 1.0f / (float)a.C;
+    const bool need_z = a.act != TEF_ACT_NONE;
+    const long tile = (long)LX * P;
+    float dw[NC], db[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) dw[i] = db[i] = 0.0f;
+    for (long t = blockIdx.x; t * tile < a.rows; t += gridDim.x) {
+        const long pos = t * tile + (long)lx * P;
+        const bool live = pos < a.rows;
+        const long o = live ? pos / a.inner : 0, at = live ? o * a.C * a.inner + (pos - o * a.inner) : 0;
+        float mean[P], rstd[P], u[NC][P], h[NC][P], s1[P], s2[P];
+        load_n<float, P>(a.mean + (live ? pos : 0), live ? P : 0, mean);
+        load_n<float, P>(a.rstd + (live ? pos : 0), live ? P : 0, rstd);
+#pragma unroll
+        for (int k = 0; k < P; ++k) s1[k] = s2[k] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const int c = g + G * i, n = live && c < a.C ? P : 0;
+            const long off = at + (long)c * a.inner;
+            load_n<T, P>(reinterpret_cast<const T *>(a.x) + off, n, u[i]);
+            load_n<T, P>(reinterpret_cast<const T *>(a.dy) + off, n, h[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const int c = g + G * i;
+            const bool in = live && c < a.C;
+            const long off = at + (long)c * a.inner;
+            const float w = in ? vec_at(a.v.w, a.v.dtype, c, 1.0f) : 0.0f;
+            float e[P];
+#pragma unroll
+            for (int k = 0; k < P; ++k) { e[k] = 0.0f; u[i][k] = in ? (u[i][k] - mean[k]) * rstd[k] : 0.0f; }
+            if (need_z && in) {
+                const float b = vec_at(a.v.b, a.v.dtype, c, 0.0f);
+                if (a.res) load<T, P>(reinterpret_cast<const T *>(a.res) + off, e);
+#pragma unroll
+                for (int k = 0; k < P; ++k) h[i][k] *= act_slope(a.act, u[i][k] * w + b + e[k]);
+            }
+            if (a.dres && in) store<T, P>(reinterpret_cast<T *>(a.dres) + off, h[i]);
+#pragma unroll
+            for (int k = 0; k < P; ++k) {
+                dw[i] += h[i][k] * u[i][k];
+                db[i] += h[i][k];
+                h[i][k] *= w;
+                s1[k] += h[i][k];
+                s2[k] += h[i][k] * u[i][k];
+            }
+        }
+        if (!a.dx) continue;
+        map_sum<P>(s1, LX, red);
+        map_sum<P>(s2, LX, red);
+        if (!live) continue;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const int c = g + G * i;
+            if (c >= a.C) continue;
+            float e[P];
+#pragma unroll
+            for (int k = 0; k < P; ++k) e[k] = rstd[k] * (h[i][k] - s1[k] * inv - u[i][k] * (s2[k] * inv));
+            store<T, P>(reinterpret_cast<T *>(a.dx) + at + (long)c * a.inner, e);
+        }
+    }
+    if (!a.part) return;
+    float *part = a.part + (long)blockIdx.x * 2 * a.C;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        for (int o2 = LX >> 1; o2 > 0; o2 >>= 1) {
+            dw[i] += __shfl_xor(dw[i], o2, 64);
+            db[i] += __shfl_xor(db[i], o2, 64);
+        }
+        const int c = g + G * i;
+        if (lx == 0 && c < a.C) { part[c] = dw[i]; part[a.C + c] = db[i]; }
+    }
+}
+
+// ---- any C: one workgroup per position, the row read again for every sum ------------------------------------------------
+// For rows and channel counts that do not fit into the registers of a workgroup.
+template <typename T> __global__ __launch_bounds__(kThreads) void long_fwd(Args a)
+{
+    __shared__ float red[kThreads / 64];
+    const float inv = 1.0f / (float)a.C;
+    for (long r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const long o = r / a.inner, at = o * a.C * a.inner + (r - o * a.inner);
+        const T *x = reinterpret_cast<const T *>(a.x) + at;
+        float s = 0.0f, q = 0.0f;
+        for (int c = threadIdx.x; c < a.C; c += kThreads) s += to_f<T>(x[(long)c * a.inner]);
+        const float mean = row_sum<true>(s, 64, red) * inv;
+        for (int c = threadIdx.x; c < a.C; c += kThreads) {
+            const float d = to_f<T>(x[(long)c * a.inner]) - mean;
+            q += d * d;
+        }
+        const float rstd = 1.0f / sqrtf(row_sum<true>(q, 64, red) * inv + a.eps);
+        if (threadIdx.x == 0 && a.mean) { a.mean[r] = mean; a.rstd[r] = rstd; }
+        for (int c = threadIdx.x; c < a.C; c += kThreads) {
+            const long off = at + (long)c * a.inner;
+            const float e = a.res ? to_f<T>(reinterpret_cast<const T *>(a.res)[off]) : 0.0f;
+            const float z = (to_f<T>(reinterpret_cast<const T *>(a.x)[off]) - mean) * rstd * vec_at(a.v.w, a.v.dtype, c, 1.0f) +
+                            vec_at(a.v.b, a.v.dtype, c, 0.0f) + e;
+            reinterpret_cast<T *>(a.y)[off] = from_f<T>(act(a.act, z));
+        }
+    }
+}
+
+template <typename T> __device__ inline float long_g(const Args &a, long off, int c, float mean, float rstd, float *u)
+{
+    *u = (to_f<T>(reinterpret_cast<const T *>(a.x)[off]) - mean) * rstd;
+    float g = to_f<T>(reinterpret_cast<const T *>(a.dy)[off]);
+    if (a.act != TEF_ACT_NONE) {
+        const float e = a.res ? to_f<T>(reinterpret_cast<const T *>(a.res)[off]) : 0.0f;
+        g *= act_slope(a.act, *u * vec_at(a.v.w, a.v.dtype, c, 1.0f) + vec_at(a.v.b, a.v.dtype, c, 0.0f) + e);
+    }
+    return g;
+}
+
+template <typename T> __global__ __launch_bounds__(kThreads) void long_bwd(Args a)
+{
+    __shared__ float red[kThreads / 64];
+    const float inv = 1.0f / (float)a.C;
+    for (long r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const long o = r / a.inner, at = o * a.C * a.inner + (r - o * a.inner);
+        const float mean = a.mean[r], rstd = a.rstd[r];
+        float s1 = 0.0f, s2 = 0.0f, u;
+        for (int c = threadIdx.x; c < a.C; c += kThreads) {
+            const long off = at + (long)c * a.inner;
+            const float g = long_g<T>(a, off, c, mean, rstd, &u), h = g * vec_at(a.v.w, a.v.dtype, c, 1.0f);
+            s1 += h;
+            s2 += h * u;
+            if (a.dres) reinterpret_cast<T *>(a.dres)[off] = from_f<T>(g);
+            if (a.part) {      // this thread is the only one of the workgroup at channel c
+                float *p = a.part + (long)blockIdx.x * 2 * a.C + c;
+                const bool first = r == (long)blockIdx.x;
+                p[0] = (first ? 0.0f : p[0]) + g * u;
+                p[a.C] = (first ? 0.0f : p[a.C]) + g;
+            }
+        }
+        if (!a.dx) continue;
+        s1 = row_sum<true>(s1, 64, red) * inv;
+        s2 = row_sum<true>(s2, 64, red) * inv;
+        for (int c = threadIdx.x; c < a.C; c += kThreads) {
+            const long off = at + (long)c * a.inner;
+            const float h = long_g<T>(a, off, c, mean, rstd, &u) * vec_at(a.v.w, a.v.dtype, c, 1.0f);
+            reinterpret_cast<T *>(a.dx)[off] = from_f<T>(rstd * (h - s1 - u * s2));
+        }
+    }
+}
+
+// dweight / dbias = the sum of the workgroups' partial rows: 64 columns a workgroup, 4 waves that each take every fourth row,
+// four running sums a lane (fixed order).
+__global__ __launch_bounds__(kThreads) void norm_join(const float *__restrict__ part, int parts, int C, void *dw, void *db, int dtype)
+{
+    __shared__ float red[kThreads];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.x * 64 + lane;
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (col < 2 * C) {
+        int k = wave;
+        for (; k + 12 < parts; k += 16)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[j] += part[(long)(k + 4 * j) * 2 * C + col];
+        for (int j = 0; k < parts; k += 4, ++j) s[j] += part[(long)k * 2 * C + col];
+    }
+    red[threadIdx.x] = (s[0] + s[1]) + (s[2] + s[3]);
+    __syncthreads();
+    if (wave == 0 && col < 2 * C) {
+        const float v = (red[lane] + red[64 + lane]) + (red[128 + lane] + red[192 + lane]);
+        if (col < C) { if (dw) vec_put(dw, dtype, col, v); }
+        else if (db) vec_put(db, dtype, col - C, v);
+    }
+}
+
+__global__ __launch_bounds__(kThreads) void norm_zero(void *dw, void *db, int C, int dtype)
+{
+    const int c = blockIdx.x * kThreads + threadIdx.x;
+    if (c >= C) return;
+    if (dw) vec_put(dw, dtype, c, 0.0f);
+    if (db) vec_put(db, dtype, c, 0.0f);
+}
+
+// How a description is cut: which kernel, its register blocking, its grid.
+struct Plan {
+    int kind;          // 0 rows (lanes of a wave), 1 rows (workgroup), 2 maps, 3 long
+    int n;             // NV or NC
+    int lanes;         // L or LX
+    int per;           // P (maps)
+    long tiles;
+};
+
+inline int pow2_at_least(long v)
+{
+    int p = 1;
+    while (p < v) p <<= 1;
+    return p;
+}
+
+Plan make_plan(const tef_norm_desc &d)
+{
+    Plan p{};
+    const long rows = (long)d.outer * d.inner;
+    if (d.inner == 1) {
+        const long packs = (d.channels + V - 1) / V;
+        if (packs <= 64 * 8) {
+            p.kind = 0;
+            p.lanes = packs < 64 ? pow2_at_least(packs) : 64;
+            p.n = pow2_at_least((packs + p.lanes - 1) / p.lanes);
+            p.tiles = (rows + kThreads / p.lanes - 1) / (kThreads / p.lanes);
+            return p;
+        }
+        if (packs <= kThreads * 8) {
+            p.kind = 1;
+            p.lanes = kThreads;
+            p.n = pow2_at_least((packs + kThreads - 1) / kThreads);
+            p.tiles = rows;
+            return p;
+        }
+    } else {
+        p.per = d.inner % 4 == 0 ? 4 : 1;
+        // as many lanes along the positions as leave a thread at most 64 values (long runs of memory per channel), then
+        // fewer while the grid does not cover the 256 CUs twice
+        const int most = 64 / p.per;
+        int lx = p.per == 4 ? 16 : 64;
+        while (lx > 4 && (d.channels + kThreads / lx - 1) / (kThreads / lx) > most) lx >>= 1;
+        while (lx > 4 && (rows + lx * p.per - 1) / (lx * p.per) < 512 && (long)d.channels * lx > kThreads) lx >>= 1;
+        const int nc = (d.channels + kThreads / lx - 1) / (kThreads / lx);
+        if (nc <= most) {
+            p.kind = 2;
+            p.lanes = lx;
+            p.n = pow2_at_least(nc);
+            p.tiles = (rows + (long)lx * p.per - 1) / ((long)lx * p.per);
+            return p;
+        }
+    }
+    p.kind = 3;
+    p.tiles = rows;
+    return p;
+}
+
+template <typename T, int N> void go_n(const Plan &p, bool bwd, dim3 grid, hipStream_t st, const Args &a)
+{
+    const dim3 block(kThreads);
+    if (p.kind == 0) {
+        if constexpr (N <= 8) {
+            if (bwd) hipLaunchKernelGGL((rows_bwd<T, N, false>), grid, block, 0, st, a, p.lanes);
+            else hipLaunchKernelGGL((rows_fwd<T, N, false>), grid, block, 0, st, a, p.lanes);
+        }
+    } else if (p.kind == 1) {
+        if constexpr (N <= 8 && N > 1) {
+            if (bwd) hipLaunchKernelGGL((rows_bwd<T, N, true>), grid, block, 0, st, a, p.lanes);
+            else hipLaunchKernelGGL((rows_fwd<T, N, true>), grid, block, 0, st, a, p.lanes);
+        }
+    } else if (p.per == 4) {
+        if constexpr (N <= 16) {
+            if (bwd) hipLaunchKernelGGL((maps_bwd<T, N, 4>), grid, block, 0, st, a, p.lanes);
+            else hipLaunchKernelGGL((maps_fwd<T, N, 4>), grid, block, 0, st, a, p.lanes);
+        }
+    } else {
+        if (bwd) hipLaunchKernelGGL((maps_bwd<T, N, 1>), grid, block, 0, st, a, p.lanes);
+        else hipLaunchKernelGGL((maps_fwd<T, N, 1>), grid, block, 0, st, a, p.lanes);
+    }
+}
+
+template <typename T> void go(const Plan &p, bool bwd, dim3 grid, hipStream_t st, const Args &a)
+{
+    if (p.kind == 3) {
+        if (bwd) hipLaunchKernelGGL(long_bwd<T>, grid, dim3(kThreads), 0, st, a);
+        else hipLaunchKernelGGL(long_fwd<T>, grid, dim3(kThreads), 0, st, a);
+        return;
+    }
+    switch (p.n) {
+    case 1: go_n<T, 1>(p, bwd, grid, st, a); break;
+    case 2: go_n<T, 2>(p, bwd, grid, st, a); break;
+    case 4: go_n<T, 4>(p, bwd, grid, st, a); break;
+    case 8: go_n<T, 8>(p, bwd, grid, st, a); break;
+    case 16: go_n<T, 16>(p, bwd, grid, st, a); break;
+    case 32: go_n<T, 32>(p, bwd, grid, st, a); break;
+    default: go_n<T, 64>(p, bwd, grid, st, a); break;
+    }
+}
+
+void launch(const tef_norm_desc &d, const Plan &p, bool bwd, unsigned blocks, hipStream_t st, const Args &a)
+{
+    const dim3 grid(blocks);
+    if (d.dtype == TEF_F32) go<float>(p, bwd, grid, st, a);
+    else if (d.dtype == TEF_F16) go<__half>(p, bwd, grid, st, a);
+    else go<__hip_bfloat16>(p, bwd, grid, st, a);
+}
+
+unsigned bwd_blocks(const Plan &p) { return (unsigned)(p.tiles < kMaxBlocks ? p.tiles : kMaxBlocks); }
+
+bool valid(const tef_norm_desc *d)
+{
+    if (!d) return tef::fail("layer norm: null description");
+    const bool ok = d->channels >= 1 && d->outer >= 0 && d->inner >= 1 && d->dtype >= TEF_F32 && d->dtype <= TEF_BF16 &&
+                    (d->wdtype == TEF_F32 || d->wdtype == d->dtype) && d->act >= TEF_ACT_NONE && d->act <= TEF_ACT_SIGMOID &&
+                    d->eps >= 0.0f && d->eps < 1e30f;
+    if (!ok) return tef::fail("layer norm: invalid description (sizes, types, activation or eps)");
+    const double n = (double)d->outer * (double)d->inner * (double)d->channels;
+    if (n > 4e18) return tef::fail("layer norm: more elements than 64-bit offsets can address");
+    return true;
+}
+
+}  // namespace
+
+extern "C" {
+
+int tef_layer_norm_forward(const tef_norm_desc *d, const void *x, const void *weight, const void *bias, const void *residual,
+                           void *y, float *mean, float *rstd, void *stream)
+{
+    if (!valid(d)) return TEF_ERR_INVALID;
+    if (d->outer == 0) return 0;
+    if (!x || !y || (!mean != !rstd)) return tef::fail("tef_layer_norm_forward: null pointer"), TEF_ERR_INVALID;
+    const Plan p = make_plan(*d);
+    Args a{};
+    a.x = x; a.res = residual; a.y = y; a.mean = mean; a.rstd = rstd;
+    a.v = Vecs{weight, bias, d->wdtype};
+    a.rows = (long)d->outer * d->inner; a.inner = d->inner; a.C = d->channels; a.act = d->act; a.eps = d->eps;
+    const long most = 1l << 20;      // (the kernels stride over what a grid of that size leaves)
+    launch(*d, p, false, (unsigned)(p.tiles < most ? p.tiles : most), (hipStream_t)stream, a);
+    return tef::check_launch("layer norm forward");
+}
+
+size_t tef_layer_norm_workspace_bytes(const tef_norm_desc *d)
+{
+    if (!valid(d)) return 0;
+    if (d->outer == 0) return 16;
+    return (size_t)bwd_blocks(make_plan(*d)) * 2 * (size_t)d->channels * sizeof(float);
+}
+
+int tef_layer_norm_backward(const tef_norm_desc *d, const void *x, const void *weight, const void *bias, const void *residual,
+                            const float *mean, const float *rstd, const void *dy, void *dx, void *dresidual, void *dweight,
+                            void *dbias, void *workspace, size_t workspace_bytes, void *stream)
+{
+    if (!valid(d)) return TEF_ERR_INVALID;
+    hipStream_t st = (hipStream_t)stream;
+    if (d->outer == 0) {      // no rows: the sums over rows are zero
+        if (dweight || dbias)
+            hipLaunchKernelGGL(norm_zero, dim3((unsigned)((d->channels + kThreads - 1) / kThreads)), dim3(kThreads), 0, st, dweight, dbias, d->channels, d->wdtype);
+        return tef::check_launch("layer norm backward");
+    }
+    if (!x || !mean || !rstd || !dy) return tef::fail("tef_layer_norm_backward: null pointer"), TEF_ERR_INVALID;
+    const bool sums = dweight || dbias;
+    if (!dx && !dresidual && !sums) return 0;
+    if (sums && (!workspace || workspace_bytes < tef_layer_norm_workspace_bytes(d)))
+        return tef::fail("tef_layer_norm_backward: workspace too small"), TEF_ERR_WORKSPACE;
+    const Plan p = make_plan(*d);
+    Args a{};
+    a.x = x; a.res = residual; a.dy = dy; a.dx = dx; a.dres = dresidual;
+    a.mean = const_cast<float *>(mean); a.rstd = const_cast<float *>(rstd);
+    a.part = sums ? (float *)workspace : nullptr;
+    a.v = Vecs{weight, bias, d->wdtype};
+    a.rows = (long)d->outer * d->inner; a.inner = d->inner; a.C = d->channels; a.act = d->act; a.eps = d->eps;
+    const unsigned blocks = bwd_blocks(p);
+    launch(*d, p, true, blocks, st, a);
+    if (sums)
+        hipLaunchKernelGGL(norm_join, dim3((unsigned)((2l * d->channels + 63) / 64)), dim3(kThreads), 0, st, (const float *)workspace, (int)blocks,
+                           d->channels, dweight, dbias, d->wdtype);
+    return tef::check_launch("layer norm backward");
+}
+
+}  // extern "C"

@@ -17,6 +17,8 @@ try:
 except ImportError:      # drop-in mode: this package's directory itself is on sys.path
     import _lib
 
+from .norm import LayerNorm
+
 
 def _ptr(t):
     return t.data_ptr() if t is not None else None
@@ -370,9 +372,15 @@ def _act_name(activation):
     return activation
 
 
-def _no_norm(norm):
-    if norm is not None:
-        raise NotImplementedError("norm layers are unused by RecEVFlowNet (norm=None, reference models/model.py:28)")
+def _norm_layer(norm, channels):
+    """The normalisation between a convolution and its activation: None, or the channels of every position ("LN"); the
+    reference's "BN" / "IN" are not built."""
+    if norm is None:
+        return None
+    if norm != "LN":
+        raise NotImplementedError(f"norm={norm!r}: RecEVFlowNet uses norm=None (reference models/model.py:28); \"LN\" is the other "
+                                  "normalisation built here")
+    return LayerNorm(channels)
 
 
 class ConvLayer(nn.Module):
@@ -381,7 +389,7 @@ class ConvLayer(nn.Module):
     def __init__(self, in_channels, out_channels, kernel_size, stride=1, activation="relu", norm=None,
                  BN_momentum=0.1, w_scale=None, padding=None, bias=None):
         super().__init__()
-        _no_norm(norm)
+        norm_layer = _norm_layer(norm, out_channels)
         if padding is not None and padding != kernel_size // 2:
             raise NotImplementedError("only padding = kernel_size // 2 is implemented")
         if bias is None:
@@ -395,10 +403,15 @@ class ConvLayer(nn.Module):
         self.activation = _act_name(activation)
         self.stride = stride
         self.norm = norm
+        if norm_layer is not None:
+            self.norm_layer = norm_layer
         self._packed = PackedWeights()
 
     def forward(self, x):
-        return conv2d(self._packed, x, self.conv2d.weight, self.conv2d.bias, self.stride, self.activation)
+        if self.norm is None:
+            return conv2d(self._packed, x, self.conv2d.weight, self.conv2d.bias, self.stride, self.activation)
+        out = conv2d(self._packed, x, self.conv2d.weight, self.conv2d.bias, self.stride, None)
+        return self.norm_layer(out, activation=self.activation)
 
 
 class ConvGRU(nn.Module):
@@ -461,7 +474,7 @@ class ResidualBlock(nn.Module):
     def __init__(self, in_channels, out_channels, kernel_size=3, stride=1, activation="relu", downsample=None,
                  norm=None, BN_momentum=0.1):
         super().__init__()
-        _no_norm(norm)
+        norm1, norm2 = _norm_layer(norm, out_channels), _norm_layer(norm, out_channels)
         if downsample is not None:
             raise NotImplementedError("downsample is unused by RecEVFlowNet")
         self.conv1 = nn.Conv2d(in_channels, out_channels, kernel_size=kernel_size, stride=stride,
@@ -472,9 +485,15 @@ class ResidualBlock(nn.Module):
         self.stride = stride
         self.norm = norm
         self.downsample = downsample
+        if norm is not None:
+            self.norm1, self.norm2 = norm1, norm2
         self._packed1, self._packed2 = PackedWeights(), PackedWeights()
 
     def forward(self, x):
+        if self.norm is not None:      # the sum and the last activation ride on the second normalisation
+            out1 = self.norm1(conv2d(self._packed1, x, self.conv1.weight, self.conv1.bias, self.stride, None), activation=self.activation)
+            out2 = conv2d(self._packed2, out1, self.conv2.weight, self.conv2.bias, self.stride, None)
+            return self.norm2(out2, residual=x, activation=self.activation), out1
         out1 = conv2d(self._packed1, x, self.conv1.weight, self.conv1.bias, self.stride, self.activation)
         out2 = conv2d(self._packed2, out1, self.conv2.weight, self.conv2.bias, self.stride, None)
         out2 = out2 + x
@@ -488,11 +507,13 @@ class UpsampleConvLayer(nn.Module):
 
     def __init__(self, in_channels, out_channels, kernel_size, stride=1, activation="relu", norm=None):
         super().__init__()
-        _no_norm(norm)
+        norm_layer = _norm_layer(norm, out_channels)
         self.conv2d = nn.Conv2d(in_channels, out_channels, kernel_size, stride, kernel_size // 2, bias=True)
         self.activation = _act_name(activation)
         self.stride = stride
         self.norm = norm
+        if norm_layer is not None:
+            self.norm_layer = norm_layer
         self._packed = PackedWeights()
 
     def forward(self, x):
@@ -501,9 +522,12 @@ class UpsampleConvLayer(nn.Module):
     def conv_after_upsample(self, up, up_first=None):
         """The convolution on already up-sampled features; `up_first` supplies the leading input channels from a second
         tensor (the previous prediction, reference arch.py:238) without concatenating."""
+        act = self.activation if self.norm is None else None
         if up_first is None:
-            return conv2d(self._packed, up, self.conv2d.weight, self.conv2d.bias, self.stride, self.activation)
-        return conv2d(self._packed, up_first, self.conv2d.weight, self.conv2d.bias, self.stride, self.activation, x1=up)
+            out = conv2d(self._packed, up, self.conv2d.weight, self.conv2d.bias, self.stride, act)
+        else:
+            out = conv2d(self._packed, up_first, self.conv2d.weight, self.conv2d.bias, self.stride, act, x1=up)
+        return out if self.norm is None else self.norm_layer(out, activation=self.activation)
 
 
 class TransposedConvLayer(nn.Module):
