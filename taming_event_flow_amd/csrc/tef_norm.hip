@@ -41,12 +41,7 @@ template <> __device__ inline __hip_bfloat16 from_f<__hip_bfloat16>(float v) { r
 // V consecutive elements; the address is a multiple of the ELEMENT's size only (views, odd row lengths): gfx950's global
 // loads take that, in one instruction.
 template <typename T, int V> struct __attribute__((packed, aligned(sizeof(T)))) Pack { T v[V]; };
-template <typename T, int V> __device__ inline void load(const T *p, float (&f)[V])
-{
-    const Pack<T, V> q = *reinterpret_cast<const Pack<T, V> *>(p);
-#pragma unroll
-    for (int k = 0; k < V; ++k) f[k] = to_f<T>(q.v[k]);
-}
+template <typename T, int V> __device__ inline Pack<T, V> raw(const T *p) { return *reinterpret_cast<const Pack<T, V> *>(p); }
 template <typename T, int V> __device__ inline void store(T *p, const float (&f)[V])
 {
     Pack<T, V> q;
@@ -54,19 +49,25 @@ template <typename T, int V> __device__ inline void store(T *p, const float (&f)
     for (int k = 0; k < V; ++k) q.v[k] = from_f<T>(f[k]);
     *reinterpret_cast<Pack<T, V> *>(p) = q;
 }
-// the first n of V elements (n >= V: all of them; n <= 0: none), the rest 0
-template <typename T, int V> __device__ inline void load_n(const T *p, int n, float (&f)[V])
+// Elements c .. c + V - 1 of a row of C: no branch around the load, so that all packs of a row are in flight together — what
+// lies past the row's end is read at its last element and set to 0 by the caller.  EVEN: C is a multiple of V.
+template <typename T, int V, bool EVEN> __device__ inline Pack<T, V> raw_row(const T *row, int c, int C)
 {
-    if (n >= V) return load<T, V>(p, f);
+    if (EVEN) return raw<T, V>(row + (c < C ? c : C - V));
+    Pack<T, V> q;
 #pragma unroll
-    for (int k = 0; k < V; ++k) f[k] = k < n ? to_f<T>(p[k]) : 0.0f;
+    for (int k = 0; k < V; ++k) q.v[k] = row[c + k < C ? c + k : C - 1];
+    return q;
 }
-template <typename T, int V> __device__ inline void store_n(T *p, int n, const float (&f)[V])
+template <typename T, int V, bool EVEN> __device__ inline void store_row(T *row, int c, int C, const float (&f)[V])
 {
-    if (n >= V) return store<T, V>(p, f);
+    if (EVEN) {
+        if (c < C) store<T, V>(row + c, f);
+        return;
+    }
 #pragma unroll
     for (int k = 0; k < V; ++k)
-        if (k < n) p[k] = from_f<T>(f[k]);
+        if (c + k < C) row[c + k] = from_f<T>(f[k]);
 }
 
 struct Vecs {            // weight and bias (either may be missing) in one of the three types
@@ -116,7 +117,8 @@ struct Args {
 
 // ---- rows: C contiguous --------------------------------------------------------------------------------------------------
 // A row belongs to L lanes (a power of two, at most one wave: no barrier, several short rows a wave) or, WG, to the whole
-// workgroup.  Lane l holds the elements V * (l + L * i) .. + V - 1, i < NV, in registers.
+// workgroup.  Lane l holds the elements V * (l + L * i) .. + V - 1, i < NV, in registers, and keeps the weights of its
+// columns over all rows that it takes.
 constexpr int V = 4;
 
 template <bool WG> __device__ inline float row_sum(float s, int L, float *red)
@@ -131,82 +133,101 @@ template <bool WG> __device__ inline float row_sum(float s, int L, float *red)
     return s;
 }
 
-template <typename T, int NV, bool WG> __global__ __launch_bounds__(kThreads) void rows_fwd(Args a, int L)
+template <int NV> __device__ inline void row_vec(const void *p, int dtype, int l, int L, int C, float missing, float (&f)[NV][V])
 {
-    __shared__ float red[kThreads / 64];
-    const int l = WG ? threadIdx.x : threadIdx.x & (L - 1), per = WG ? 1 : kThreads / L;
-    const float inv = 1.0f / (float)a.C;
-    for (long r0 = (long)blockIdx.x * per; r0 < a.rows; r0 += (long)gridDim.x * per) {
-        const long r = WG ? r0 : r0 + threadIdx.x / L;
-        const bool live = r < a.rows;
-        const T *x = reinterpret_cast<const T *>(a.x) + (live ? r : 0) * a.C;
-        float f[NV][V], s = 0.0f;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = V * (l + L * i);
-            load_n<T, V>(x + c, live ? a.C - c : 0, f[i]);
-            s += (f[i][0] + f[i][1]) + (f[i][2] + f[i][3]);
-        }
-        const float mean = row_sum<WG>(s, L, red) * inv;
-        float q = 0.0f;
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                f[i][k] -= mean;
-                if (V * (l + L * i) + k < a.C) q += f[i][k] * f[i][k];
-            }
-        const float rstd = 1.0f / sqrtf(row_sum<WG>(q, L, red) * inv + a.eps);
-        if (live && l == 0 && a.mean) { a.mean[r] = mean; a.rstd[r] = rstd; }
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = V * (l + L * i), n = live ? a.C - c : 0;
-            if (n <= 0) continue;
-            float e[V] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (a.res) load_n<T, V>(reinterpret_cast<const T *>(a.res) + r * a.C + c, n, e);
-#pragma unroll
-            for (int k = 0; k < V; ++k)
-                if (k < n) e[k] = act(a.act, f[i][k] * rstd * vec_at(a.v.w, a.v.dtype, c + k, 1.0f) + vec_at(a.v.b, a.v.dtype, c + k, 0.0f) + e[k]);
-            store_n<T, V>(reinterpret_cast<T *>(a.y) + r * a.C + c, n, e);
-        }
-    }
-}
-
-template <typename T, int NV, bool WG> __global__ __launch_bounds__(kThreads) void rows_bwd(Args a, int L)
-{
-    __shared__ float red[kThreads / 64];
-    __shared__ float cols[WG ? 1 : kThreads * V];
-    const int l = WG ? threadIdx.x : threadIdx.x & (L - 1), per = WG ? 1 : kThreads / L;
-    const float inv = 1.0f / (float)a.C;
-    const bool need_z = a.act != TEF_ACT_NONE;
-    float w[NV][V], b[NV][V], dw[NV][V], db[NV][V];
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             const int c = V * (l + L * i) + k;
-            w[i][k] = c < a.C ? vec_at(a.v.w, a.v.dtype, c, 1.0f) : 0.0f;
-            b[i][k] = c < a.C && need_z ? vec_at(a.v.b, a.v.dtype, c, 0.0f) : 0.0f;
-            dw[i][k] = db[i][k] = 0.0f;
+            f[i][k] = vec_at(p, dtype, c < C ? c : C - 1, missing);
         }
+}
+
+template <typename T, int NV, bool WG, bool EVEN> __global__ __launch_bounds__(kThreads) void rows_fwd(Args a, int L)
+{
+    __shared__ float red[kThreads / 64];
+    const int l = WG ? threadIdx.x : threadIdx.x & (L - 1), per = WG ? 1 : kThreads / L, C = a.C;
+    const float inv = 1.0f / (float)C;
+    float w[NV][V], b[NV][V];
+    row_vec<NV>(a.v.w, a.v.dtype, l, L, C, 1.0f, w);
+    row_vec<NV>(a.v.b, a.v.dtype, l, L, C, 0.0f, b);
     for (long r0 = (long)blockIdx.x * per; r0 < a.rows; r0 += (long)gridDim.x * per) {
         const long r = WG ? r0 : r0 + threadIdx.x / L;
         const bool live = r < a.rows;
-        const long at = (live ? r : 0) * a.C;
-        const float mean = live ? a.mean[r] : 0.0f, rstd = live ? a.rstd[r] : 0.0f;
+        const long at = (live ? r : a.rows - 1) * C;
+        Pack<T, V> q[NV], e[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) q[i] = raw_row<T, V, EVEN>(reinterpret_cast<const T *>(a.x) + at, V * (l + L * i), C);
+        if (a.res)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) e[i] = raw_row<T, V, EVEN>(reinterpret_cast<const T *>(a.res) + at, V * (l + L * i), C);
+        float f[NV][V], s = 0.0f, v = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) f[i][k] = V * (l + L * i) + k < C ? to_f<T>(q[i].v[k]) : 0.0f;
+            s += (f[i][0] + f[i][1]) + (f[i][2] + f[i][3]);
+        }
+        const float mean = row_sum<WG>(s, L, red) * inv;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                f[i][k] -= mean;
+                v += V * (l + L * i) + k < C ? f[i][k] * f[i][k] : 0.0f;
+            }
+        const float rstd = 1.0f / sqrtf(row_sum<WG>(v, L, red) * inv + a.eps);
+        if (!live) continue;
+        if (l == 0 && a.mean) { a.mean[r] = mean; a.rstd[r] = rstd; }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+                f[i][k] = act(a.act, f[i][k] * rstd * w[i][k] + b[i][k] + (a.res ? to_f<T>(e[i].v[k]) : 0.0f));
+            store_row<T, V, EVEN>(reinterpret_cast<T *>(a.y) + at, V * (l + L * i), C, f[i]);
+        }
+    }
+}
+
+template <typename T, int NV, bool WG, bool EVEN> __global__ __launch_bounds__(kThreads) void rows_bwd(Args a, int L)
+{
+    __shared__ float red[kThreads / 64];
+    __shared__ float cols[WG ? 1 : kThreads * V];
+    const int l = WG ? threadIdx.x : threadIdx.x & (L - 1), per = WG ? 1 : kThreads / L, C = a.C;
+    const float inv = 1.0f / (float)C;
+    const bool need_z = a.act != TEF_ACT_NONE, need_e = need_z && a.res;
+    float w[NV][V], b[NV][V], dw[NV][V], db[NV][V];
+    row_vec<NV>(a.v.w, a.v.dtype, l, L, C, 1.0f, w);
+    row_vec<NV>(need_z ? a.v.b : nullptr, a.v.dtype, l, L, C, 0.0f, b);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < V; ++k) dw[i][k] = db[i][k] = 0.0f;
+    for (long r0 = (long)blockIdx.x * per; r0 < a.rows; r0 += (long)gridDim.x * per) {
+        const long r = WG ? r0 : r0 + threadIdx.x / L;
+        const bool live = r < a.rows;
+        const long row = live ? r : a.rows - 1, at = row * C;
+        Pack<T, V> qx[NV], qd[NV], qe[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            qx[i] = raw_row<T, V, EVEN>(reinterpret_cast<const T *>(a.x) + at, V * (l + L * i), C);
+            qd[i] = raw_row<T, V, EVEN>(reinterpret_cast<const T *>(a.dy) + at, V * (l + L * i), C);
+        }
+        if (need_e)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) qe[i] = raw_row<T, V, EVEN>(reinterpret_cast<const T *>(a.res) + at, V * (l + L * i), C);
+        const float mean = a.mean[row], rstd = a.rstd[row];
         float u[NV][V], h[NV][V], s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = V * (l + L * i), n = live ? a.C - c : 0;
-            load_n<T, V>(reinterpret_cast<const T *>(a.x) + at + c, n, u[i]);
-            load_n<T, V>(reinterpret_cast<const T *>(a.dy) + at + c, n, h[i]);
-            float e[V] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (need_z && a.res) load_n<T, V>(reinterpret_cast<const T *>(a.res) + at + c, n, e);
+            float e[V];
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                u[i][k] = k < n ? (u[i][k] - mean) * rstd : 0.0f;
-                float g = h[i][k];
-                if (need_z && k < n) g *= act_slope(a.act, u[i][k] * w[i][k] + b[i][k] + e[k]);
+                const bool in = live && V * (l + L * i) + k < C;
+                u[i][k] = in ? (to_f<T>(qx[i].v[k]) - mean) * rstd : 0.0f;
+                float g = in ? to_f<T>(qd[i].v[k]) : 0.0f;
+                if (need_z && in) g *= act_slope(a.act, u[i][k] * w[i][k] + b[i][k] + (need_e ? to_f<T>(qe[i].v[k]) : 0.0f));
                 e[k] = g;
                 dw[i][k] += g * u[i][k];
                 db[i][k] += g;
@@ -214,42 +235,41 @@ template <typename T, int NV, bool WG> __global__ __launch_bounds__(kThreads) vo
                 s1 += h[i][k];
                 s2 += h[i][k] * u[i][k];
             }
-            if (a.dres) store_n<T, V>(reinterpret_cast<T *>(a.dres) + at + c, n, e);
+            if (a.dres && live) store_row<T, V, EVEN>(reinterpret_cast<T *>(a.dres) + at, V * (l + L * i), C, e);
         }
         if (!a.dx) continue;
         s1 = row_sum<WG>(s1, L, red) * inv;
         s2 = row_sum<WG>(s2, L, red) * inv;
+        if (!live) continue;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = V * (l + L * i), n = live ? a.C - c : 0;
             float e[V];
 #pragma unroll
             for (int k = 0; k < V; ++k) e[k] = rstd * (h[i][k] - s1 - u[i][k] * s2);
-            store_n<T, V>(reinterpret_cast<T *>(a.dx) + at + c, n, e);
+            store_row<T, V, EVEN>(reinterpret_cast<T *>(a.dx) + at, V * (l + L * i), C, e);
         }
     }
     if (!a.part) return;
-    float *part = a.part + (long)blockIdx.x * 2 * a.C;
+    float *part = a.part + (long)blockIdx.x * 2 * C;
     for (int which = 0; which < 2; ++which)
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            float *acc = which ? db[i] : dw[i];
             const int c = V * (l + L * i);
             if (WG) {
 #pragma unroll
                 for (int k = 0; k < V; ++k)
-                    if (c + k < a.C) part[which * a.C + c + k] = acc[k];
+                    if (c + k < C) part[which * C + c + k] = which ? db[i][k] : dw[i][k];
             } else {      // the row groups of the workgroup, in order
                 __syncthreads();
 #pragma unroll
-                for (int k = 0; k < V; ++k) cols[threadIdx.x * V + k] = acc[k];
+                for (int k = 0; k < V; ++k) cols[threadIdx.x * V + k] = which ? db[i][k] : dw[i][k];
                 __syncthreads();
                 if ((int)threadIdx.x < L)
 #pragma unroll
                     for (int k = 0; k < V; ++k) {
                         float s = 0.0f;
                         for (int g = 0; g < per; ++g) s += cols[(g * L + l) * V + k];
-                        if (c + k < a.C) part[which * a.C + c + k] = s;
+                        if (c + k < C) part[which * C + c + k] = s;
                     }
             }
         }
@@ -277,24 +297,36 @@ template <int P> __device__ inline void map_sum(float (&s)[P], int LX, float *re
 template <typename T, int NC, int P> __global__ __launch_bounds__(kThreads) void maps_fwd(Args a, int LX)
 {
     __shared__ float red[4 * 64 * P];
-    const int lx = threadIdx.x & (LX - 1), g = threadIdx.x / LX, G = kThreads / LX;
-    const float inv = 1.0f / (float)a.C;
+    const int lx = threadIdx.x & (LX - 1), g = threadIdx.x / LX, G = kThreads / LX, C = a.C;
+    const float inv = 1.0f / (float)C;
     const long tile = (long)LX * P;
+    float w[NC], b[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        const int c = g + G * i < C ? g + G * i : C - 1;
+        w[i] = vec_at(a.v.w, a.v.dtype, c, 1.0f);
+        b[i] = vec_at(a.v.b, a.v.dtype, c, 0.0f);
+    }
     for (long t = blockIdx.x; t * tile < a.rows; t += gridDim.x) {
-        const long pos = t * tile + (long)lx * P;
-        const bool live = pos < a.rows;
-        const long o = live ? pos / a.inner : 0, at = live ? o * a.C * a.inner + (pos - o * a.inner) : 0;
-        const T *x = reinterpret_cast<const T *>(a.x) + at;
-        float f[NC][P], s[P], q[P];
+        const bool live = t * tile + (long)lx * P < a.rows;
+        const long pos = live ? t * tile + (long)lx * P : a.rows - P;
+        const long o = pos / a.inner, at = o * C * a.inner + (pos - o * a.inner);
+        Pack<T, P> q[NC], e[NC];
 #pragma unroll
-        for (int k = 0; k < P; ++k) s[k] = q[k] = 0.0f;
+        for (int i = 0; i < NC; ++i) q[i] = raw<T, P>(reinterpret_cast<const T *>(a.x) + at + (g + G * i < C ? g + G * i : C - 1) * a.inner);
+        if (a.res)
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            const int c = g + G * i;
-            load_n<T, P>(x + (long)c * a.inner, live && c < a.C ? P : 0, f[i]);
+            for (int i = 0; i < NC; ++i) e[i] = raw<T, P>(reinterpret_cast<const T *>(a.res) + at + (g + G * i < C ? g + G * i : C - 1) * a.inner);
+        float f[NC][P], s[P], v[P];
 #pragma unroll
-            for (int k = 0; k < P; ++k) s[k] += f[i][k];
-        }
+        for (int k = 0; k < P; ++k) s[k] = v[k] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+#pragma unroll
+            for (int k = 0; k < P; ++k) {
+                f[i][k] = to_f<T>(q[i].v[k]);
+                s[k] += g + G * i < C ? f[i][k] : 0.0f;
+            }
         map_sum<P>(s, LX, red);
 #pragma unroll
         for (int k = 0; k < P; ++k) s[k] *= inv;
@@ -303,25 +335,20 @@ template <typename T, int NC, int P> __global__ __launch_bounds__(kThreads) void
 #pragma unroll
             for (int k = 0; k < P; ++k) {
                 f[i][k] -= s[k];
-                if (g + G * i < a.C) q[k] += f[i][k] * f[i][k];
+                v[k] += g + G * i < C ? f[i][k] * f[i][k] : 0.0f;
             }
-        map_sum<P>(q, LX, red);
+        map_sum<P>(v, LX, red);
 #pragma unroll
-        for (int k = 0; k < P; ++k) q[k] = 1.0f / sqrtf(q[k] * inv + a.eps);
+        for (int k = 0; k < P; ++k) v[k] = 1.0f / sqrtf(v[k] * inv + a.eps);
         if (!live) continue;
-        if (a.mean && g == 0) { store<float, P>(a.mean + pos, s); store<float, P>(a.rstd + pos, q); }
+        if (a.mean && g == 0) { store<float, P>(a.mean + pos, s); store<float, P>(a.rstd + pos, v); }
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
             const int c = g + G * i;
-            if (c >= a.C) continue;
-            const float w = vec_at(a.v.w, a.v.dtype, c, 1.0f), b = vec_at(a.v.b, a.v.dtype, c, 0.0f);
-            float e[P];
+            if (c >= C) continue;
 #pragma unroll
-            for (int k = 0; k < P; ++k) e[k] = 0.0f;
-            if (a.res) load<T, P>(reinterpret_cast<const T *>(a.res) + at + (long)c * a.inner, e);
-#pragma unroll
-            for (int k = 0; k < P; ++k) e[k] = act(a.act, f[i][k] * q[k] * w + b + e[k]);
-            store<T, P>(reinterpret_cast<T *>(a.y) + at + (long)c * a.inner, e);
+            for (int k = 0; k < P; ++k) f[i][k] = act(a.act, f[i][k] * v[k] * w[i] + b[i] + (a.res ? to_f<T>(e[i].v[k]) : 0.0f));
+            store<T, P>(reinterpret_cast<T *>(a.y) + at + c * a.inner, f[i]);
         }
     }
 }
@@ -329,50 +356,51 @@ template <typename T, int NC, int P> __global__ __launch_bounds__(kThreads) void
 template <typename T, int NC, int P> __global__ __launch_bounds__(kThreads) void maps_bwd(Args a, int LX)
 {
     __shared__ float red[4 * 64 * P];
-    const int lx = threadIdx.x & (LX - 1), g = threadIdx.x / LX, G = kThreads / LX;
-    const float inv = 1.0f / (float)a.C;
-    const bool need_z = a.act != TEF_ACT_NONE;
+    const int lx = threadIdx.x & (LX - 1), g = threadIdx.x / LX, G = kThreads / LX, C = a.C;
+    const float inv = 1.0f / (float)C;
+    const bool need_z = a.act != TEF_ACT_NONE, need_e = need_z && a.res;
     const long tile = (long)LX * P;
-    float dw[NC], db[NC];
+    float w[NC], b[NC], dw[NC], db[NC];
 #pragma unroll
-    for (int i = 0; i < NC; ++i) dw[i] = db[i] = 0.0f;
+    for (int i = 0; i < NC; ++i) {
+        const int c = g + G * i < C ? g + G * i : C - 1;
+        w[i] = vec_at(a.v.w, a.v.dtype, c, 1.0f);
+        b[i] = need_z ? vec_at(a.v.b, a.v.dtype, c, 0.0f) : 0.0f;
+        dw[i] = db[i] = 0.0f;
+    }
     for (long t = blockIdx.x; t * tile < a.rows; t += gridDim.x) {
-        const long pos = t * tile + (long)lx * P;
-        const bool live = pos < a.rows;
-        const long o = live ? pos / a.inner : 0, at = live ? o * a.C * a.inner + (pos - o * a.inner) : 0;
-        float mean[P], rstd[P], u[NC][P], h[NC][P], s1[P], s2[P];
-        load_n<float, P>(a.mean + (live ? pos : 0), live ? P : 0, mean);
-        load_n<float, P>(a.rstd + (live ? pos : 0), live ? P : 0, rstd);
+        const bool live = t * tile + (long)lx * P < a.rows;
+        const long pos = live ? t * tile + (long)lx * P : a.rows - P;
+        const long o = pos / a.inner, at = o * C * a.inner + (pos - o * a.inner);
+        Pack<T, P> qx[NC], qd[NC], qe[NC];
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const long off = at + (g + G * i < C ? g + G * i : C - 1) * a.inner;
+            qx[i] = raw<T, P>(reinterpret_cast<const T *>(a.x) + off);
+            qd[i] = raw<T, P>(reinterpret_cast<const T *>(a.dy) + off);
+        }
+        if (need_e)
+#pragma unroll
+            for (int i = 0; i < NC; ++i) qe[i] = raw<T, P>(reinterpret_cast<const T *>(a.res) + at + (g + G * i < C ? g + G * i : C - 1) * a.inner);
+        const Pack<float, P> mean = raw<float, P>(a.mean + pos), rstd = raw<float, P>(a.rstd + pos);
+        float u[NC][P], h[NC][P], s1[P], s2[P];
 #pragma unroll
         for (int k = 0; k < P; ++k) s1[k] = s2[k] = 0.0f;
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
-            const int c = g + G * i, n = live && c < a.C ? P : 0;
-            const long off = at + (long)c * a.inner;
-            load_n<T, P>(reinterpret_cast<const T *>(a.x) + off, n, u[i]);
-            load_n<T, P>(reinterpret_cast<const T *>(a.dy) + off, n, h[i]);
-        }
+            const bool in = live && g + G * i < C;
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            const int c = g + G * i;
-            const bool in = live && c < a.C;
-            const long off = at + (long)c * a.inner;
-            const float w = in ? vec_at(a.v.w, a.v.dtype, c, 1.0f) : 0.0f;
-            float e[P];
-#pragma unroll
-            for (int k = 0; k < P; ++k) { e[k] = 0.0f; u[i][k] = in ? (u[i][k] - mean[k]) * rstd[k] : 0.0f; }
-            if (need_z && in) {
-                const float b = vec_at(a.v.b, a.v.dtype, c, 0.0f);
-                if (a.res) load<T, P>(reinterpret_cast<const T *>(a.res) + off, e);
-#pragma unroll
-                for (int k = 0; k < P; ++k) h[i][k] *= act_slope(a.act, u[i][k] * w + b + e[k]);
+            for (int k = 0; k < P; ++k) {
+                u[i][k] = in ? (to_f<T>(qx[i].v[k]) - mean.v[k]) * rstd.v[k] : 0.0f;
+                h[i][k] = in ? to_f<T>(qd[i].v[k]) : 0.0f;
+                if (need_z && in) h[i][k] *= act_slope(a.act, u[i][k] * w[i] + b[i] + (need_e ? to_f<T>(qe[i].v[k]) : 0.0f));
             }
-            if (a.dres && in) store<T, P>(reinterpret_cast<T *>(a.dres) + off, h[i]);
+            if (a.dres && in) store<T, P>(reinterpret_cast<T *>(a.dres) + at + (g + G * i) * a.inner, h[i]);
 #pragma unroll
             for (int k = 0; k < P; ++k) {
                 dw[i] += h[i][k] * u[i][k];
                 db[i] += h[i][k];
-                h[i][k] *= w;
+                h[i][k] *= w[i];
                 s1[k] += h[i][k];
                 s2[k] += h[i][k] * u[i][k];
             }
@@ -384,15 +412,15 @@ template <typename T, int NC, int P> __global__ __launch_bounds__(kThreads) void
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
             const int c = g + G * i;
-            if (c >= a.C) continue;
+            if (c >= C) continue;
             float e[P];
 #pragma unroll
-            for (int k = 0; k < P; ++k) e[k] = rstd[k] * (h[i][k] - s1[k] * inv - u[i][k] * (s2[k] * inv));
-            store<T, P>(reinterpret_cast<T *>(a.dx) + at + (long)c * a.inner, e);
+            for (int k = 0; k < P; ++k) e[k] = rstd.v[k] * (h[i][k] - s1[k] * inv - u[i][k] * (s2[k] * inv));
+            store<T, P>(reinterpret_cast<T *>(a.dx) + at + c * a.inner, e);
         }
     }
     if (!a.part) return;
-    float *part = a.part + (long)blockIdx.x * 2 * a.C;
+    float *part = a.part + (long)blockIdx.x * 2 * C;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
         for (int o2 = LX >> 1; o2 > 0; o2 >>= 1) {
@@ -400,7 +428,7 @@ template <typename T, int NC, int P> __global__ __launch_bounds__(kThreads) void
             db[i] += __shfl_xor(db[i], o2, 64);
         }
         const int c = g + G * i;
-        if (lx == 0 && c < a.C) { part[c] = dw[i]; part[a.C + c] = db[i]; }
+        if (lx == 0 && c < C) { part[c] = dw[i]; part[C + c] = db[i]; }
     }
 }
 
@@ -475,24 +503,29 @@ template <typename T> __global__ __launch_bounds__(kThreads) void long_bwd(Args 
     }
 }
 
-// dweight / dbias = the sum of the workgroups' partial rows: 64 columns a workgroup, 4 waves that each take every fourth row,
-// four running sums a lane (fixed order).
-__global__ __launch_bounds__(kThreads) void norm_join(const float *__restrict__ part, int parts, int C, void *dw, void *db, int dtype)
+// dweight / dbias = the sum of the workgroups' partial rows: 64 columns a workgroup of 16 waves, wave k takes the rows k, k + 16,
+// ..., eight of them in flight (a partial row comes from another XCD's L2: latency is all there is), joined in a fixed order.
+constexpr int kJoinWaves = 16;
+__global__ __launch_bounds__(64 * kJoinWaves) void norm_join(const float *__restrict__ part, int parts, int C, void *dw, void *db, int dtype)
 {
-    __shared__ float red[kThreads];
+    __shared__ float red[kJoinWaves][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.x * 64 + lane;
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (col < 2 * C) {
-        int k = wave;
-        for (; k + 12 < parts; k += 16)
+    float s[8];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[j] += part[(long)(k + 4 * j) * 2 * C + col];
-        for (int j = 0; k < parts; k += 4, ++j) s[j] += part[(long)k * 2 * C + col];
-    }
-    red[threadIdx.x] = (s[0] + s[1]) + (s[2] + s[3]);
+    for (int j = 0; j < 8; ++j) s[j] = 0.0f;
+    if (col < 2 * C)
+        for (int k = wave; k < parts; k += 8 * kJoinWaves) {
+            float f[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = part[(long)(k + kJoinWaves * j < parts ? k + kJoinWaves * j : parts - 1) * 2 * C + col];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s[j] += k + kJoinWaves * j < parts ? f[j] : 0.0f;
+        }
+    red[wave][lane] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
     __syncthreads();
     if (wave == 0 && col < 2 * C) {
-        const float v = (red[lane] + red[64 + lane]) + (red[128 + lane] + red[192 + lane]);
+        float v = 0.0f;
+        for (int k = 0; k < kJoinWaves; ++k) v += red[k][lane];
         if (col < C) { if (dw) vec_put(dw, dtype, col, v); }
         else if (db) vec_put(db, dtype, col - C, v);
     }
@@ -545,11 +578,11 @@ Plan make_plan(const tef_norm_desc &d)
     } else {
         p.per = d.inner % 4 == 0 ? 4 : 1;
         // as many lanes along the positions as leave a thread at most 64 values (long runs of memory per channel), then
-        // fewer while the grid does not cover the 256 CUs twice
+        // fewer while the grid does not cover the 256 CUs and a thread still has more than one channel
         const int most = 64 / p.per;
         int lx = p.per == 4 ? 16 : 64;
-        while (lx > 4 && (d.channels + kThreads / lx - 1) / (kThreads / lx) > most) lx >>= 1;
-        while (lx > 4 && (rows + lx * p.per - 1) / (lx * p.per) < 512 && (long)d.channels * lx > kThreads) lx >>= 1;
+        while (lx > 1 && (d.channels + kThreads / lx - 1) / (kThreads / lx) > most) lx >>= 1;
+        while (lx > 1 && (rows + lx * p.per - 1) / (lx * p.per) < 256 && (long)d.channels * lx > kThreads) lx >>= 1;
         const int nc = (d.channels + kThreads / lx - 1) / (kThreads / lx);
         if (nc <= most) {
             p.kind = 2;
@@ -564,28 +597,32 @@ Plan make_plan(const tef_norm_desc &d)
     return p;
 }
 
-template <typename T, int N> void go_n(const Plan &p, bool bwd, dim3 grid, hipStream_t st, const Args &a)
+template <typename T, int N, bool WG> void go_rows(const Plan &p, bool bwd, dim3 grid, hipStream_t st, const Args &a)
 {
     const dim3 block(kThreads);
-    if (p.kind == 0) {
-        if constexpr (N <= 8) {
-            if (bwd) hipLaunchKernelGGL((rows_bwd<T, N, false>), grid, block, 0, st, a, p.lanes);
-            else hipLaunchKernelGGL((rows_fwd<T, N, false>), grid, block, 0, st, a, p.lanes);
-        }
-    } else if (p.kind == 1) {
-        if constexpr (N <= 8 && N > 1) {
-            if (bwd) hipLaunchKernelGGL((rows_bwd<T, N, true>), grid, block, 0, st, a, p.lanes);
-            else hipLaunchKernelGGL((rows_fwd<T, N, true>), grid, block, 0, st, a, p.lanes);
-        }
-    } else if (p.per == 4) {
-        if constexpr (N <= 16) {
-            if (bwd) hipLaunchKernelGGL((maps_bwd<T, N, 4>), grid, block, 0, st, a, p.lanes);
-            else hipLaunchKernelGGL((maps_fwd<T, N, 4>), grid, block, 0, st, a, p.lanes);
-        }
+    if (a.C % V == 0) {
+        if (bwd) hipLaunchKernelGGL((rows_bwd<T, N, WG, true>), grid, block, 0, st, a, p.lanes);
+        else hipLaunchKernelGGL((rows_fwd<T, N, WG, true>), grid, block, 0, st, a, p.lanes);
     } else {
-        if (bwd) hipLaunchKernelGGL((maps_bwd<T, N, 1>), grid, block, 0, st, a, p.lanes);
-        else hipLaunchKernelGGL((maps_fwd<T, N, 1>), grid, block, 0, st, a, p.lanes);
+        if (bwd) hipLaunchKernelGGL((rows_bwd<T, N, WG, false>), grid, block, 0, st, a, p.lanes);
+        else hipLaunchKernelGGL((rows_fwd<T, N, WG, false>), grid, block, 0, st, a, p.lanes);
     }
+}
+template <typename T, int N, int P> void go_maps(const Plan &p, bool bwd, dim3 grid, hipStream_t st, const Args &a)
+{
+    if (bwd) hipLaunchKernelGGL((maps_bwd<T, N, P>), grid, dim3(kThreads), 0, st, a, p.lanes);
+    else hipLaunchKernelGGL((maps_fwd<T, N, P>), grid, dim3(kThreads), 0, st, a, p.lanes);
+}
+template <typename T, int N> void go_n(const Plan &p, bool bwd, dim3 grid, hipStream_t st, const Args &a)
+{
+    if constexpr (N <= 8) {
+        if (p.kind == 0) return go_rows<T, N, false>(p, bwd, grid, st, a);
+        if constexpr (N > 1)
+            if (p.kind == 1) return go_rows<T, N, true>(p, bwd, grid, st, a);
+    }
+    if constexpr (N <= 16)
+        if (p.kind == 2 && p.per == 4) return go_maps<T, N, 4>(p, bwd, grid, st, a);
+    if (p.kind == 2 && p.per == 1) go_maps<T, N, 1>(p, bwd, grid, st, a);
 }
 
 template <typename T> void go(const Plan &p, bool bwd, dim3 grid, hipStream_t st, const Args &a)
@@ -681,7 +718,7 @@ int tef_layer_norm_backward(const tef_norm_desc *d, const void *x, const void *w
     const unsigned blocks = bwd_blocks(p);
     launch(*d, p, true, blocks, st, a);
     if (sums)
-        hipLaunchKernelGGL(norm_join, dim3((unsigned)((2l * d->channels + 63) / 64)), dim3(kThreads), 0, st, (const float *)workspace, (int)blocks,
+        hipLaunchKernelGGL(norm_join, dim3((unsigned)((2l * d->channels + 63) / 64)), dim3(64 * kJoinWaves), 0, st, (const float *)workspace, (int)blocks,
                            d->channels, dweight, dbias, d->wdtype);
     return tef::check_launch("layer norm backward");
 }

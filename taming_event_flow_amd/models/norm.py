@@ -24,65 +24,66 @@ def _ptr(t):
     return t.data_ptr() if t is not None else None
 
 
-def _rows_last(t, dim):
-    return t.movedim(dim, -1)
+_TORCH = {code: dtype for dtype, code in _DTYPES.items()}
 
 
 class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, dim, eps, act):
-        lib = _lib.lib()
         # a map in channels-last memory is a matrix of rows as it stands; anything else is taken in x's own dimension order
-        last = _rows_last(x, dim)
-        rows = last.is_contiguous()
-        arrange = (lambda t: _rows_last(t, dim).contiguous()) if rows else (lambda t: t.contiguous())
         shape = x.shape
-        xc = arrange(x)
-        rc = arrange(residual) if residual is not None else None
+        last = x if dim == len(shape) - 1 else x.movedim(dim, -1)
+        rows = last.is_contiguous()
+        xc = last if rows else x.contiguous()
+        rc = residual
+        if rc is not None:
+            rc = (rc.movedim(dim, -1) if rows else rc).contiguous()
         w = weight.contiguous() if weight is not None else None
         b = bias.contiguous() if bias is not None else None
-        outer, inner = (math.prod(xc.shape[:-1]), 1) if rows else (math.prod(shape[:dim]), math.prod(shape[dim + 1:]))
-        if inner == 0:
-            outer, inner = 0, 1
+        C = shape[dim]
+        inner = 1 if rows else math.prod(shape[dim + 1:])
+        n = x.numel() // C      # positions
         vec = w if w is not None else b
-        d = _lib.NormDesc(outer, inner, shape[dim], _DTYPES[x.dtype], _DTYPES[vec.dtype if vec is not None else x.dtype], _lib.ACT[act],
-                          eps)
+        dtype = _DTYPES[x.dtype]
+        d = _lib.NormDesc(n // inner if n else 0, inner if n else 1, C, dtype, dtype if vec is None else _DTYPES[vec.dtype], _lib.ACT[act], eps)
         y = torch.empty_like(xc)
         keep = any(ctx.needs_input_grad)
-        stats = torch.empty((2, outer * inner), dtype=torch.float32, device=x.device) if keep else None
-        n = 4 * outer * inner
+        stats = torch.empty((2 * n,), dtype=torch.float32, device=x.device) if keep else None
+        at = stats.data_ptr() if keep else None
         with torch.cuda.device_of(x):
-            rc_ = lib.tef_layer_norm_forward(ctypes.byref(d), xc.data_ptr(), _ptr(w), _ptr(b), _ptr(rc), y.data_ptr(),
-                                             stats.data_ptr() if keep else None, stats.data_ptr() + n if keep else None,
-                                             _lib.stream_ptr())
-        _lib.check(rc_, "tef_layer_norm_forward")
+            code = _lib.lib().tef_layer_norm_forward(ctypes.byref(d), xc.data_ptr(), _ptr(w), _ptr(b), _ptr(rc), y.data_ptr(), at,
+                                                     at + 4 * n if keep else None, _lib.stream_ptr())
+        _lib.check(code, "tef_layer_norm_forward")
         if keep:
-            need_z = act is not None
-            ctx.save_for_backward(xc, w, b if need_z else None, rc if need_z else None, stats)
-            ctx.desc, ctx.rows, ctx.dim, ctx.shape, ctx.vec = d, rows, dim, shape, (weight is not None, bias is not None)
+            if act is None:      # (only an activation's slope needs them again)
+                b = rc = None
+            ctx.save_for_backward(xc, w, b, rc, stats)
+            ctx.info = d, n, rows, dim
         return y.movedim(-1, dim) if rows else y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        lib = _lib.lib()
+        if torch.is_grad_enabled():      # (create_graph=True)
+            raise RuntimeError("layer_norm is differentiable once: its backward pass has no gradient of its own")
         xc, w, b, rc, stats = ctx.saved_tensors
-        d = ctx.desc
+        d, n, rows, dim = ctx.info
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        dyc = (_rows_last(dy, ctx.dim) if ctx.rows else dy).contiguous()
-        wdtype = {v: k for k, v in _DTYPES.items()}[d.wdtype]
-        new = lambda need: torch.empty_like(xc) if need else None  # noqa: E731
-        vec = lambda need: torch.empty((d.channels,), dtype=wdtype, device=xc.device) if need else None  # noqa: E731
-        dx, dr, dw, db = new(need_x), new(need_r), vec(need_w), vec(need_b)
-        nbytes = lib.tef_layer_norm_workspace_bytes(ctypes.byref(d)) if need_w or need_b else 0
-        ws = torch.empty((nbytes,), dtype=torch.uint8, device=xc.device) if nbytes else None
+        dy = (dy.movedim(dim, -1) if rows else dy).contiguous()
+        dx = torch.empty_like(xc) if need_x else None
+        dr = torch.empty_like(xc) if need_r else None
+        lib, dw, db, ws, nbytes = _lib.lib(), None, None, None, 0
+        if need_w or need_b:
+            dw, db = torch.empty((2, d.channels), dtype=_TORCH[d.wdtype], device=xc.device).unbind(0)
+            nbytes = lib.tef_layer_norm_workspace_bytes(ctypes.byref(d))
+            ws = torch.empty((nbytes,), dtype=torch.uint8, device=xc.device)
+        at = stats.data_ptr()
         with torch.cuda.device_of(xc):
-            rc_ = lib.tef_layer_norm_backward(ctypes.byref(d), xc.data_ptr(), _ptr(w), _ptr(b), _ptr(rc), stats.data_ptr(),
-                                              stats.data_ptr() + 4 * d.outer * d.inner, dyc.data_ptr(), _ptr(dx), _ptr(dr),
-                                              _ptr(dw), _ptr(db), _ptr(ws), nbytes, _lib.stream_ptr())
-        _lib.check(rc_, "tef_layer_norm_backward")
-        back = (lambda t: t.movedim(-1, ctx.dim) if t is not None and ctx.rows else t)
-        return back(dx), dw, db, back(dr), None, None, None
+            code = lib.tef_layer_norm_backward(ctypes.byref(d), xc.data_ptr(), _ptr(w), _ptr(b), _ptr(rc), at, at + 4 * n, dy.data_ptr(),
+                                               _ptr(dx), _ptr(dr), _ptr(dw), _ptr(db), _ptr(ws), nbytes, _lib.stream_ptr())
+        _lib.check(code, "tef_layer_norm_backward")
+        if rows:
+            dx, dr = (t.movedim(-1, dim) if t is not None else None for t in (dx, dr))
+        return dx, dw if need_w else None, db if need_b else None, dr, None, None, None
 
 
 def layer_norm(x, weight=None, bias=None, dim=1, eps=1e-5, activation=None, residual=None):

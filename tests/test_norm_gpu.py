@@ -221,6 +221,14 @@ def test_gradient_against_differences(dev):
         assert abs((hi - lo) / (2 * h) - slope) <= scale * (200 * U + 1e-8) + 1e-8, i
 
 
+def test_second_derivative_is_refused(dev):
+    from taming_event_flow_amd.models.norm import layer_norm
+
+    x = torch.randn(3, 8, device=dev, requires_grad=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(layer_norm(x).sum(), x, create_graph=True)
+
+
 def test_empty(dev):
     from taming_event_flow_amd.models.norm import layer_norm
 
