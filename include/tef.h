@@ -561,6 +561,49 @@ int tef_layer_norm_backward(const tef_norm_desc *d, const void *x, const void *w
                             const float *mean, const float *rstd, const void *dy, void *dx, void *dresidual, void *dweight,
                             void *dbias, void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- orthogonalised updates (csrc/tef_ortho.hip) -----------------------------------------------------------------------
+ * tef_orthogonalize: for every matrix U [rows][cols] (batch of them, `*_stride` elements apart, rows `*_ld` elements apart, a
+ * row's elements contiguous) X = U / max(|U|_F, eps), then `steps` times X <- a X + (b A + c A A) X with A = X X^T (X^T X for tall
+ * ones: same result), written to dst (which may be src).  All matrices of a call go through the same launches.
+ * src and dst have type `dtype` (TEF_F32 / F16 / BF16) and the alignment of their elements; the arithmetic is fp32-grade
+ * whatever the type.  1 <= steps <= 32; coefficients under which a singular value in [0, 1] would leave |s| < 3.9 are
+ * refused.  The matrix list is read during the call only.  Workspace: 256-byte aligned, the caller's, of the size asked for with the same
+ * list; two calls that may run at once need two. */
+typedef struct tef_ortho_matrix {
+    const void *src;
+    void *dst;
+    long rows;
+    long cols;
+    long src_ld;
+    long dst_ld;
+    long batch;
+    long src_stride;
+    long dst_stride;
+} tef_ortho_matrix;
+size_t tef_orthogonalize_workspace_bytes(const tef_ortho_matrix *matrices, int count);
+int tef_orthogonalize(const tef_ortho_matrix *matrices, int count, int dtype, int steps, double a, double b, double c, double eps,
+                      void *workspace, size_t workspace_bytes, void *stream);
+/* tef_muon_step: one optimiser step on flat fp32 buffers p (parameters), g (gradients), m (momentum), v (Adam's second moments of
+ * the vectors only, packed in list order).  g is first scaled by min(1, max_norm / (norm + 1e-6)) (max_norm <= 0: not).
+ * Matrices: m += (1 - momentum) (g - m); u = nesterov ? g + momentum (m - g) : m; p <- p (1 - lr weight_decay) - lr scale O(u),
+ * O as above.  Vectors: Adam like tef_adam_clip_step with adam_lr, beta1, beta2, adam_eps; `step` is the device counter that
+ * tef_l2_norm increments.  g is cleared.  hp (device, doubles) = {lr, momentum, weight_decay, max_norm, adam_lr, beta1, beta2,
+ * adam_eps}.  Ranges must not overlap; what no range covers stays as it is. */
+typedef struct tef_muon_matrix {
+    long offset;
+    long rows;
+    long cols;
+    float scale;
+} tef_muon_matrix;
+typedef struct tef_muon_vector {
+    long offset;
+    long size;
+} tef_muon_vector;
+size_t tef_muon_workspace_bytes(const tef_muon_matrix *matrices, int count);
+int tef_muon_step(float *p, float *g, float *m, float *v, const tef_muon_matrix *matrices, int nmatrices, const tef_muon_vector *vectors,
+                  int nvectors, const float *norm, const double *hp, const float *step, int nesterov, int steps, double a, double b,
+                  double c, double eps, void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- validation metrics (loss/flow_val.py; evaluation only, batch 1, no gradients) ---------------------------------
  * Flow maps are planar [H][W] (fx, fy separately); event lists are loc [N][2] = (y, x), ts [N], mask [N][2]. */
 /* one warping step: flow lookup at loc (flow_out [N][2] = (f_y, f_x) if not NULL); if do_warp: loc += (tref - ts) * flow,

@@ -98,6 +98,25 @@ class NormDesc(ctypes.Structure):
                 ("wdtype", ctypes.c_int), ("act", ctypes.c_int), ("eps", ctypes.c_float)]
 
 
+class OrthoMatrix(ctypes.Structure):
+    """struct tef_ortho_matrix (include/tef.h)"""
+
+    _fields_ = [("src", _fp), ("dst", _fp)] + [(n, ctypes.c_long) for n in ("rows", "cols", "src_ld", "dst_ld", "batch", "src_stride",
+                                                                            "dst_stride")]
+
+
+class MuonMatrix(ctypes.Structure):
+    """struct tef_muon_matrix (include/tef.h)"""
+
+    _fields_ = [("offset", ctypes.c_long), ("rows", ctypes.c_long), ("cols", ctypes.c_long), ("scale", ctypes.c_float)]
+
+
+class MuonVector(ctypes.Structure):
+    """struct tef_muon_vector (include/tef.h)"""
+
+    _fields_ = [("offset", ctypes.c_long), ("size", ctypes.c_long)]
+
+
 # name -> (restype, argtypes); every symbol include/tef.h declares
 SIGNATURES = {
     "tef_version": (ctypes.c_int, []),
@@ -226,6 +245,12 @@ SIGNATURES = {
     "tef_layer_norm_forward": (ctypes.c_int, [ctypes.POINTER(NormDesc)] + [_fp] * 8),
     "tef_layer_norm_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(NormDesc)]),
     "tef_layer_norm_backward": (ctypes.c_int, [ctypes.POINTER(NormDesc)] + [_fp] * 12 + [ctypes.c_size_t, _fp]),
+    "tef_orthogonalize_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(OrthoMatrix), ctypes.c_int]),
+    "tef_orthogonalize": (ctypes.c_int, [ctypes.POINTER(OrthoMatrix), ctypes.c_int, ctypes.c_int, ctypes.c_int] + [ctypes.c_double] * 4
+                          + [_fp, ctypes.c_size_t, _fp]),
+    "tef_muon_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(MuonMatrix), ctypes.c_int]),
+    "tef_muon_step": (ctypes.c_int, [_fp] * 4 + [ctypes.POINTER(MuonMatrix), ctypes.c_int, ctypes.POINTER(MuonVector), ctypes.c_int]
+                      + [_fp] * 3 + [ctypes.c_int, ctypes.c_int] + [ctypes.c_double] * 4 + [_fp, ctypes.c_size_t, _fp]),
     "tef_gru_blend": (ctypes.c_int, [_fp, _fp, _fp, ctypes.c_size_t, _fp, _fp]),
     "tef_gru_blend_backward": (ctypes.c_int, [_fp, _fp, _fp, _fp, ctypes.c_size_t, _fp, _fp, _fp, _fp]),
     "tef_val_event_step": (ctypes.c_int, [_fp, _fp, ctypes.c_int, ctypes.c_int, _fp, _fp, _fp, ctypes.c_int,

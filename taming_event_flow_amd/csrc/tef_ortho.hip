@@ -1,0 +1,971 @@
+// tef_ortho.hip — orthogonalised updates: Newton-Schulz orthogonalisation of matrices, and the optimiser step built on it
+// (clip, momentum, orthogonalise, apply; Adam for the vectors).
+//
+// Orthogonalisation.  For U [m][n] (m <= n; a tall matrix is taken transposed) and X_0 = U / max(|U|_F, eps) the iteration
+//
+//   A = X X^T,  P = a I + b A + c A A,  X <- P X            (the singular values go through  a s + b s^3 + c s^5)
+//
+// is run on the small side: P is a polynomial of A, so A' = X' X'^T = P A P and X_k = Q_k X_0 with Q' = P Q, and a segment of up to
+// three steps needs ONE Gram matrix of X and ONE product Q X; in between all matrices are m x m, symmetric, and commute
+// (products of them are symmetric: half of the tiles are computed, the other half mirrored).  The recurrence for A amplifies
+// its rounding errors by up to a^2 = 12 a step where the direct iteration amplifies them by a: after three steps the Gram
+// matrix is formed anew from X (five steps: 3 + 2), which keeps the result within a small factor of a plain fp32 iteration on
+// rank-deficient matrices too; all five in one segment lose a further digit.  Work for five steps, in multiply-adds
+// with symmetric products counted half: 3 m^2 n + 7 m^3 instead of 7.5 m^2 n + 2.5 m^3.
+//
+// Arithmetic.  fp32 matrix instructions run at 1/16 of the fp16 rate, so every operand is held as two fp16 planes, v = hi + lo
+// with hi = fp16(v), lo = fp16(v - hi) — 22 bits — and a product is hi hi + hi lo + lo hi with fp32 accumulation; the dropped lo lo
+// is 2^-22 of the product.  All matrices have bounded entries (|X|, |A|, |P| <= a few; |Q| <= a^3), so a fixed power of two
+// per matrix kind puts them into fp16's normal range.  Nothing is rounded to a single fp16 anywhere.
+//
+// Layout.  A split matrix is [rows][cols / 32][hi 32 | lo 32]: a row's 32 columns are one 128-byte line with both planes, so a
+// step of 32 along k loads whole lines.  Rows and columns are padded to multiples of 32 with zeros.
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+#include <string.h>
+
+#include "tef.h"
+#include "tef_common.h"
+
+namespace {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef float float16v __attribute__((ext_vector_type(16)));
+typedef unsigned uint4v __attribute__((ext_vector_type(4)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+
+constexpr int kThreads = 256;
+constexpr int kGroup = 64;             // matrices (with their batches) a set of launches takes
+constexpr int kChunk = 16;             // of them per kernel argument
+constexpr int kMaxParts = 512;         // partial sums of a matrix's squares
+constexpr int kSegment = 3;            // steps between two Gram matrices
+constexpr int kExpX = 12, kExpA = 12, kExpP = 12, kExpQ = 10;      // powers of two the split matrices are scaled by
+
+// What the kernels know of a matrix (a batch of equal ones): lives in the workspace, written by the first launch.
+struct Mat {
+    const void *src;                   // [rows][cols], row stride src_ld, batch stride src_stride (elements)
+    void *dst;
+    long src_ld, dst_ld, src_stride, dst_stride;
+    long ws;                           // bytes from the workspace's start to this matrix's area
+    long area;                         // ... of one batch element
+    int m, n, mp, np;                  // short and long side, padded
+    int tall;                          // src is [n][m]
+    int batch;
+    int parts;                         // partial sums of squares per batch element
+    int splits;                        // pieces of the Gram product's k
+    float scale;                       // of the applied update (optimiser)
+    int first[5];                      // first workgroup in the launch of each phase (below)
+};
+enum { PH_SQ = 0, PH_PACK, PH_GRAM, PH_CHAIN, PH_APPLY };
+
+// One batch element's area: doubles parts[kMaxParts], int exponents[kMaxSteps + 1], then the split matrices.
+__host__ __device__ inline long split_bytes(long rows, long cols) { return rows * cols * 4; }
+enum { BUF_X0 = 0, BUF_X1, BUF_A, BUF_W, BUF_P0, BUF_P1, BUF_Q0, BUF_Q1, BUF_PART };
+constexpr int kMaxSteps = 32;
+constexpr long kHead = kMaxParts * 8 + 256;      // (a multiple of 256, at least 4 * (kMaxSteps + 1) past the sums)
+__host__ __device__ inline long buf_at(int which, int mp, int np)
+{
+    const long x = split_bytes(mp, np), s = split_bytes(mp, mp);
+    return which <= BUF_X1 ? kHead + which * x : kHead + 2 * x + (which - BUF_A) * s;
+}
+
+struct Table { const Mat *mats; int count; };
+
+// Which matrix a workgroup of a phase belongs to: `first` is ascending, the wave looks at up to 64 of them at once.
+__device__ inline int find(const Table &t, int phase)
+{
+    const int lane = threadIdx.x & 63;
+    const int f = lane < t.count ? t.mats[lane].first[phase] : 0x7fffffff;
+    return __popcll(__ballot(f <= (int)blockIdx.x)) - 1;
+}
+
+template <typename T> __device__ inline float to_f(T v);
+template <> __device__ inline float to_f<float>(float v) { return v; }
+template <> __device__ inline float to_f<__half>(__half v) { return __half2float(v); }
+template <> __device__ inline float to_f<__hip_bfloat16>(__hip_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ inline T from_f(float v);
+template <> __device__ inline float from_f<float>(float v) { return v; }
+template <> __device__ inline __half from_f<__half>(float v) { return __float2half(v); }
+template <> __device__ inline __hip_bfloat16 from_f<__hip_bfloat16>(float v) { return __float2bfloat16(v); }
+template <typename T, int V> struct __attribute__((packed, aligned(sizeof(T)))) Pack { T v[V]; };
+
+__device__ inline void split(float v, _Float16 &hi, _Float16 &lo)
+{
+    hi = (_Float16)v;
+    lo = (_Float16)(v - (float)hi);      // (infinite hi: NaN, as an overflow should show)
+}
+
+__device__ inline double block_sum(double s, double *red)
+{
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    return (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+// ---- the matrices' values ---------------------------------------------------------------------------------------------------
+// Orthogonalisation: the caller's matrix.  Optimiser step: the look-ahead of the momentum, u = g + mu (m' - g) (Nesterov) or m',
+// g the clipped gradient, m' = m + (1 - mu) (g - m); the first sweep writes m', the second one clears g.
+struct Step {
+    float *g, *m, *p;                  // flat buffers; a Mat's src / dst are element offsets into them
+    const float *norm;
+    const double *hp;                  // lr, momentum, weight_decay, max_norm
+    int nesterov;
+};
+__device__ inline float clip_scale(const float *norm, double max_norm)
+{
+    if (!(max_norm > 0.0)) return 1.0f;
+    const float s = (float)max_norm / (norm[0] + 1e-6f);      // (a NaN norm poisons the step: loud, like clip_grad_norm_)
+    return s < 1.0f || s != s ? s : 1.0f;
+}
+
+// ---- phase 0: sums of squares (double: no overflow or underflow of a square for any fp32 input) -----------------------------
+struct Chunk { Mat m[kChunk]; int n, at; };
+
+template <typename T, bool STEP> __global__ __launch_bounds__(kThreads) void ortho_squares(Chunk ch, Mat *table, char *ws, Step st)
+{
+    __shared__ double red[4];
+    int k = 0;
+    const int base = ch.m[0].first[PH_SQ];
+    const int wg = blockIdx.x + base;
+    while (k + 1 < ch.n && ch.m[k + 1].first[PH_SQ] <= wg) ++k;
+    if (blockIdx.x == 0 && (int)threadIdx.x < ch.n) table[ch.at + threadIdx.x] = ch.m[threadIdx.x];
+    const Mat &M = ch.m[k];
+    const int part = (wg - M.first[PH_SQ]) % M.parts, bi = (wg - M.first[PH_SQ]) / M.parts;
+    const long total = (long)M.m * M.n, per = ((total + M.parts - 1) / M.parts + 3) & ~3l;
+    const long lo = part * per, hi = lo + per < total ? lo + per : total;
+    double s = 0.0;
+    if (STEP) {
+        const float mu = (float)st.hp[1], clip = clip_scale(st.norm, st.hp[3]), w = (float)(1.0 - st.hp[1]);
+        const long off = (long)M.src;
+        auto one = [&](long i) {
+            const float g = st.g[off + i] * clip;
+            float mm = st.m[off + i];
+            mm = mm + w * (g - mm);
+            st.m[off + i] = mm;
+            const float u = st.nesterov ? g + mu * (mm - g) : mm;
+            s += (double)u * u;
+        };
+        long i = lo + 4l * threadIdx.x;
+        for (; i + 4 <= hi; i += 4l * kThreads) {
+            Pack<float, 4> g = *reinterpret_cast<const Pack<float, 4> *>(st.g + off + i), mm = *reinterpret_cast<const Pack<float, 4> *>(st.m + off + i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float gc = g.v[j] * clip;
+                mm.v[j] = mm.v[j] + w * (gc - mm.v[j]);
+                const float u = st.nesterov ? gc + mu * (mm.v[j] - gc) : mm.v[j];
+                s += (double)u * u;
+            }
+            *reinterpret_cast<Pack<float, 4> *>(st.m + off + i) = mm;
+        }
+        for (; i < hi; ++i) one(i);
+    } else {
+        const int cols = M.tall ? M.m : M.n;
+        const T *src = reinterpret_cast<const T *>(M.src) + bi * M.src_stride;
+        if (M.src_ld == cols) {
+            long i = lo + 4l * threadIdx.x;
+            for (; i + 4 <= hi; i += 4l * kThreads) {
+                const Pack<T, 4> q = *reinterpret_cast<const Pack<T, 4> *>(src + i);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s += (double)to_f<T>(q.v[j]) * to_f<T>(q.v[j]);
+            }
+            for (; i < hi; ++i) s += (double)to_f<T>(src[i]) * to_f<T>(src[i]);
+        } else {
+            for (long i = lo + threadIdx.x; i < hi; i += kThreads) {
+                const float v = to_f<T>(src[(i / cols) * M.src_ld + i % cols]);
+                s += (double)v * v;
+            }
+        }
+    }
+    s = block_sum(s, red);
+    if (threadIdx.x == 0) reinterpret_cast<double *>(ws + M.ws + bi * M.area)[part] = s;
+}
+
+// ---- phase 1: normalise and split ---------------------------------------------------------------------------------------------
+// A workgroup writes 32 rows x 64 columns of the padded X (8 values a thread).  The scale is kExpX plus, where |U| < eps leaves
+// X small, the power of two that brings it back up: what is multiplied later always has 22 good bits.
+template <typename T, bool STEP> __global__ __launch_bounds__(kThreads) void ortho_pack(Table t, char *ws, double eps, Step st)
+{
+    __shared__ double red[4];
+    __shared__ float turn[64][33];
+    const Mat &M = t.mats[find(t, PH_PACK)];
+    const int tiles_n = (M.np + 63) / 64, tiles = (M.mp / 32) * tiles_n;
+    const int wg = blockIdx.x - M.first[PH_PACK], bi = wg / tiles, ti = wg % tiles / tiles_n, tj = wg % tiles % tiles_n;
+    char *area = ws + M.ws + bi * M.area;
+    const double *parts = reinterpret_cast<const double *>(area);
+    double s = 0.0;
+    for (int k = threadIdx.x; k < M.parts; k += kThreads) s += parts[k];
+    s = sqrt(block_sum(s, red));
+    const double div = s < eps ? eps : s, rho = s / div;      // (a NaN norm: NaN everywhere)
+    int up = 0;
+    if (rho < 1.0 && rho > 0.0) {
+        up = -ilogb(rho);
+        up = up > 100 ? 100 : up;
+    }
+    if (wg % tiles == 0 && threadIdx.x == 0) {
+        int *e = reinterpret_cast<int *>(area + kMaxParts * 8);
+        e[0] = kExpX + up;
+        for (int k = 1; k <= kMaxSteps; ++k) {      // a segment multiplies X by at most 2^6
+            up = up > 6 ? up - 6 : 0;
+            e[k] = kExpX + up;
+        }
+        up = e[0] - kExpX;
+    }
+    const double mul = ldexp(1.0 / div, kExpX + up);
+    const float clip = STEP ? clip_scale(st.norm, st.hp[3]) : 1.0f, mu = STEP ? (float)st.hp[1] : 0.0f;
+    const T *src = reinterpret_cast<const T *>(M.src) + bi * M.src_stride;
+    auto value = [&](long off) -> float {      // element `off` of the source
+        if constexpr (STEP) {
+            const long i = (long)M.src + off;
+            const float g = st.g[i] * clip, mm = st.m[i];
+            st.g[i] = 0.0f;
+            return st.nesterov ? g + mu * (mm - g) : mm;
+        } else {
+            return to_f<T>(src[off]);
+        }
+    };
+    float f[8];
+    const int r = threadIdx.x >> 3, c = (threadIdx.x & 7) * 8;      // row of the tile, first of 8 columns
+    const int i0 = ti * 32, j0 = tj * 64;
+    if (M.tall) {      // X[i][j] = src[j][i]: read along i, turn in LDS
+        const int i = threadIdx.x & 31;
+        for (int j = threadIdx.x >> 5; j < 64; j += 8)
+            turn[j][i] = i0 + i < M.m && j0 + j < M.n ? value((long)(j0 + j) * M.src_ld + i0 + i) : 0.0f;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[k] = turn[c + k][r];
+    } else {
+        const int i = i0 + r, j = j0 + c;
+        const long off = (long)i * M.src_ld + j;
+        if (i < M.m && j + 8 <= M.n) {
+            if constexpr (STEP) {
+                const long at = (long)M.src + off;
+                const Pack<float, 8> g = *reinterpret_cast<const Pack<float, 8> *>(st.g + at), mm = *reinterpret_cast<const Pack<float, 8> *>(st.m + at);
+                Pack<float, 8> zero;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const float gc = g.v[k] * clip;
+                    f[k] = st.nesterov ? gc + mu * (mm.v[k] - gc) : mm.v[k];
+                    zero.v[k] = 0.0f;
+                }
+                *reinterpret_cast<Pack<float, 8> *>(st.g + at) = zero;
+            } else {
+                const Pack<T, 8> q = *reinterpret_cast<const Pack<T, 8> *>(src + off);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) f[k] = to_f<T>(q.v[k]);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) f[k] = i < M.m && j + k < M.n ? value(off + k) : 0.0f;
+        }
+    }
+    if (j0 + c >= M.np) return;
+    half8 hi, lo;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        _Float16 h, l;
+        split((float)((double)f[k] * mul), h, l);
+        hi[k] = h;
+        lo[k] = l;
+    }
+    _Float16 *x = reinterpret_cast<_Float16 *>(area + buf_at(BUF_X0, M.mp, M.np)) + ((long)(i0 + r) * M.np + j0 + (c & ~31)) * 2 + (c & 31);
+    *reinterpret_cast<half8 *>(x) = hi;
+    *reinterpret_cast<half8 *>(x + 32) = lo;
+}
+
+// ---- the products -----------------------------------------------------------------------------------------------------------
+// A workgroup of four waves computes TS x TS values (TS = 128 or 64), each wave a quarter of them in 32 x 32 blocks.  k advances
+// by 32: TS lines of 128 bytes per operand, from global memory through registers into LDS while the previous step's lines
+// are multiplied (two buffers, one barrier a step).  The 16-byte chunks of a line are permuted by the row, chunk ^ (row & 7), so that the eight
+// lanes of an LDS cycle that read the same chunk of eight rows meet eight different bank groups.
+template <int TS> struct Geo {
+    static constexpr int FR = TS / 64;                       // 32 x 32 blocks of a wave along each side
+    static constexpr int LOADS = TS * 8 / kThreads;          // 16-byte chunks of an operand's step per thread
+    static constexpr int STAGE = TS * 128;                   // bytes of an operand's step
+    static constexpr int PITCH = TS + 4;                     // floats; the finished tile
+    static constexpr int LDS = 4 * STAGE > TS * PITCH * 4 ? 4 * STAGE : TS * PITCH * 4;
+};
+
+// operand whose rows run along k: chunk q of the tile = row q / 8, chunk q % 8
+template <int TS> __device__ inline void load_rows(uint4v (&r)[Geo<TS>::LOADS], const char *base, long ld, int row0, int rows, int kb)
+{
+#pragma unroll
+    for (int i = 0; i < Geo<TS>::LOADS; ++i) {
+        const int q = threadIdx.x + i * kThreads, row = row0 + (q >> 3);
+        r[i] = *reinterpret_cast<const uint4v *>(base + (long)(row < rows ? row : rows - 1) * ld + (long)kb * 128 + (q & 7) * 16);
+    }
+}
+template <int TS> __device__ inline void put_rows(char *lds, const uint4v (&r)[Geo<TS>::LOADS])
+{
+#pragma unroll
+    for (int i = 0; i < Geo<TS>::LOADS; ++i) {
+        const int q = threadIdx.x + i * kThreads, row = q >> 3;
+        *reinterpret_cast<uint4v *>(lds + row * 128 + (((q & 7) ^ (row & 7)) << 4)) = r[i];
+    }
+}
+// rows `row` (this lane's), k = 16 * s + 8 * (lane >> 5) ..: plane 0 hi, 1 lo
+__device__ inline half8 frag_rows(const char *lds, int row, int s, int plane)
+{
+    const int chunk = plane * 4 + s * 2 + ((threadIdx.x & 63) >> 5);
+    return *reinterpret_cast<const half8 *>(lds + row * 128 + ((chunk ^ (row & 7)) << 4));
+}
+// operand whose COLUMNS are the tile's (X in Q X): a step is 32 rows of TS / 32 lines.  64-byte slots (one plane of one line) are
+// permuted by the row; ds_read_b64_tr_b16 hands every lane four consecutive k of its column.
+template <int TS> __device__ inline void load_cols(uint4v (&r)[Geo<TS>::LOADS], const char *base, long ld, int blk0, int blks, int kb)
+{
+    constexpr int per = TS / 4;      // chunks of a row
+#pragma unroll
+    for (int i = 0; i < Geo<TS>::LOADS; ++i) {
+        const int q = threadIdx.x + i * kThreads, row = kb * 32 + q / per, c = q % per, blk = blk0 + (c >> 3);
+        r[i] = *reinterpret_cast<const uint4v *>(base + (long)row * ld + (long)(blk < blks ? blk : blks - 1) * 128 + (c & 7) * 16);
+    }
+}
+template <int TS> __device__ inline void put_cols(char *lds, const uint4v (&r)[Geo<TS>::LOADS])
+{
+    constexpr int per = TS / 4, slots = TS / 16;
+#pragma unroll
+    for (int i = 0; i < Geo<TS>::LOADS; ++i) {
+        const int q = threadIdx.x + i * kThreads, row = q / per, c = q % per, slot = (c >> 2) ^ (row & (slots - 1));
+        *reinterpret_cast<uint4v *>(lds + row * (TS * 4) + slot * 64 + (c & 3) * 16) = r[i];
+    }
+}
+template <int TS> __device__ inline half8 frag_cols(const char *lds, int col0, int s, int plane)
+{
+    constexpr int slots = TS / 16;
+    const int lane = threadIdx.x & 63, g = lane >> 4, src = lane & 15;
+    const int slot = (col0 >> 5) * 2 + plane, within = ((g & 1) * 16 + (src & 3) * 4) * 2;
+    half8 v;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int row = s * 16 + (g >> 1) * 8 + h * 4 + (src >> 2);
+        const char *p = lds + row * (TS * 4) + (slot ^ (row & (slots - 1))) * 64 + within;
+        const short4v q = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v *)p);
+        const half4 f = __builtin_bit_cast(half4, q);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[h * 4 + k] = f[k];
+    }
+    return v;
+}
+
+template <int TS> struct Acc { float16v v[Geo<TS>::FR][Geo<TS>::FR]; };
+
+// acc = L (rows li0 ..) times R (rows rj0 .. as columns, or, COLS, the 32-column blocks rj0 / 32 ..), k lines k0 .. k1
+template <int TS, bool COLS>
+__device__ inline void product(Acc<TS> &acc, char *lds, const char *L, long ldL, int li0, int rowsL, const char *R, long ldR, int rj0, int limR, int k0, int k1)
+{
+    using G = Geo<TS>;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = (wave >> 1) * (TS / 2), wj = (wave & 1) * (TS / 2);
+#pragma unroll
+    for (int i = 0; i < G::FR; ++i)
+#pragma unroll
+        for (int j = 0; j < G::FR; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc.v[i][j][e] = 0.0f;
+    uint4v a[G::LOADS], b[G::LOADS];
+    load_rows<TS>(a, L, ldL, li0, rowsL, k0);
+    if (COLS) load_cols<TS>(b, R, ldR, rj0 >> 5, limR, k0);
+    else load_rows<TS>(b, R, ldR, rj0, limR, k0);
+    __syncthreads();      // (whoever used this LDS before is done with it)
+    put_rows<TS>(lds, a);
+    if (COLS) put_cols<TS>(lds + G::STAGE, b);
+    else put_rows<TS>(lds + G::STAGE, b);
+    __syncthreads();
+    for (int kb = k0; kb < k1; ++kb) {
+        const char *la = lds + ((kb - k0) & 1) * 2 * G::STAGE, *lb = la + G::STAGE;
+        const int next = kb + 1 < k1 ? kb + 1 : kb;      // (the last step fetches its own lines again: no branch around the loads)
+        load_rows<TS>(a, L, ldL, li0, rowsL, next);
+        if (COLS) load_cols<TS>(b, R, ldR, rj0 >> 5, limR, next);
+        else load_rows<TS>(b, R, ldR, rj0, limR, next);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            half8 fa[G::FR][2], fb[G::FR][2];
+#pragma unroll
+            for (int i = 0; i < G::FR; ++i)
+#pragma unroll
+                for (int pl = 0; pl < 2; ++pl) {
+                    fa[i][pl] = frag_rows(la, wi + i * 32 + (lane & 31), s, pl);
+                    fb[i][pl] = COLS ? frag_cols<TS>(lb, wj + i * 32, s, pl) : frag_rows(lb, wj + i * 32 + (lane & 31), s, pl);
+                }
+#pragma unroll
+            for (int t = 0; t < 3; ++t)      // lo hi, hi lo, hi hi
+#pragma unroll
+                for (int i = 0; i < G::FR; ++i)
+#pragma unroll
+                    for (int j = 0; j < G::FR; ++j)
+                        acc.v[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[i][t == 0], fb[j][t == 1], acc.v[i][j], 0, 0, 0);
+        }
+        char *other = lds + ((kb + 1 - k0) & 1) * 2 * G::STAGE;
+        put_rows<TS>(other, a);
+        if (COLS) put_cols<TS>(other + G::STAGE, b);
+        else put_rows<TS>(other + G::STAGE, b);
+        __syncthreads();
+    }
+}
+
+// the finished tile, row-major in LDS (32 x 32 block: column lane & 31, row 8 (e / 4) + 4 (lane >> 5) + e % 4)
+template <int TS> __device__ inline float *to_tile(const Acc<TS> &acc, char *lds)
+{
+    using G = Geo<TS>;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = (wave >> 1) * (TS / 2), wj = (wave & 1) * (TS / 2);
+    float *tile = reinterpret_cast<float *>(lds);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < G::FR; ++i)
+#pragma unroll
+        for (int j = 0; j < G::FR; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                tile[(wi + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * G::PITCH + wj + j * 32 + (lane & 31)] = acc.v[i][j][e];
+    __syncthreads();
+    return tile;
+}
+
+// four neighbouring values of a split matrix's row
+__device__ inline void put_split(char *base, long cols, long row, int col, const float (&f)[4])
+{
+    _Float16 *p = reinterpret_cast<_Float16 *>(base) + (row * cols + (col & ~31)) * 2 + (col & 31);
+    half4 hi, lo;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        _Float16 h, l;
+        split(f[k], h, l);
+        hi[k] = h;
+        lo[k] = l;
+    }
+    *reinterpret_cast<half4 *>(p) = hi;
+    *reinterpret_cast<half4 *>(p + 32) = lo;
+}
+__device__ inline void get_split(const char *base, long cols, long row, int col, float (&f)[4])
+{
+    const _Float16 *p = reinterpret_cast<const _Float16 *>(base) + (row * cols + (col & ~31)) * 2 + (col & 31);
+    const half4 hi = *reinterpret_cast<const half4 *>(p), lo = *reinterpret_cast<const half4 *>(p + 32);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f[k] = (float)hi[k] + (float)lo[k];
+}
+
+// Writes the tile (i0, j0) of a symmetric matrix and its mirror image: value = mul * tile + (POLY: the rest of P = a I + b A + c A A).
+template <int TS, bool POLY>
+__device__ inline void put_symmetric(const float *tile, char *out, int mp, int i0, int j0, float mul, const char *A, float pa, float pb)
+{
+    constexpr int quads = TS / 4;
+    for (int pass = 0; pass < (i0 == j0 ? 1 : 2); ++pass)
+        for (int q = threadIdx.x; q < TS * quads; q += kThreads) {
+            const int r = q / quads, c = q % quads * 4;
+            const int row = (pass ? j0 : i0) + r, col = (pass ? i0 : j0) + c;
+            if (row >= mp || col >= mp) continue;
+            float f[4];
+            // the diagonal tile: both triangles hold the same products in another order; the upper one is taken for both, so
+            // that the matrix is symmetric to the last bit
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const bool turn = i0 == j0 ? r > c + k : pass == 1;
+                f[k] = mul * (turn ? tile[(c + k) * Geo<TS>::PITCH + r] : tile[r * Geo<TS>::PITCH + c + k]);
+            }
+            if (POLY) {
+                float g[4];
+                get_split(A, mp, row, col, g);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) f[k] += pb * g[k] + (row == col + k ? pa : 0.0f);
+            }
+            put_split(out, mp, row, col, f);
+        }
+}
+
+// tile number -> (i, j), j >= i, of a symmetric matrix of T x T tiles
+__device__ inline void triangle(int t, int T, int &i, int &j)
+{
+    i = 0;
+    while (t >= T - i) { t -= T - i; ++i; }
+    j = i + t;
+}
+
+// ---- phase 2: A = X X^T, k in pieces when there are few tiles; the pieces' sums go to the workspace as the threads hold them ----
+template <int TS> __global__ __launch_bounds__(kThreads, 2) void ortho_gram(Table t, char *ws, int seg)
+{
+    __shared__ __attribute__((aligned(16))) char lds[Geo<TS>::LDS];
+    const Mat &M = t.mats[find(t, PH_GRAM)];
+    const int T = (M.mp + TS - 1) / TS, tiles = T * (T + 1) / 2;
+    const int wg = blockIdx.x - M.first[PH_GRAM], bi = wg / (tiles * M.splits), rest = wg % (tiles * M.splits), tile = rest / M.splits, piece = rest % M.splits;
+    int ti, tj;
+    triangle(tile, T, ti, tj);
+    char *area = ws + M.ws + bi * M.area;
+    const char *X = area + buf_at(seg & 1 ? BUF_X1 : BUF_X0, M.mp, M.np);
+    const int lines = M.np / 32, k0 = (int)((long)lines * piece / M.splits), k1 = (int)((long)lines * (piece + 1) / M.splits);
+    Acc<TS> acc;
+    product<TS, false>(acc, lds, X, (long)M.np * 4, ti * TS, M.mp, X, (long)M.np * 4, tj * TS, M.mp, k0, k1);
+    if (M.splits > 1) {
+        float *part = reinterpret_cast<float *>(area + buf_at(BUF_PART, M.mp, M.np)) + ((long)tile * M.splits + piece) * TS * TS;
+#pragma unroll
+        for (int i = 0; i < Geo<TS>::FR; ++i)
+#pragma unroll
+            for (int j = 0; j < Geo<TS>::FR; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) part[((i * Geo<TS>::FR + j) * 16 + e) * kThreads + threadIdx.x] = acc.v[i][j][e];
+        return;
+    }
+    const int e = reinterpret_cast<const int *>(area + kMaxParts * 8)[seg];
+    put_symmetric<TS, false>(to_tile<TS>(acc, lds), area + buf_at(BUF_A, M.mp, M.np), M.mp, ti * TS, tj * TS, ldexpf(1.0f, kExpA - 2 * e), nullptr, 0.0f, 0.0f);
+}
+
+template <int TS> __global__ __launch_bounds__(kThreads) void ortho_join(Table t, char *ws, int seg)
+{
+    __shared__ __attribute__((aligned(16))) char lds[Geo<TS>::LDS];
+    const Mat &M = t.mats[find(t, PH_CHAIN)];
+    if (M.splits == 1) return;
+    const int T = (M.mp + TS - 1) / TS, tiles = T * (T + 1) / 2;
+    const int wg = blockIdx.x - M.first[PH_CHAIN], bi = wg / tiles, tile = wg % tiles;
+    int ti, tj;
+    triangle(tile, T, ti, tj);
+    char *area = ws + M.ws + bi * M.area;
+    const float *part = reinterpret_cast<const float *>(area + buf_at(BUF_PART, M.mp, M.np)) + (long)tile * M.splits * TS * TS;
+    Acc<TS> acc;
+#pragma unroll
+    for (int i = 0; i < Geo<TS>::FR; ++i)
+#pragma unroll
+        for (int j = 0; j < Geo<TS>::FR; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc.v[i][j][e] = 0.0f;
+    for (int s = 0; s < M.splits; ++s)
+#pragma unroll
+        for (int i = 0; i < Geo<TS>::FR; ++i)
+#pragma unroll
+            for (int j = 0; j < Geo<TS>::FR; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc.v[i][j][e] += part[(long)s * TS * TS + ((i * Geo<TS>::FR + j) * 16 + e) * kThreads + threadIdx.x];
+    const int e = reinterpret_cast<const int *>(area + kMaxParts * 8)[seg];
+    put_symmetric<TS, false>(to_tile<TS>(acc, lds), area + buf_at(BUF_A, M.mp, M.np), M.mp, ti * TS, tj * TS, ldexpf(1.0f, kExpA - 2 * e), nullptr, 0.0f, 0.0f);
+}
+
+// ---- phase 3: products of the m x m matrices ----------------------------------------------------------------------------------
+struct Chain {
+    int l[2], r[2], out[2];            // buffers of the (up to two, blockIdx.y) products of this launch
+    float mul[2];
+    int poly;                          // product 0 is A A, its result P
+    float pa, pb;
+};
+template <int TS> __global__ __launch_bounds__(kThreads, 2) void ortho_chain(Table t, char *ws, Chain c)
+{
+    __shared__ __attribute__((aligned(16))) char lds[Geo<TS>::LDS];
+    const Mat &M = t.mats[find(t, PH_CHAIN)];
+    const int T = (M.mp + TS - 1) / TS, tiles = T * (T + 1) / 2;
+    const int wg = blockIdx.x - M.first[PH_CHAIN], bi = wg / tiles, w = blockIdx.y;
+    int ti, tj;
+    triangle(wg % tiles, T, ti, tj);
+    char *area = ws + M.ws + bi * M.area;
+    const char *L = area + buf_at(c.l[w], M.mp, M.np), *R = area + buf_at(c.r[w], M.mp, M.np);
+    Acc<TS> acc;
+    product<TS, false>(acc, lds, L, (long)M.mp * 4, ti * TS, M.mp, R, (long)M.mp * 4, tj * TS, M.mp, 0, M.mp / 32);
+    const float *tile = to_tile<TS>(acc, lds);
+    char *out = area + buf_at(c.out[w], M.mp, M.np);
+    if (c.poly) put_symmetric<TS, true>(tile, out, M.mp, ti * TS, tj * TS, c.mul[w], L, c.pa, c.pb);
+    else put_symmetric<TS, false>(tile, out, M.mp, ti * TS, tj * TS, c.mul[w], nullptr, 0.0f, 0.0f);
+}
+
+// ---- phase 4: X' = Q X, into the other X, the caller's matrix, or the parameters -------------------------------------------------
+enum { TO_X = 0, TO_DST, TO_PARAM };
+template <int TS, typename T, int DEST> __global__ __launch_bounds__(kThreads, 2) void ortho_apply(Table t, char *ws, int seg, int q, int qexp, Step st)
+{
+    __shared__ __attribute__((aligned(16))) char lds[Geo<TS>::LDS];
+    const Mat &M = t.mats[find(t, PH_APPLY)];
+    const int Ti = (M.mp + TS - 1) / TS, Tj = (M.np + TS - 1) / TS;
+    const int wg = blockIdx.x - M.first[PH_APPLY], bi = wg / (Ti * Tj), ti = wg % (Ti * Tj) % Ti, tj = wg % (Ti * Tj) / Ti;
+    char *area = ws + M.ws + bi * M.area;
+    const char *X = area + buf_at(seg & 1 ? BUF_X1 : BUF_X0, M.mp, M.np);
+    const int *ex = reinterpret_cast<const int *>(area + kMaxParts * 8);
+    const int e0 = ex[seg], e1 = ex[seg + 1];
+    Acc<TS> acc;
+    product<TS, true>(acc, lds, area + buf_at(q, M.mp, M.np), (long)M.mp * 4, ti * TS, M.mp, X, (long)M.np * 4, tj * TS, M.np / 32, 0, M.mp / 32);
+    const float *tile = to_tile<TS>(acc, lds);
+    constexpr int quads = TS / 4;
+    if constexpr (DEST == TO_X) {
+        const float mul = ldexpf(1.0f, e1 - e0 - qexp);
+        char *out = area + buf_at(seg & 1 ? BUF_X0 : BUF_X1, M.mp, M.np);
+        for (int k = threadIdx.x; k < TS * quads; k += kThreads) {
+            const int r = k / quads, c = k % quads * 4;
+            if (ti * TS + r >= M.mp || tj * TS + c >= M.np) continue;
+            float f[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) f[x] = mul * tile[r * Geo<TS>::PITCH + c + x];
+            put_split(out, M.np, ti * TS + r, tj * TS + c, f);
+        }
+        return;
+    }
+    // the result, in the caller's orientation: row r of the output tile, four neighbours of it
+    const float mul = ldexpf(1.0f, -(e0 + qexp));
+    float keep = 1.0f, step = 1.0f;
+    if constexpr (DEST == TO_PARAM) {
+        keep = (float)(1.0 - st.hp[0] * st.hp[2]);
+        step = (float)(st.hp[0] * (double)M.scale);
+    }
+    const int R = M.tall ? M.n : M.m, C = M.tall ? M.m : M.n, r0 = (M.tall ? tj : ti) * TS, c0 = (M.tall ? ti : tj) * TS;
+    for (int k = threadIdx.x; k < TS * quads; k += kThreads) {
+        const int r = k / quads, c = k % quads * 4, row = r0 + r, col = c0 + c;
+        if (row >= R || col >= C) continue;
+        float f[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) f[x] = mul * (M.tall ? tile[(c + x) * Geo<TS>::PITCH + r] : tile[r * Geo<TS>::PITCH + c + x]);
+        if constexpr (DEST == TO_PARAM) {
+            float *p = st.p + (long)M.dst + (long)row * M.dst_ld + col;
+            if (col + 4 <= C) {
+                Pack<float, 4> o = *reinterpret_cast<const Pack<float, 4> *>(p);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) o.v[x] = o.v[x] * keep - step * f[x];
+                *reinterpret_cast<Pack<float, 4> *>(p) = o;
+            } else {
+                for (int x = 0; x < 4 && col + x < C; ++x) p[x] = p[x] * keep - step * f[x];
+            }
+        } else {
+            T *p = reinterpret_cast<T *>(M.dst) + bi * M.dst_stride + (long)row * M.dst_ld + col;
+            if (col + 4 <= C) {
+                Pack<T, 4> o;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) o.v[x] = from_f<T>(f[x]);
+                *reinterpret_cast<Pack<T, 4> *>(p) = o;
+            } else {
+                for (int x = 0; x < 4 && col + x < C; ++x) p[x] = from_f<T>(f[x]);
+            }
+        }
+    }
+}
+
+// ---- Adam for the vectors (the same arithmetic as tef_adam_clip_step, over a list of ranges of the flat buffers) --------------------
+constexpr int kRanges = 96;
+struct Ranges { long off[kRanges]; int first[kRanges + 1]; int v0; int n; };
+__global__ __launch_bounds__(kThreads) void muon_vectors(Ranges rg, float *p, float *g, float *m, float *v, const float *norm, const double *hp, const float *step)
+{
+    const float clip = clip_scale(norm, hp[3]);
+    const double b1 = hp[5], b2d = hp[6], t = (double)step[0];
+    const double bc1 = 1.0 - pow(b1, t), bc2 = 1.0 - pow(b2d, t);
+    const float step_size = (float)(hp[4] / bc1), bc2_sqrt = (float)sqrt(bc2), w1 = (float)(1.0 - b1), b2 = (float)b2d, w2 = (float)(1.0 - b2d), eps = (float)hp[7];
+    const int total = rg.first[rg.n];
+    for (int i = blockIdx.x * kThreads + threadIdx.x; i < total; i += gridDim.x * kThreads) {
+        int lo = 0, hi = rg.n - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (rg.first[mid] <= i) lo = mid;
+            else hi = mid - 1;
+        }
+        const long at = rg.off[lo] + (i - rg.first[lo]);
+        const float gr = g[at] * clip;
+        const float mm = m[at] + w1 * (gr - m[at]), vv = v[rg.v0 + i] * b2 + (w2 * gr) * gr;
+        m[at] = mm;
+        v[rg.v0 + i] = vv;
+        p[at] = p[at] - step_size * (mm / (sqrtf(vv) / bc2_sqrt + eps));
+        g[at] = 0.0f;
+    }
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------------------
+struct Poly { float a, b, c; int steps; int seg_len; };
+
+// The bounds that the fixed scales rely on, for singular values that start anywhere in [0, 1]: X and A stay below 2^2 (s < 4 would
+// square to 16: 2^12 * 16 = 65536 overflows fp16), P below 15, and Q of a segment below 60.
+bool bounded(Poly &p)
+{
+    double a = p.a, b = p.b, c = p.c;
+    if (!(isfinite(a) && isfinite(b) && isfinite(c))) return tef::fail("orthogonalisation: coefficients are not finite");
+    for (p.seg_len = kSegment; p.seg_len >= 1; --p.seg_len) {
+        bool ok = true;
+        for (int g = 0; g <= 512 && ok; ++g) {
+            double s = g / 512.0, q = 1.0;
+            for (int k = 0; k < p.steps && ok; ++k) {
+                const double l = s * s, poly = a + b * l + c * l * l;
+                if (k % p.seg_len == 0) q = 1.0;
+                q *= poly;
+                s *= poly;
+                if (!(fabs(poly) < 15.0 && fabs(s) < 3.9)) return tef::fail("orthogonalisation: these coefficients let a singular value grow past what the iteration can hold (|s| < 3.9, |p(s)/s| < 15)");
+                ok = fabs(q) < 60.0;
+            }
+        }
+        if (ok) return true;
+    }
+    return tef::fail("orthogonalisation: these coefficients grow too fast");
+}
+
+struct Group {
+    Mat m[kGroup];
+    int n;
+    long bytes;                        // workspace
+    int grid[5];
+    int ts_gram, ts_chain, ts_apply;
+    bool joined;
+};
+
+inline int round32(long v) { return (int)((v + 31) & ~31l); }
+
+// Tile sizes: 128 where the launch then still covers the 256 CUs, else 64 (a quarter of the work each, so that four times as many
+// workgroups share it).  The Gram product is cut along k until there are about two workgroups a CU, in pieces of at least
+// eight lines, since a piece's fp32 sums have to be written and read again.
+void plan(Group &g)
+{
+    long chain128 = 0, apply128 = 0, steps128 = 0;
+    for (int k = 0; k < g.n; ++k) {
+        const Mat &M = g.m[k];
+        const long T = (M.mp + 127) / 128;
+        chain128 += (long)M.batch * T * (T + 1) / 2;
+        apply128 += (long)M.batch * T * ((M.np + 127) / 128);
+        steps128 += (long)M.batch * T * (T + 1) / 2 * (M.np / 32);
+    }
+    g.ts_chain = chain128 >= 256 ? 128 : 64;
+    g.ts_gram = g.ts_chain;
+    g.ts_apply = apply128 >= 256 ? 128 : 64;
+    long steps = 0;
+    for (int k = 0; k < g.n; ++k) {
+        const Mat &M = g.m[k];
+        const long T = (M.mp + g.ts_gram - 1) / g.ts_gram;
+        steps += (long)M.batch * T * (T + 1) / 2 * (M.np / 32);
+    }
+    const long piece = steps / 512 > 8 ? steps / 512 : 8;
+    long at = 0, first[5] = {0, 0, 0, 0, 0};
+    g.joined = false;
+    at = (long)((sizeof(Mat) * kGroup + 255) & ~255ul);
+    for (int k = 0; k < g.n; ++k) {
+        Mat &M = g.m[k];
+        const long T = (M.mp + g.ts_gram - 1) / g.ts_gram, tiles = T * (T + 1) / 2, lines = M.np / 32;
+        long splits = (lines + piece - 1) / piece;
+        M.splits = (int)(splits < 1 ? 1 : splits > 64 ? 64 : splits);
+        if (M.splits > 1) g.joined = true;
+        const long total = (long)M.m * M.n;
+        long parts = (total + 16383) / 16384;
+        M.parts = (int)(parts < 1 ? 1 : parts > kMaxParts ? kMaxParts : parts);
+        M.area = buf_at(BUF_PART, M.mp, M.np) + (M.splits > 1 ? tiles * M.splits * g.ts_gram * g.ts_gram * 4 : 0);
+        M.area = (M.area + 255) & ~255l;
+        M.ws = at;
+        at += M.area * M.batch;
+        const long Ta = (M.mp + g.ts_apply - 1) / g.ts_apply, Tb = (M.np + g.ts_apply - 1) / g.ts_apply;
+        const long per[5] = {M.parts, (M.mp / 32) * ((M.np + 63l) / 64), tiles * M.splits, tiles, Ta * Tb};
+        for (int f = 0; f < 5; ++f) {
+            M.first[f] = (int)first[f];
+            first[f] += per[f] * M.batch;
+        }
+    }
+    for (int f = 0; f < 5; ++f) g.grid[f] = first[f] > 0x7fffffff ? -1 : (int)first[f];
+    g.bytes = at;
+}
+
+bool describe(Mat &M, long rows, long cols, long batch)
+{
+    if (rows < 1 || cols < 1 || batch < 1) return tef::fail("orthogonalisation: empty matrix");
+    const long m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
+    if (n > (1l << 24) || m > (1l << 15) || batch > (1l << 20)) return tef::fail("orthogonalisation: matrix sides up to 2^15 x 2^24, batches up to 2^20");
+    memset(&M, 0, sizeof(M));
+    M.m = (int)m; M.n = (int)n; M.mp = round32(m); M.np = round32(n);
+    M.tall = rows > cols;
+    M.batch = (int)batch;
+    return true;
+}
+
+#define TS_LAUNCH(ts, call128, call64) do { if ((ts) == 128) { call128; } else { call64; } } while (0)
+
+template <typename T, bool STEP>
+int iterate(Group &g, const Poly &p, double eps, char *ws, const Step &st, hipStream_t stream)
+{
+    for (int f = 0; f < 5; ++f)
+        if (g.grid[f] < 0) return tef::fail("orthogonalisation: too many tiles for one launch"), TEF_ERR_INVALID;
+    Mat *table = reinterpret_cast<Mat *>(ws);
+    const dim3 block(kThreads);
+    for (int at = 0; at < g.n; at += kChunk) {
+        Chunk ch;
+        ch.at = at;
+        ch.n = g.n - at < kChunk ? g.n - at : kChunk;
+        memcpy(ch.m, g.m + at, sizeof(Mat) * ch.n);
+        const int end = at + ch.n < g.n ? g.m[at + ch.n].first[PH_SQ] : g.grid[PH_SQ];
+        hipLaunchKernelGGL((ortho_squares<T, STEP>), dim3((unsigned)(end - ch.m[0].first[PH_SQ])), block, 0, stream, ch, table, ws, st);
+    }
+    const Table t{table, g.n};
+    hipLaunchKernelGGL((ortho_pack<T, STEP>), dim3((unsigned)g.grid[PH_PACK]), block, 0, stream, t, ws, eps, st);
+    const dim3 gram((unsigned)g.grid[PH_GRAM]), apply((unsigned)g.grid[PH_APPLY]);
+    // steps in segments of nearly equal length (5: 3 + 2)
+    const int segs = (p.steps + p.seg_len - 1) / p.seg_len;
+    int done = 0;
+    for (int s = 0; s < segs; ++s) {
+        const int len = (p.steps - done + segs - s - 1) / (segs - s);
+        done += len;
+        TS_LAUNCH(g.ts_gram, hipLaunchKernelGGL(ortho_gram<128>, gram, block, 0, stream, t, ws, s), hipLaunchKernelGGL(ortho_gram<64>, gram, block, 0, stream, t, ws, s));
+        if (g.joined)
+            TS_LAUNCH(g.ts_gram, hipLaunchKernelGGL(ortho_join<128>, dim3((unsigned)g.grid[PH_CHAIN]), block, 0, stream, t, ws, s),
+                      hipLaunchKernelGGL(ortho_join<64>, dim3((unsigned)g.grid[PH_CHAIN]), block, 0, stream, t, ws, s));
+        int q = -1;
+        for (int k = 0; k < len; ++k) {
+            const int P = k & 1 ? BUF_P1 : BUF_P0;
+            auto chain = [&](const Chain &c, int products) {
+                const dim3 grid((unsigned)g.grid[PH_CHAIN], (unsigned)products);
+                TS_LAUNCH(g.ts_chain, hipLaunchKernelGGL(ortho_chain<128>, grid, block, 0, stream, t, ws, c), hipLaunchKernelGGL(ortho_chain<64>, grid, block, 0, stream, t, ws, c));
+            };
+            // P = a I + b A + c A A
+            Chain c{};
+            c.l[0] = c.r[0] = BUF_A; c.out[0] = P; c.poly = 1;
+            c.mul[0] = ldexpf(p.c, kExpP - 2 * kExpA); c.pa = ldexpf(p.a, kExpP); c.pb = ldexpf(p.b, kExpP - kExpA);
+            chain(c, 1);
+            // W = A P and Q' = Q P, then A' = W P
+            Chain d{};
+            int products = 0;
+            if (k + 1 < len) {
+                d.l[products] = BUF_A; d.r[products] = P; d.out[products] = BUF_W; d.mul[products] = ldexpf(1.0f, kExpA - kExpA - kExpP);
+                ++products;
+            }
+            if (k > 0) {
+                const int out = q == BUF_Q0 ? BUF_Q1 : BUF_Q0;
+                d.l[products] = q; d.r[products] = P; d.out[products] = out;
+                d.mul[products] = ldexpf(1.0f, kExpQ - (q == BUF_Q0 || q == BUF_Q1 ? kExpQ : kExpP) - kExpP);
+                ++products;
+                q = out;
+            } else {
+                q = P;
+            }
+            if (products) chain(d, products);
+            if (k + 1 < len) {
+                Chain e{};
+                e.l[0] = BUF_W; e.r[0] = P; e.out[0] = BUF_A; e.mul[0] = ldexpf(1.0f, kExpA - kExpA - kExpP);
+                chain(e, 1);
+            }
+        }
+        const bool last = s + 1 == segs;
+        const int qexp = q == BUF_Q0 || q == BUF_Q1 ? kExpQ : kExpP;
+        if (!last) {
+            TS_LAUNCH(g.ts_apply, hipLaunchKernelGGL((ortho_apply<128, float, TO_X>), apply, block, 0, stream, t, ws, s, q, qexp, st),
+                      hipLaunchKernelGGL((ortho_apply<64, float, TO_X>), apply, block, 0, stream, t, ws, s, q, qexp, st));
+        } else {
+            constexpr int D = STEP ? TO_PARAM : TO_DST;
+            TS_LAUNCH(g.ts_apply, hipLaunchKernelGGL((ortho_apply<128, T, D>), apply, block, 0, stream, t, ws, s, q, qexp, st),
+                      hipLaunchKernelGGL((ortho_apply<64, T, D>), apply, block, 0, stream, t, ws, s, q, qexp, st));
+        }
+    }
+    return tef::check_launch("orthogonalisation");
+}
+
+bool polynomial(Poly &p, int steps, double a, double b, double c, double eps)
+{
+    if (steps < 1 || steps > kMaxSteps) return tef::fail("orthogonalisation: 1 to 32 steps");
+    if (!(eps > 0.0 && eps < 1e30)) return tef::fail("orthogonalisation: eps must be positive");
+    p = Poly{(float)a, (float)b, (float)c, steps, kSegment};
+    return bounded(p);
+}
+
+bool group_of(Group &g, const tef_ortho_matrix *m, int at, int count)
+{
+    g.n = count - at < kGroup ? count - at : kGroup;
+    for (int k = 0; k < g.n; ++k) {
+        const tef_ortho_matrix &d = m[at + k];
+        Mat &M = g.m[k];
+        if (!describe(M, d.rows, d.cols, d.batch)) return false;
+        if (d.src_ld < d.cols || d.dst_ld < d.cols) return tef::fail("orthogonalisation: row stride shorter than a row");
+        M.src = d.src; M.dst = d.dst;
+        M.src_ld = d.src_ld; M.dst_ld = d.dst_ld;
+        M.src_stride = d.src_stride; M.dst_stride = d.dst_stride;
+    }
+    plan(g);
+    return true;
+}
+
+bool group_of(Group &g, const tef_muon_matrix *m, int at, int count)
+{
+    g.n = count - at < kGroup ? count - at : kGroup;
+    for (int k = 0; k < g.n; ++k) {
+        const tef_muon_matrix &d = m[at + k];
+        Mat &M = g.m[k];
+        if (!describe(M, d.rows, d.cols, 1)) return false;
+        if (d.offset < 0) return tef::fail("tef_muon_step: negative offset");
+        M.src = reinterpret_cast<const void *>(d.offset); M.dst = reinterpret_cast<void *>(d.offset);
+        M.src_ld = M.dst_ld = d.cols;
+        M.scale = d.scale;
+    }
+    plan(g);
+    return true;
+}
+
+template <typename D> size_t workspace_of(const D *m, int count)
+{
+    if (count < 0 || (count && !m)) return tef::fail("orthogonalisation: null matrix list"), 0;
+    size_t most = 256;
+    Group g;
+    for (int at = 0; at < count; at += kGroup) {
+        if (!group_of(g, m, at, count)) return 0;
+        if ((size_t)g.bytes > most) most = (size_t)g.bytes;
+    }
+    return most;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t tef_orthogonalize_workspace_bytes(const tef_ortho_matrix *matrices, int count) { return workspace_of(matrices, count); }
+
+int tef_orthogonalize(const tef_ortho_matrix *matrices, int count, int dtype, int steps, double a, double b, double c, double eps,
+                      void *workspace, size_t workspace_bytes, void *stream)
+{
+    Poly p;
+    if (!polynomial(p, steps, a, b, c, eps)) return TEF_ERR_INVALID;
+    if (dtype < TEF_F32 || dtype > TEF_BF16) return tef::fail("tef_orthogonalize: type"), TEF_ERR_INVALID;
+    const size_t need = workspace_of(matrices, count);
+    if (!need) return TEF_ERR_INVALID;
+    if (count == 0) return 0;
+    for (int k = 0; k < count; ++k)
+        if (!matrices[k].src || !matrices[k].dst) return tef::fail("tef_orthogonalize: null pointer"), TEF_ERR_INVALID;
+    if (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < need)
+        return tef::fail("tef_orthogonalize: workspace too small or not 256-byte aligned"), TEF_ERR_WORKSPACE;
+    Group g;
+    for (int at = 0; at < count; at += kGroup) {
+        if (!group_of(g, matrices, at, count)) return TEF_ERR_INVALID;
+        const Step none{};
+        const int rc = dtype == TEF_F32 ? iterate<float, false>(g, p, eps, (char *)workspace, none, (hipStream_t)stream)
+                     : dtype == TEF_F16 ? iterate<__half, false>(g, p, eps, (char *)workspace, none, (hipStream_t)stream)
+                                        : iterate<__hip_bfloat16, false>(g, p, eps, (char *)workspace, none, (hipStream_t)stream);
+        if (rc) return rc;
+    }
+    return 0;
+}
+
+size_t tef_muon_workspace_bytes(const tef_muon_matrix *matrices, int count) { return workspace_of(matrices, count); }
+
+int tef_muon_step(float *p, float *g, float *m, float *v, const tef_muon_matrix *matrices, int nmatrices, const tef_muon_vector *vectors,
+                  int nvectors, const float *norm, const double *hp, const float *step, int nesterov, int steps, double a, double b,
+                  double c, double eps, void *workspace, size_t workspace_bytes, void *stream)
+{
+    Poly poly;
+    if (!polynomial(poly, steps, a, b, c, eps)) return TEF_ERR_INVALID;
+    if (!p || !g || !m || !norm || !hp || !step || nvectors < 0 || (nvectors && (!vectors || !v)))
+        return tef::fail("tef_muon_step: null pointer"), TEF_ERR_INVALID;
+    long total = 0;
+    for (int k = 0; k < nvectors; ++k) {
+        if (vectors[k].offset < 0 || vectors[k].size < 1) return tef::fail("tef_muon_step: empty or misplaced vector"), TEF_ERR_INVALID;
+        total += vectors[k].size;
+    }
+    if (total > 0x3fffffff) return tef::fail("tef_muon_step: more than 2^30 vector elements"), TEF_ERR_INVALID;
+    const size_t need = workspace_of(matrices, nmatrices);
+    if (!need) return TEF_ERR_INVALID;
+    if (nmatrices && (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < need))
+        return tef::fail("tef_muon_step: workspace too small or not 256-byte aligned"), TEF_ERR_WORKSPACE;
+    hipStream_t st = (hipStream_t)stream;
+    const Step s{g, m, p, norm, hp, nesterov != 0};
+    Group gr;
+    for (int at = 0; at < nmatrices; at += kGroup) {
+        if (!group_of(gr, matrices, at, nmatrices)) return TEF_ERR_INVALID;
+        const int rc = iterate<float, true>(gr, poly, eps, (char *)workspace, s, st);
+        if (rc) return rc;
+    }
+    long v0 = 0;
+    for (int at = 0; at < nvectors; at += kRanges) {
+        Ranges rg;
+        rg.n = nvectors - at < kRanges ? nvectors - at : kRanges;
+        rg.v0 = (int)v0;
+        rg.first[0] = 0;
+        for (int k = 0; k < rg.n; ++k) {
+            rg.off[k] = vectors[at + k].offset;
+            rg.first[k + 1] = rg.first[k] + (int)vectors[at + k].size;
+        }
+        const int n = rg.first[rg.n];
+        v0 += n;
+        const int blocks = (n + kThreads - 1) / kThreads;
+        hipLaunchKernelGGL(muon_vectors, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(kThreads), 0, st, rg, p, g, m, v, norm, hp, step);
+    }
+    return tef::check_launch("muon step");
+}
+
+}  // extern "C"

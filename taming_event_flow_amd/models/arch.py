@@ -27,6 +27,8 @@ Row = namedtuple("Row", "kind level cin cout ksize stride act")
 class NetPlan:
     """Static description of the network: `rows` lists every convolution (in state_dict order)."""
 
+    norm = None      # (plans pickled before there was a choice)
+
     def __init__(self, num_bins, base_channels=64, num_encoders=4, num_residual_blocks=2, num_output_channels=2,
                  skip_type="sum", norm=None, use_upsample_conv=True, kernel_size=3, encoder_stride=2, channel_multiplier=2,
                  activations=("relu", None), final_activation=None, final_bias=True, final_w_scale=None,
@@ -34,7 +36,7 @@ class NetPlan:
         unsupported = []
         if skip_type != "sum":
             unsupported.append(f"skip_type={skip_type!r}")
-        if norm is not None:
+        if norm not in (None, "LN"):
             unsupported.append(f"norm={norm!r}")
         if not use_upsample_conv:
             unsupported.append("transposed-convolution decoders")
@@ -49,6 +51,7 @@ class NetPlan:
                                       + ", ".join(unsupported))
         self.num_bins, self.levels, self.nres, self.nout = num_bins, num_encoders, num_residual_blocks, num_output_channels
         self.stride, self.ksize = encoder_stride, kernel_size
+        self.norm = norm        # "LN": layer-normalised convolutions (not the reference's default); such a network runs layer by layer
         self.final_activation, self.final_bias, self.final_w_scale = final_activation, final_bias, final_w_scale
         self.width = [int(base_channels * channel_multiplier ** i) for i in range(num_encoders)]     # 64, 128, 256, 512
         self.multiple = encoder_stride ** num_encoders if min_size is None else min_size
@@ -87,9 +90,9 @@ class MultiResUNetRecurrent(nn.Module):
         self.num_encoders = self.num_states = plan.levels
         self.encoders = nn.ModuleList(
             RecurrentConvLayer(r.cin, r.cout, kernel_size=r.ksize, stride=r.stride, recurrent_block_type="convgru",
-                               activation_ff=r.act, activation_rec=None) for r in plan.of("head"))
-        self.resblocks = nn.ModuleList(ResidualBlock(r.cin, r.cout, activation=r.act) for r in plan.of("res"))
-        self.decoders = nn.ModuleList(UpsampleConvLayer(r.cin, r.cout, kernel_size=r.ksize, activation=r.act)
+                               activation_ff=r.act, activation_rec=None, norm=plan.norm) for r in plan.of("head"))
+        self.resblocks = nn.ModuleList(ResidualBlock(r.cin, r.cout, activation=r.act, norm=plan.norm) for r in plan.of("res"))
+        self.decoders = nn.ModuleList(UpsampleConvLayer(r.cin, r.cout, kernel_size=r.ksize, activation=r.act, norm=plan.norm)
                                       for r in plan.of("dec"))
         self.preds = nn.ModuleList(ConvLayer(r.cin, r.cout, 1, activation=r.act, w_scale=plan.final_w_scale,
                                              bias=plan.final_bias) for r in plan.of("pred"))
@@ -119,6 +122,8 @@ class MultiResUNetRecurrent(nn.Module):
 
     @property
     def engine(self):
+        if self.plan.norm is not None:          # the fused pass has no normalisation between a convolution and its activation
+            return None
         if self._engine is None:
             self._engine = PassEngine(self)
         return self._engine
@@ -204,6 +209,8 @@ class MultiResUNetRecurrent(nn.Module):
     def encode(self, x):
         """The encoder half of one pass: updates `states` and queues the pass for decode_window().  Needs the training
         loop's in-place gradient buffers (direct_grads) like every split pass."""
+        if self.engine is None:
+            raise NotImplementedError("window mode runs on the fused pass, which a network with normalisation layers does not have")
         # (first: no pass of this window has gone onto the level streams yet — a fresh sequence's first pass does not)
         new_states, rec = encode_pass(self.engine, x, self.states, first=not any(r.hub is not None for r, _ in self._window))
         self.states = new_states
@@ -221,7 +228,20 @@ class MultiResUNetRecurrent(nn.Module):
 
     def step(self, x):
         """One fused pass on an input of any size: -> 4 flows at the input resolution, coarse to fine; updates `states`."""
+        if self.plan.norm is not None:
+            return self._step_layers(x)
         flows, self.states = run_pass(self.engine, x, self.states)
+        return flows
+
+    def _step_layers(self, x):
+        """step() through the modules' own autograd nodes: zero rows / columns at the top / left until every level halves exactly, the
+        predictions up-sampled to the input's size and scaled with it, the added rows / columns cut off."""
+        ph, pw = self.plan.padding(x.shape[-2], x.shape[-1])
+        preds = self.forward(nn.functional.pad(x, (pw, 0, ph, 0)) if ph or pw else x)
+        flows = []
+        for k, p in enumerate(preds):
+            s = self.plan.stride ** (self.plan.levels - 1 - k)
+            flows.append(upsample_bilinear(p, s, s, float(s) * self.flow_scale)[..., ph:, pw:])
         return flows
 
     def forward(self, x):
@@ -229,10 +249,11 @@ class MultiResUNetRecurrent(nn.Module):
         2**num_encoders, as the reference's forward (:217-242) returns them: layer by layer through the modules' own
         autograd nodes.  RecEVFlowNet does not come through here (it calls `step`); this path exists for users of the
         bare architecture and as the independent check of the fused pass (tests/test_model_gpu.py)."""
-        feats, cur = [], x
+        feats, cur, states = [], x, list(self.states)
         for i, enc in enumerate(self.encoders):
-            cur, self.states[i] = enc(cur, self.states[i])
+            cur, states[i] = enc(cur, states[i])
             feats.append(cur)
+        self.states = states      # (a new list, as step() assigns: a captured window holds on to the one it started from)
         for rb in self.resblocks:
             cur, _ = rb(cur)
         preds = []

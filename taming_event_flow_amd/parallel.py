@@ -74,6 +74,8 @@ class FusedAdam:
     operands of the convolutions are keyed on the parameters' version counters, which a kernel behind autograd's back
     does not bump: the caller invalidates them after every step (models.submodules.invalidate_packed)."""
 
+    _MAX_NORM_AT = 4       # of the clipping norm among _hyperparams()
+
     def __init__(self, bucket, lr, betas=(0.9, 0.999), eps=1e-8):
         import ctypes
 
@@ -146,6 +148,11 @@ class FusedAdam:
             if k != "params":
                 self.param_groups[0][k] = tuple(v) if k == "betas" else v
 
+    def _hyperparams(self, max_norm):
+        """The numbers the kernel reads from device memory, in its order."""
+        g = self.param_groups[0]
+        return (float(g["lr"]), float(g["betas"][0]), float(g["betas"][1]), float(g["eps"]), float(max_norm))
+
     def refresh_hyperparams(self, max_norm=None):
         """Upload (lr, betas, eps, max_norm) if any of them changed since the last upload.  Called by step() outside graph
         capture and by CapturedWindow.replay() before the graph is launched — there with the window's OWN capture-time
@@ -153,13 +160,11 @@ class FusedAdam:
         values go through a small ring of pinned host buffers with a non-blocking copy: stream-ordered before whatever is
         enqueued next, and the host does not wait for the previous window to drain (a per-step learning-rate schedule would
         otherwise serialise host and device at every replay)."""
-        g = self.param_groups[0]
-        mn = self._max_norm if max_norm is None else float(max_norm)
-        vals = (float(g["lr"]), float(g["betas"][0]), float(g["betas"][1]), float(g["eps"]), float(mn))
+        vals = self._hyperparams(self._max_norm if max_norm is None else max_norm)
         if vals != self._hp_uploaded:
             if self.hp.is_cuda:
                 if self._hp_ring is None:
-                    self._hp_ring = [(torch.empty((5,), dtype=torch.float64).pin_memory(), torch.cuda.Event()) for _ in range(8)]
+                    self._hp_ring = [(torch.empty((len(vals),), dtype=torch.float64).pin_memory(), torch.cuda.Event()) for _ in range(8)]
                     self._hp_next = 0
                 buf, ev = self._hp_ring[self._hp_next % len(self._hp_ring)]
                 if self._hp_next >= len(self._hp_ring):
@@ -183,14 +188,19 @@ class FusedAdam:
         self._max_norm = -1.0 if max_norm is None else float(max_norm)
         if not (self.hp.is_cuda and torch.cuda.is_current_stream_capturing()):
             self.refresh_hyperparams()      # (inside a capture: the values are uploaded before every replay instead)
-        elif self._hp_uploaded is None or self._hp_uploaded[4] != self._max_norm:
-            raise RuntimeError("FusedAdam.step: captured with a max_norm no eager step has uploaded (run a warm-up window)")
+        elif self._hp_uploaded is None or self._hp_uploaded[self._MAX_NORM_AT] != self._max_norm:
+            raise RuntimeError(f"{type(self).__name__}.step: captured with a max_norm no eager step has uploaded (run a warm-up window)")
         self._lib.check(lib.tef_l2_norm(self.bucket.flat.data_ptr(), n, self.scratch.data_ptr(), self.norm.data_ptr(),
                                         self.step_count.data_ptr(), st), "tef_l2_norm")
-        self._lib.check(lib.tef_adam_clip_step_hp(self.flat_p.data_ptr(), self.bucket.flat.data_ptr(), self.m.data_ptr(),
-                                                  self.v.data_ptr(), n, self.norm.data_ptr(), self.hp.data_ptr(),
-                                                  self.step_count.data_ptr(), st), "tef_adam_clip_step_hp")
+        self._update(st)
         return self.norm.view(())
+
+    def _update(self, stream):
+        """What follows the norm: the clipped update of the parameters, and the gradient cleared."""
+        self._lib.check(self._lib.lib().tef_adam_clip_step_hp(self.flat_p.data_ptr(), self.bucket.flat.data_ptr(), self.m.data_ptr(),
+                                                              self.v.data_ptr(), self.bucket.flat.numel(), self.norm.data_ptr(),
+                                                              self.hp.data_ptr(), self.step_count.data_ptr(), stream),
+                        "tef_adam_clip_step_hp")
 
 
 _FLAG_GROUP = None

@@ -17,6 +17,7 @@ from .dataloader import base as dl_base
 from .loss.flow import Iterative, Linear  # noqa: F401  (selected by name like the reference's eval(...))
 from .models import submodules
 from .models.model import RecEVFlowNet  # noqa: F401
+from .optim import FusedMuon
 
 DEFAULT_CONFIG = {     # reference configs/train_flow.yml
     "data": {"passes_loss": 10, "scales_loss": 1, "voxel": None},
@@ -259,6 +260,10 @@ class Trainer:
             # the optimiser-like surface callers reach for (param_groups[0]["lr"] for schedulers, state_dict /
             # load_state_dict for checkpoints, zero_grad); TEF_TORCH_ADAM=1 puts torch.optim.Adam here instead
             self.optimizer = self.fused_opt
+        elif config["optimizer"]["name"] == "Muon":
+            # orthogonalised updates for the matrices, Adam for the vectors (optim.FusedMuon's keyword arguments in the config)
+            self.fused_opt = self.optimizer = FusedMuon(self.bucket, config["optimizer"]["lr"],
+                                                        **{k: config["optimizer"][k] for k in extra})
         else:
             self.optimizer = getattr(torch.optim, config["optimizer"]["name"])(self.model.parameters(), **opt_kwargs)
         self.last_loss = None
@@ -290,6 +295,8 @@ class Trainer:
         # larger.  The loss container's update() calls follow it, the batches of the window stay referenced until then.
         self.window_decode = (eng is not None and torch.device(device).type == "cuda" and hasattr(self.model.arch, "encode")
                               and os.environ.get("TEF_WINDOW_DECODE", "1") != "0") if window_decode is None else bool(window_decode)
+        if self.window_decode and eng is None:
+            raise ValueError("window_decode=True needs the fused pass (a network without normalisation layers on a HIP device)")
         self._win_inputs = []
         if self.window_decode and hasattr(self.loss_function, "defer_update"):
             # the P update() calls of a window follow its batched decoders back to back: packed in ONE launch when the loss is
