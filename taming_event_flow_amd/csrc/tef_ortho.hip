@@ -58,9 +58,9 @@ struct Mat {
     int parts;                         // partial sums of squares per batch element
     int splits;                        // pieces of the Gram product's k
     float scale;                       // of the applied update (optimiser)
-    int first[5];                      // first workgroup in the launch of each phase (below)
+    int first[6];                       // first workgroup in the launch of each phase (below)
 };
-enum { PH_SQ = 0, PH_PACK, PH_GRAM, PH_CHAIN, PH_APPLY };
+enum { PH_SQ = 0, PH_PACK, PH_GRAM, PH_JOIN, PH_CHAIN, PH_APPLY, PHASES };
 
 // One batch element's area: doubles parts[kMaxParts], int exponents[kMaxSteps + 1], then the split matrices.
 __host__ __device__ inline long split_bytes(long rows, long cols) { return rows * cols * 4; }
@@ -75,12 +75,19 @@ __host__ __device__ inline long buf_at(int which, int mp, int np)
 
 struct Table { const Mat *mats; int count; };
 
-// Which matrix a workgroup of a phase belongs to: `first` is ascending, the wave looks at up to 64 of them at once.
-__device__ inline int find(const Table &t, int phase)
+// The work item of a workgroup: consecutive ones — tiles that read the same rows — go to ONE of the 8 XCDs (workgroups are dealt to
+// them in turn), so that a matrix is read into one L2 instead of all eight.
+__device__ inline int work_item()
+{
+    const int total = gridDim.x * gridDim.y, lin = blockIdx.y * gridDim.x + blockIdx.x, xcd = lin & 7, each = total >> 3, more = total & 7;
+    return xcd * each + (xcd < more ? xcd : more) + (lin >> 3);
+}
+// Which matrix an item of a phase belongs to: `first` is ascending, the wave looks at up to 64 of them at once.
+__device__ inline int find(const Table &t, int phase, int item)
 {
     const int lane = threadIdx.x & 63;
     const int f = lane < t.count ? t.mats[lane].first[phase] : 0x7fffffff;
-    return __popcll(__ballot(f <= (int)blockIdx.x)) - 1;
+    return __popcll(__ballot(f <= item)) - 1;
 }
 
 template <typename T> __device__ inline float to_f(T v);
@@ -193,7 +200,7 @@ template <typename T, bool STEP> __global__ __launch_bounds__(kThreads) void ort
 {
     __shared__ double red[4];
     __shared__ float turn[64][33];
-    const Mat &M = t.mats[find(t, PH_PACK)];
+    const Mat &M = t.mats[find(t, PH_PACK, (int)blockIdx.x)];
     const int tiles_n = (M.np + 63) / 64, tiles = (M.mp / 32) * tiles_n;
     const int wg = blockIdx.x - M.first[PH_PACK], bi = wg / tiles, ti = wg % tiles / tiles_n, tj = wg % tiles % tiles_n;
     char *area = ws + M.ws + bi * M.area;
@@ -280,32 +287,34 @@ template <typename T, bool STEP> __global__ __launch_bounds__(kThreads) void ort
 
 // ---- the products -----------------------------------------------------------------------------------------------------------
 // A workgroup of four waves computes TS x TS values (TS = 128 or 64), each wave a quarter of them in 32 x 32 blocks.  k advances
-// by 32: TS lines of 128 bytes per operand, from global memory through registers into LDS while the previous step's lines
-// are multiplied (two buffers, one barrier a step).  The 16-byte chunks of a line are permuted by the row, chunk ^ (row & 7), so that the eight
+// by one line of 32 a stage, from global memory through registers (AHEAD stages in flight) into LDS while the previous stage is
+// multiplied: two buffers, one barrier a stage.  The 16-byte chunks of a row are permuted by the row, chunk ^ (row & 7), so that the eight
 // lanes of an LDS cycle that read the same chunk of eight rows meet eight different bank groups.
 template <int TS> struct Geo {
     static constexpr int FR = TS / 64;                       // 32 x 32 blocks of a wave along each side
-    static constexpr int LOADS = TS * 8 / kThreads;          // 16-byte chunks of an operand's step per thread
-    static constexpr int STAGE = TS * 128;                   // bytes of an operand's step
+    static constexpr int STAGE = TS * 128;                   // bytes of an operand's stage
+    static constexpr int LOADS = STAGE / 16 / kThreads;      // 16-byte chunks of it per thread
     static constexpr int PITCH = TS + 4;                     // floats; the finished tile
     static constexpr int LDS = 4 * STAGE > TS * PITCH * 4 ? 4 * STAGE : TS * PITCH * 4;
 };
 
-// operand whose rows run along k: chunk q of the tile = row q / 8, chunk q % 8
+// operand whose rows run along k: a row's 8 chunks side by side
 template <int TS> __device__ inline void load_rows(uint4v (&r)[Geo<TS>::LOADS], const char *base, long ld, int row0, int rows, int kb)
 {
+    constexpr int per = 8;
 #pragma unroll
     for (int i = 0; i < Geo<TS>::LOADS; ++i) {
-        const int q = threadIdx.x + i * kThreads, row = row0 + (q >> 3);
-        r[i] = *reinterpret_cast<const uint4v *>(base + (long)(row < rows ? row : rows - 1) * ld + (long)kb * 128 + (q & 7) * 16);
+        const int q = threadIdx.x + i * kThreads, row = row0 + q / per;
+        r[i] = *reinterpret_cast<const uint4v *>(base + (long)(row < rows ? row : rows - 1) * ld + (long)kb * 128 + (q % per) * 16);
     }
 }
 template <int TS> __device__ inline void put_rows(char *lds, const uint4v (&r)[Geo<TS>::LOADS])
 {
+    constexpr int per = 8;
 #pragma unroll
     for (int i = 0; i < Geo<TS>::LOADS; ++i) {
-        const int q = threadIdx.x + i * kThreads, row = q >> 3;
-        *reinterpret_cast<uint4v *>(lds + row * 128 + (((q & 7) ^ (row & 7)) << 4)) = r[i];
+        const int q = threadIdx.x + i * kThreads, row = q / per;
+        *reinterpret_cast<uint4v *>(lds + row * (per * 16) + (((q % per) ^ (row & 7)) << 4)) = r[i];
     }
 }
 // rows `row` (this lane's), k = 16 * s + 8 * (lane >> 5) ..: plane 0 hi, 1 lo
@@ -314,8 +323,8 @@ __device__ inline half8 frag_rows(const char *lds, int row, int s, int plane)
     const int chunk = plane * 4 + s * 2 + ((threadIdx.x & 63) >> 5);
     return *reinterpret_cast<const half8 *>(lds + row * 128 + ((chunk ^ (row & 7)) << 4));
 }
-// operand whose COLUMNS are the tile's (X in Q X): a step is 32 rows of TS / 32 lines.  64-byte slots (one plane of one line) are
-// permuted by the row; ds_read_b64_tr_b16 hands every lane four consecutive k of its column.
+// operand whose COLUMNS are the tile's (X in Q X): a stage is 32 rows of TS / 32 lines.  64-byte slots (one plane of one line)
+// are permuted by the row; ds_read_b64_tr_b16 hands every lane four consecutive k of its column.
 template <int TS> __device__ inline void load_cols(uint4v (&r)[Geo<TS>::LOADS], const char *base, long ld, int blk0, int blks, int kb)
 {
     constexpr int per = TS / 4;      // chunks of a row
@@ -355,7 +364,7 @@ template <int TS> __device__ inline half8 frag_cols(const char *lds, int col0, i
 template <int TS> struct Acc { float16v v[Geo<TS>::FR][Geo<TS>::FR]; };
 
 // acc = L (rows li0 ..) times R (rows rj0 .. as columns, or, COLS, the 32-column blocks rj0 / 32 ..), k lines k0 .. k1
-template <int TS, bool COLS>
+template <int TS, int AHEAD, bool COLS>
 __device__ inline void product(Acc<TS> &acc, char *lds, const char *L, long ldL, int li0, int rowsL, const char *R, long ldR, int rj0, int limR, int k0, int k1)
 {
     using G = Geo<TS>;
@@ -366,21 +375,28 @@ __device__ inline void product(Acc<TS> &acc, char *lds, const char *L, long ldL,
         for (int j = 0; j < G::FR; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc.v[i][j][e] = 0.0f;
-    uint4v a[G::LOADS], b[G::LOADS];
-    load_rows<TS>(a, L, ldL, li0, rowsL, k0);
-    if (COLS) load_cols<TS>(b, R, ldR, rj0 >> 5, limR, k0);
-    else load_rows<TS>(b, R, ldR, rj0, limR, k0);
+    uint4v a[AHEAD][G::LOADS], b[AHEAD][G::LOADS];
+    // (past the end the last line is fetched again: no branch around the loads)
+#define TEF_FETCH(slot, line)                                                              \
+    do {                                                                                   \
+        const int at_ = (line) < k1 ? (line) : k1 - 1;                                     \
+        load_rows<TS>(a[slot], L, ldL, li0, rowsL, at_);                                   \
+        if (COLS) load_cols<TS>(b[slot], R, ldR, rj0 >> 5, limR, at_);                     \
+        else load_rows<TS>(b[slot], R, ldR, rj0, limR, at_);                               \
+    } while (0)
+#define TEF_PUT(slot, buf)                                                                 \
+    do {                                                                                   \
+        put_rows<TS>(lds + (buf) * 2 * G::STAGE, a[slot]);                                 \
+        if (COLS) put_cols<TS>(lds + (buf) * 2 * G::STAGE + G::STAGE, b[slot]);            \
+        else put_rows<TS>(lds + (buf) * 2 * G::STAGE + G::STAGE, b[slot]);                 \
+    } while (0)
+#pragma unroll
+    for (int d = 0; d < AHEAD; ++d) TEF_FETCH(d, k0 + d);
     __syncthreads();      // (whoever used this LDS before is done with it)
-    put_rows<TS>(lds, a);
-    if (COLS) put_cols<TS>(lds + G::STAGE, b);
-    else put_rows<TS>(lds + G::STAGE, b);
+    TEF_PUT(0, 0);
     __syncthreads();
-    for (int kb = k0; kb < k1; ++kb) {
-        const char *la = lds + ((kb - k0) & 1) * 2 * G::STAGE, *lb = la + G::STAGE;
-        const int next = kb + 1 < k1 ? kb + 1 : kb;      // (the last step fetches its own lines again: no branch around the loads)
-        load_rows<TS>(a, L, ldL, li0, rowsL, next);
-        if (COLS) load_cols<TS>(b, R, ldR, rj0 >> 5, limR, next);
-        else load_rows<TS>(b, R, ldR, rj0, limR, next);
+    auto multiply = [&](int d) {      // the line in LDS buffer d & 1
+        const char *la = lds + (d & 1) * 2 * G::STAGE, *lb = la + G::STAGE;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             half8 fa[G::FR][2], fb[G::FR][2];
@@ -399,16 +415,58 @@ __device__ inline void product(Acc<TS> &acc, char *lds, const char *L, long ldL,
                     for (int j = 0; j < G::FR; ++j)
                         acc.v[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[i][t == 0], fb[j][t == 1], acc.v[i][j], 0, 0, 0);
         }
-        char *other = lds + ((kb + 1 - k0) & 1) * 2 * G::STAGE;
-        put_rows<TS>(other, a);
-        if (COLS) put_cols<TS>(other + G::STAGE, b);
-        else put_rows<TS>(other + G::STAGE, b);
-        __syncthreads();
+    };
+    int kb = k0;
+    for (; kb + AHEAD <= k1; kb += AHEAD) {      // (no way out in between: a wait would have to cover loads of both paths)
+#pragma unroll
+        for (int d = 0; d < AHEAD; ++d) {        // line kb + d lies in LDS buffer d & 1, the following AHEAD - 1 on their way in registers
+            TEF_FETCH(d, kb + d + AHEAD);
+            multiply(d);
+            TEF_PUT((d + 1) % AHEAD, (d + 1) & 1);
+            __syncthreads();
+        }
     }
+#pragma unroll
+    for (int d = 0; d + 1 < AHEAD; ++d)
+        if (kb + d < k1) {
+            multiply(d);
+            TEF_PUT(d + 1, (d + 1) & 1);
+            __syncthreads();
+        }
+#undef TEF_FETCH
+#undef TEF_PUT
 }
 
-// the finished tile, row-major in LDS (32 x 32 block: column lane & 31, row 8 (e / 4) + 4 (lane >> 5) + e % 4)
-template <int TS> __device__ inline float *to_tile(const Acc<TS> &acc, char *lds)
+// The finished tile in LDS, row-major or, TURN, transposed (a lane of a 32 x 32 block holds column lane & 31 and the rows
+// 8 (e / 4) + 4 (lane >> 5) + e % 4: four neighbours of a row of the transposed tile, one 16-byte write); either way free of
+// bank conflicts, and read back in rows.
+template <int TS, bool TURN> __device__ inline float *to_tile(const Acc<TS> &acc, char *lds)
+{
+    using G = Geo<TS>;
+    typedef float float4v __attribute__((ext_vector_type(4)));
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = (wave >> 1) * (TS / 2), wj = (wave & 1) * (TS / 2);
+    float *tile = reinterpret_cast<float *>(lds);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < G::FR; ++i)
+#pragma unroll
+        for (int j = 0; j < G::FR; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int row = wi + i * 32 + 8 * e + 4 * (lane >> 5), col = wj + j * 32 + (lane & 31);
+                if (TURN) {
+                    *reinterpret_cast<float4v *>(tile + col * G::PITCH + row) = float4v{acc.v[i][j][4 * e], acc.v[i][j][4 * e + 1], acc.v[i][j][4 * e + 2], acc.v[i][j][4 * e + 3]};
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) tile[(row + k) * G::PITCH + col] = acc.v[i][j][4 * e + k];
+                }
+            }
+    __syncthreads();
+    return tile;
+}
+
+// a diagonal tile: its upper triangle, and that mirrored
+template <int TS> __device__ inline float *to_tile_upper(const Acc<TS> &acc, char *lds)
 {
     using G = Geo<TS>;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = (wave >> 1) * (TS / 2), wj = (wave & 1) * (TS / 2);
@@ -419,61 +477,75 @@ template <int TS> __device__ inline float *to_tile(const Acc<TS> &acc, char *lds
 #pragma unroll
         for (int j = 0; j < G::FR; ++j)
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-                tile[(wi + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * G::PITCH + wj + j * 32 + (lane & 31)] = acc.v[i][j][e];
+            for (int e = 0; e < 16; ++e) {
+                const int row = wi + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3), col = wj + j * 32 + (lane & 31);
+                if (row <= col) {
+                    tile[row * G::PITCH + col] = acc.v[i][j][e];
+                    tile[col * G::PITCH + row] = acc.v[i][j][e];
+                }
+            }
     __syncthreads();
     return tile;
 }
 
-// four neighbouring values of a split matrix's row
-__device__ inline void put_split(char *base, long cols, long row, int col, const float (&f)[4])
+// eight neighbouring values of a split matrix's row
+__device__ inline _Float16 *split_at(char *base, long cols, long row, int col)
 {
-    _Float16 *p = reinterpret_cast<_Float16 *>(base) + (row * cols + (col & ~31)) * 2 + (col & 31);
-    half4 hi, lo;
+    return reinterpret_cast<_Float16 *>(base) + (row * cols + (col & ~31)) * 2 + (col & 31);
+}
+__device__ inline void put_split(char *base, long cols, long row, int col, const float (&f)[8])
+{
+    _Float16 *p = split_at(base, cols, row, col);
+    half8 hi, lo;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < 8; ++k) {
         _Float16 h, l;
         split(f[k], h, l);
         hi[k] = h;
         lo[k] = l;
     }
-    *reinterpret_cast<half4 *>(p) = hi;
-    *reinterpret_cast<half4 *>(p + 32) = lo;
-}
-__device__ inline void get_split(const char *base, long cols, long row, int col, float (&f)[4])
-{
-    const _Float16 *p = reinterpret_cast<const _Float16 *>(base) + (row * cols + (col & ~31)) * 2 + (col & 31);
-    const half4 hi = *reinterpret_cast<const half4 *>(p), lo = *reinterpret_cast<const half4 *>(p + 32);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) f[k] = (float)hi[k] + (float)lo[k];
+    *reinterpret_cast<half8 *>(p) = hi;
+    *reinterpret_cast<half8 *>(p + 32) = lo;
 }
 
-// Writes the tile (i0, j0) of a symmetric matrix and its mirror image: value = mul * tile + (POLY: the rest of P = a I + b A + c A A).
+// Writes rows row0 .. of the tile in LDS to the split matrix `out`, from column col0 on: mul * value + (POLY: the rest of
+// P = a I + b A + c A A).
 template <int TS, bool POLY>
-__device__ inline void put_symmetric(const float *tile, char *out, int mp, int i0, int j0, float mul, const char *A, float pa, float pb)
+__device__ inline void put_tile(const float *tile, char *out, int rows, int cols, int row0, int col0, float mul, char *A, float pa, float pb)
 {
-    constexpr int quads = TS / 4;
-    for (int pass = 0; pass < (i0 == j0 ? 1 : 2); ++pass)
-        for (int q = threadIdx.x; q < TS * quads; q += kThreads) {
-            const int r = q / quads, c = q % quads * 4;
-            const int row = (pass ? j0 : i0) + r, col = (pass ? i0 : j0) + c;
-            if (row >= mp || col >= mp) continue;
-            float f[4];
-            // the diagonal tile: both triangles hold the same products in another order; the upper one is taken for both, so
-            // that the matrix is symmetric to the last bit
+    constexpr int per = TS / 8, ROUNDS = TS * per / kThreads, BATCH = ROUNDS < 4 ? ROUNDS : 4;
+    for (int at = 0; at < ROUNDS; at += BATCH) {
+        half8 hi[BATCH], lo[BATCH];
+        if (POLY)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const bool turn = i0 == j0 ? r > c + k : pass == 1;
-                f[k] = mul * (turn ? tile[(c + k) * Geo<TS>::PITCH + r] : tile[r * Geo<TS>::PITCH + c + k]);
+            for (int i = 0; i < BATCH; ++i) {      // (on their way before the first value is needed)
+                const int q = threadIdx.x + (at + i) * kThreads, row = row0 + q / per, col = col0 + q % per * 8;
+                const _Float16 *p = split_at(A, cols, row < rows ? row : rows - 1, col < cols ? col : cols - 8);
+                hi[i] = *reinterpret_cast<const half8 *>(p);
+                lo[i] = *reinterpret_cast<const half8 *>(p + 32);
             }
-            if (POLY) {
-                float g[4];
-                get_split(A, mp, row, col, g);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) f[k] += pb * g[k] + (row == col + k ? pa : 0.0f);
+        for (int i = 0; i < BATCH; ++i) {
+            const int q = threadIdx.x + (at + i) * kThreads, r = q / per, c = q % per * 8, row = row0 + r, col = col0 + c;
+            float f[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                f[k] = mul * tile[r * Geo<TS>::PITCH + c + k];
+                if (POLY) f[k] += pb * ((float)hi[i][k] + (float)lo[i][k]) + (row == col + k ? pa : 0.0f);
             }
-            put_split(out, mp, row, col, f);
+            if (row < rows && col < cols) put_split(out, cols, row, col, f);
         }
+    }
+}
+
+// ... of a symmetric matrix: the tile (i0, j0) and its mirror image.  A diagonal tile holds both triangles, the same products added
+// up in another order: the upper one is taken for both.  (The iteration relies on it: an asymmetry of one rounding grows with every step and
+// cost a factor of twelve in the result of a 40 x 300 matrix of rank one.)
+template <int TS, bool POLY>
+__device__ inline void put_symmetric(const Acc<TS> &acc, char *lds, char *out, int mp, int i0, int j0, float mul, char *A, float pa, float pb)
+{
+    put_tile<TS, POLY>(i0 == j0 ? to_tile_upper<TS>(acc, lds) : to_tile<TS, false>(acc, lds), out, mp, mp, i0, j0, mul, A, pa, pb);
+    if (i0 != j0) put_tile<TS, POLY>(to_tile<TS, true>(acc, lds), out, mp, mp, j0, i0, mul, A, pa, pb);
 }
 
 // tile number -> (i, j), j >= i, of a symmetric matrix of T x T tiles
@@ -488,16 +560,18 @@ __device__ inline void triangle(int t, int T, int &i, int &j)
 template <int TS> __global__ __launch_bounds__(kThreads, 2) void ortho_gram(Table t, char *ws, int seg)
 {
     __shared__ __attribute__((aligned(16))) char lds[Geo<TS>::LDS];
-    const Mat &M = t.mats[find(t, PH_GRAM)];
+    const int item = work_item();
+    const Mat &M = t.mats[find(t, PH_GRAM, item)];
     const int T = (M.mp + TS - 1) / TS, tiles = T * (T + 1) / 2;
-    const int wg = blockIdx.x - M.first[PH_GRAM], bi = wg / (tiles * M.splits), rest = wg % (tiles * M.splits), tile = rest / M.splits, piece = rest % M.splits;
+    // (the tiles of one piece of k next to each other: they read the same lines of X)
+    const int wg = item - M.first[PH_GRAM], bi = wg / (tiles * M.splits), rest = wg % (tiles * M.splits), tile = rest % tiles, piece = rest / tiles;
     int ti, tj;
     triangle(tile, T, ti, tj);
     char *area = ws + M.ws + bi * M.area;
     const char *X = area + buf_at(seg & 1 ? BUF_X1 : BUF_X0, M.mp, M.np);
     const int lines = M.np / 32, k0 = (int)((long)lines * piece / M.splits), k1 = (int)((long)lines * (piece + 1) / M.splits);
     Acc<TS> acc;
-    product<TS, false>(acc, lds, X, (long)M.np * 4, ti * TS, M.mp, X, (long)M.np * 4, tj * TS, M.mp, k0, k1);
+    product<TS, TS == 64 ? 4 : 2, false>(acc, lds, X, (long)M.np * 4, ti * TS, M.mp, X, (long)M.np * 4, tj * TS, M.mp, k0, k1);
     if (M.splits > 1) {
         float *part = reinterpret_cast<float *>(area + buf_at(BUF_PART, M.mp, M.np)) + ((long)tile * M.splits + piece) * TS * TS;
 #pragma unroll
@@ -509,16 +583,17 @@ template <int TS> __global__ __launch_bounds__(kThreads, 2) void ortho_gram(Tabl
         return;
     }
     const int e = reinterpret_cast<const int *>(area + kMaxParts * 8)[seg];
-    put_symmetric<TS, false>(to_tile<TS>(acc, lds), area + buf_at(BUF_A, M.mp, M.np), M.mp, ti * TS, tj * TS, ldexpf(1.0f, kExpA - 2 * e), nullptr, 0.0f, 0.0f);
+    put_symmetric<TS, false>(acc, lds, area + buf_at(BUF_A, M.mp, M.np), M.mp, ti * TS, tj * TS, ldexpf(1.0f, kExpA - 2 * e), nullptr, 0.0f, 0.0f);
 }
 
 template <int TS> __global__ __launch_bounds__(kThreads) void ortho_join(Table t, char *ws, int seg)
 {
     __shared__ __attribute__((aligned(16))) char lds[Geo<TS>::LDS];
-    const Mat &M = t.mats[find(t, PH_CHAIN)];
+    const int item = work_item();
+    const Mat &M = t.mats[find(t, PH_JOIN, item)];
     if (M.splits == 1) return;
     const int T = (M.mp + TS - 1) / TS, tiles = T * (T + 1) / 2;
-    const int wg = blockIdx.x - M.first[PH_CHAIN], bi = wg / tiles, tile = wg % tiles;
+    const int wg = item - M.first[PH_JOIN], bi = wg / tiles, tile = wg % tiles;
     int ti, tj;
     triangle(tile, T, ti, tj);
     char *area = ws + M.ws + bi * M.area;
@@ -538,32 +613,33 @@ template <int TS> __global__ __launch_bounds__(kThreads) void ortho_join(Table t
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc.v[i][j][e] += part[(long)s * TS * TS + ((i * Geo<TS>::FR + j) * 16 + e) * kThreads + threadIdx.x];
     const int e = reinterpret_cast<const int *>(area + kMaxParts * 8)[seg];
-    put_symmetric<TS, false>(to_tile<TS>(acc, lds), area + buf_at(BUF_A, M.mp, M.np), M.mp, ti * TS, tj * TS, ldexpf(1.0f, kExpA - 2 * e), nullptr, 0.0f, 0.0f);
+    put_symmetric<TS, false>(acc, lds, area + buf_at(BUF_A, M.mp, M.np), M.mp, ti * TS, tj * TS, ldexpf(1.0f, kExpA - 2 * e), nullptr, 0.0f, 0.0f);
 }
 
 // ---- phase 3: products of the m x m matrices ----------------------------------------------------------------------------------
 struct Chain {
-    int l[2], r[2], out[2];            // buffers of the (up to two, blockIdx.y) products of this launch
+    int l[2], r[2], out[2];            // buffers of the (up to two, gridDim.y) products of this launch
     float mul[2];
     int poly;                          // product 0 is A A, its result P
     float pa, pb;
 };
-template <int TS> __global__ __launch_bounds__(kThreads, 2) void ortho_chain(Table t, char *ws, Chain c)
+// DEEP: at most one workgroup a CU, which then has the registers for twice the lines in flight.
+template <int TS, bool DEEP> __global__ __launch_bounds__(kThreads, DEEP ? 1 : 2) void ortho_chain(Table t, char *ws, Chain c)
 {
     __shared__ __attribute__((aligned(16))) char lds[Geo<TS>::LDS];
-    const Mat &M = t.mats[find(t, PH_CHAIN)];
+    const int item = work_item(), w = item / (int)gridDim.x;
+    const Mat &M = t.mats[find(t, PH_CHAIN, item % (int)gridDim.x)];
     const int T = (M.mp + TS - 1) / TS, tiles = T * (T + 1) / 2;
-    const int wg = blockIdx.x - M.first[PH_CHAIN], bi = wg / tiles, w = blockIdx.y;
+    const int wg = item % (int)gridDim.x - M.first[PH_CHAIN], bi = wg / tiles;
     int ti, tj;
     triangle(wg % tiles, T, ti, tj);
     char *area = ws + M.ws + bi * M.area;
-    const char *L = area + buf_at(c.l[w], M.mp, M.np), *R = area + buf_at(c.r[w], M.mp, M.np);
+    char *L = area + buf_at(c.l[w], M.mp, M.np), *R = area + buf_at(c.r[w], M.mp, M.np);
     Acc<TS> acc;
-    product<TS, false>(acc, lds, L, (long)M.mp * 4, ti * TS, M.mp, R, (long)M.mp * 4, tj * TS, M.mp, 0, M.mp / 32);
-    const float *tile = to_tile<TS>(acc, lds);
+    product<TS, (TS == 64 ? 4 : 2) * (DEEP ? 2 : 1), false>(acc, lds, L, (long)M.mp * 4, ti * TS, M.mp, R, (long)M.mp * 4, tj * TS, M.mp, 0, M.mp / 32);
     char *out = area + buf_at(c.out[w], M.mp, M.np);
-    if (c.poly) put_symmetric<TS, true>(tile, out, M.mp, ti * TS, tj * TS, c.mul[w], L, c.pa, c.pb);
-    else put_symmetric<TS, false>(tile, out, M.mp, ti * TS, tj * TS, c.mul[w], nullptr, 0.0f, 0.0f);
+    if (c.poly) put_symmetric<TS, true>(acc, lds, out, M.mp, ti * TS, tj * TS, c.mul[w], L, c.pa, c.pb);
+    else put_symmetric<TS, false>(acc, lds, out, M.mp, ti * TS, tj * TS, c.mul[w], nullptr, 0.0f, 0.0f);
 }
 
 // ---- phase 4: X' = Q X, into the other X, the caller's matrix, or the parameters -------------------------------------------------
@@ -571,28 +647,18 @@ enum { TO_X = 0, TO_DST, TO_PARAM };
 template <int TS, typename T, int DEST> __global__ __launch_bounds__(kThreads, 2) void ortho_apply(Table t, char *ws, int seg, int q, int qexp, Step st)
 {
     __shared__ __attribute__((aligned(16))) char lds[Geo<TS>::LDS];
-    const Mat &M = t.mats[find(t, PH_APPLY)];
+    const int item = work_item();
+    const Mat &M = t.mats[find(t, PH_APPLY, item)];
     const int Ti = (M.mp + TS - 1) / TS, Tj = (M.np + TS - 1) / TS;
-    const int wg = blockIdx.x - M.first[PH_APPLY], bi = wg / (Ti * Tj), ti = wg % (Ti * Tj) % Ti, tj = wg % (Ti * Tj) / Ti;
+    const int wg = item - M.first[PH_APPLY], bi = wg / (Ti * Tj), ti = wg % (Ti * Tj) % Ti, tj = wg % (Ti * Tj) / Ti;
     char *area = ws + M.ws + bi * M.area;
     const char *X = area + buf_at(seg & 1 ? BUF_X1 : BUF_X0, M.mp, M.np);
     const int *ex = reinterpret_cast<const int *>(area + kMaxParts * 8);
     const int e0 = ex[seg], e1 = ex[seg + 1];
     Acc<TS> acc;
-    product<TS, true>(acc, lds, area + buf_at(q, M.mp, M.np), (long)M.mp * 4, ti * TS, M.mp, X, (long)M.np * 4, tj * TS, M.np / 32, 0, M.mp / 32);
-    const float *tile = to_tile<TS>(acc, lds);
-    constexpr int quads = TS / 4;
+    product<TS, TS == 64 ? 4 : 2, true>(acc, lds, area + buf_at(q, M.mp, M.np), (long)M.mp * 4, ti * TS, M.mp, X, (long)M.np * 4, tj * TS, M.np / 32, 0, M.mp / 32);
     if constexpr (DEST == TO_X) {
-        const float mul = ldexpf(1.0f, e1 - e0 - qexp);
-        char *out = area + buf_at(seg & 1 ? BUF_X0 : BUF_X1, M.mp, M.np);
-        for (int k = threadIdx.x; k < TS * quads; k += kThreads) {
-            const int r = k / quads, c = k % quads * 4;
-            if (ti * TS + r >= M.mp || tj * TS + c >= M.np) continue;
-            float f[4];
-#pragma unroll
-            for (int x = 0; x < 4; ++x) f[x] = mul * tile[r * Geo<TS>::PITCH + c + x];
-            put_split(out, M.np, ti * TS + r, tj * TS + c, f);
-        }
+        put_tile<TS, false>(to_tile<TS, false>(acc, lds), area + buf_at(seg & 1 ? BUF_X0 : BUF_X1, M.mp, M.np), M.mp, M.np, ti * TS, tj * TS, ldexpf(1.0f, e1 - e0 - qexp), nullptr, 0.0f, 0.0f);
         return;
     }
     // the result, in the caller's orientation: row r of the output tile, four neighbours of it
@@ -602,13 +668,15 @@ template <int TS, typename T, int DEST> __global__ __launch_bounds__(kThreads, 2
         keep = (float)(1.0 - st.hp[0] * st.hp[2]);
         step = (float)(st.hp[0] * (double)M.scale);
     }
+    constexpr int quads = TS / 4;
+    const float *tile = M.tall ? to_tile<TS, true>(acc, lds) : to_tile<TS, false>(acc, lds);
     const int R = M.tall ? M.n : M.m, C = M.tall ? M.m : M.n, r0 = (M.tall ? tj : ti) * TS, c0 = (M.tall ? ti : tj) * TS;
     for (int k = threadIdx.x; k < TS * quads; k += kThreads) {
         const int r = k / quads, c = k % quads * 4, row = r0 + r, col = c0 + c;
         if (row >= R || col >= C) continue;
         float f[4];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) f[x] = mul * (M.tall ? tile[(c + x) * Geo<TS>::PITCH + r] : tile[r * Geo<TS>::PITCH + c + x]);
+        for (int x = 0; x < 4; ++x) f[x] = mul * tile[r * Geo<TS>::PITCH + c + x];
         if constexpr (DEST == TO_PARAM) {
             float *p = st.p + (long)M.dst + (long)row * M.dst_ld + col;
             if (col + 4 <= C) {
@@ -691,7 +759,7 @@ struct Group {
     Mat m[kGroup];
     int n;
     long bytes;                        // workspace
-    int grid[5];
+    int grid[PHASES];
     int ts_gram, ts_chain, ts_apply;
     bool joined;
 };
@@ -712,7 +780,7 @@ void plan(Group &g)
         steps128 += (long)M.batch * T * (T + 1) / 2 * (M.np / 32);
     }
     g.ts_chain = chain128 >= 256 ? 128 : 64;
-    g.ts_gram = g.ts_chain;
+    g.ts_gram = steps128 >= 256 * 16 ? 128 : 64;
     g.ts_apply = apply128 >= 256 ? 128 : 64;
     long steps = 0;
     for (int k = 0; k < g.n; ++k) {
@@ -721,7 +789,7 @@ void plan(Group &g)
         steps += (long)M.batch * T * (T + 1) / 2 * (M.np / 32);
     }
     const long piece = steps / 512 > 8 ? steps / 512 : 8;
-    long at = 0, first[5] = {0, 0, 0, 0, 0};
+    long at = 0, first[PHASES] = {};
     g.joined = false;
     at = (long)((sizeof(Mat) * kGroup + 255) & ~255ul);
     for (int k = 0; k < g.n; ++k) {
@@ -738,13 +806,14 @@ void plan(Group &g)
         M.ws = at;
         at += M.area * M.batch;
         const long Ta = (M.mp + g.ts_apply - 1) / g.ts_apply, Tb = (M.np + g.ts_apply - 1) / g.ts_apply;
-        const long per[5] = {M.parts, (M.mp / 32) * ((M.np + 63l) / 64), tiles * M.splits, tiles, Ta * Tb};
-        for (int f = 0; f < 5; ++f) {
+        const long Tc = (M.mp + g.ts_chain - 1) / g.ts_chain;
+        const long per[PHASES] = {M.parts, (M.mp / 32) * ((M.np + 63l) / 64), tiles * M.splits, tiles, Tc * (Tc + 1) / 2, Ta * Tb};
+        for (int f = 0; f < PHASES; ++f) {
             M.first[f] = (int)first[f];
             first[f] += per[f] * M.batch;
         }
     }
-    for (int f = 0; f < 5; ++f) g.grid[f] = first[f] > 0x7fffffff ? -1 : (int)first[f];
+    for (int f = 0; f < PHASES; ++f) g.grid[f] = first[f] > 0x7fffffff ? -1 : (int)first[f];
     g.bytes = at;
 }
 
@@ -765,7 +834,7 @@ bool describe(Mat &M, long rows, long cols, long batch)
 template <typename T, bool STEP>
 int iterate(Group &g, const Poly &p, double eps, char *ws, const Step &st, hipStream_t stream)
 {
-    for (int f = 0; f < 5; ++f)
+    for (int f = 0; f < PHASES; ++f)
         if (g.grid[f] < 0) return tef::fail("orthogonalisation: too many tiles for one launch"), TEF_ERR_INVALID;
     Mat *table = reinterpret_cast<Mat *>(ws);
     const dim3 block(kThreads);
@@ -788,14 +857,21 @@ int iterate(Group &g, const Poly &p, double eps, char *ws, const Step &st, hipSt
         done += len;
         TS_LAUNCH(g.ts_gram, hipLaunchKernelGGL(ortho_gram<128>, gram, block, 0, stream, t, ws, s), hipLaunchKernelGGL(ortho_gram<64>, gram, block, 0, stream, t, ws, s));
         if (g.joined)
-            TS_LAUNCH(g.ts_gram, hipLaunchKernelGGL(ortho_join<128>, dim3((unsigned)g.grid[PH_CHAIN]), block, 0, stream, t, ws, s),
-                      hipLaunchKernelGGL(ortho_join<64>, dim3((unsigned)g.grid[PH_CHAIN]), block, 0, stream, t, ws, s));
+            TS_LAUNCH(g.ts_gram, hipLaunchKernelGGL(ortho_join<128>, dim3((unsigned)g.grid[PH_JOIN]), block, 0, stream, t, ws, s),
+                      hipLaunchKernelGGL(ortho_join<64>, dim3((unsigned)g.grid[PH_JOIN]), block, 0, stream, t, ws, s));
         int q = -1;
         for (int k = 0; k < len; ++k) {
             const int P = k & 1 ? BUF_P1 : BUF_P0;
             auto chain = [&](const Chain &c, int products) {
                 const dim3 grid((unsigned)g.grid[PH_CHAIN], (unsigned)products);
-                TS_LAUNCH(g.ts_chain, hipLaunchKernelGGL(ortho_chain<128>, grid, block, 0, stream, t, ws, c), hipLaunchKernelGGL(ortho_chain<64>, grid, block, 0, stream, t, ws, c));
+                const bool deep = (long)g.grid[PH_CHAIN] * products <= 256;
+                if (g.ts_chain == 128) {
+                    if (deep) hipLaunchKernelGGL((ortho_chain<128, true>), grid, block, 0, stream, t, ws, c);
+                    else hipLaunchKernelGGL((ortho_chain<128, false>), grid, block, 0, stream, t, ws, c);
+                } else {
+                    if (deep) hipLaunchKernelGGL((ortho_chain<64, true>), grid, block, 0, stream, t, ws, c);
+                    else hipLaunchKernelGGL((ortho_chain<64, false>), grid, block, 0, stream, t, ws, c);
+                }
             };
             // P = a I + b A + c A A
             Chain c{};
