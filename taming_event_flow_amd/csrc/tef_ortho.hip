@@ -288,8 +288,8 @@ template <typename T, bool STEP> __global__ __launch_bounds__(kThreads) void ort
 // ---- the products -----------------------------------------------------------------------------------------------------------
 // A workgroup of four waves computes TS x TS values (TS = 128 or 64), each wave a quarter of them in 32 x 32 blocks.  k advances
 // by one line of 32 a stage, from global memory through registers (AHEAD stages in flight) into LDS while the previous stage is
-// multiplied: two buffers, one barrier a stage.  The 16-byte chunks of a row are permuted by the row, chunk ^ (row & 7), so that the eight
-// lanes of an LDS cycle that read the same chunk of eight rows meet eight different bank groups.
+// multiplied: two buffers, one barrier a stage.  The 16-byte chunks of a row are permuted by the row, chunk ^ (row / 2 & 7):
+// sixteen lanes that read the same chunk of sixteen neighbouring rows (128 bytes each) meet all 64 banks once.
 template <int TS> struct Geo {
     static constexpr int FR = TS / 64;                       // 32 x 32 blocks of a wave along each side
     static constexpr int STAGE = TS * 128;                   // bytes of an operand's stage
@@ -314,14 +314,14 @@ template <int TS> __device__ inline void put_rows(char *lds, const uint4v (&r)[G
 #pragma unroll
     for (int i = 0; i < Geo<TS>::LOADS; ++i) {
         const int q = threadIdx.x + i * kThreads, row = q / per;
-        *reinterpret_cast<uint4v *>(lds + row * (per * 16) + (((q % per) ^ (row & 7)) << 4)) = r[i];
+        *reinterpret_cast<uint4v *>(lds + row * (per * 16) + (((q % per) ^ (row >> 1 & 7)) << 4)) = r[i];
     }
 }
 // rows `row` (this lane's), k = 16 * s + 8 * (lane >> 5) ..: plane 0 hi, 1 lo
 __device__ inline half8 frag_rows(const char *lds, int row, int s, int plane)
 {
     const int chunk = plane * 4 + s * 2 + ((threadIdx.x & 63) >> 5);
-    return *reinterpret_cast<const half8 *>(lds + row * 128 + ((chunk ^ (row & 7)) << 4));
+    return *reinterpret_cast<const half8 *>(lds + row * 128 + ((chunk ^ (row >> 1 & 7)) << 4));
 }
 // operand whose COLUMNS are the tile's (X in Q X): a stage is 32 rows of TS / 32 lines.  64-byte slots (one plane of one line)
 // are permuted by the row; ds_read_b64_tr_b16 hands every lane four consecutive k of its column.
