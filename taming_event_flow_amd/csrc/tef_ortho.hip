@@ -52,19 +52,23 @@ struct Mat {
     long src_ld, dst_ld, src_stride, dst_stride;
     long ws;                           // bytes from the workspace's start to this matrix's area
     long area;                         // ... of one batch element
+    long part;                         // bytes to the sums of products that are cut along k
     int m, n, mp, np;                  // short and long side, padded
     int tall;                          // src is [n][m]
     int batch;
     int parts;                         // partial sums of squares per batch element
-    int splits;                        // pieces of the Gram product's k
+    int splits;                        // pieces of the Gram product's k (lists of matrices)
     float scale;                       // of the applied update (optimiser)
-    int first[6];                       // first workgroup in the launch of each phase (below)
+    int first[6];                      // first work item in the launch of each phase (below)
 };
 enum { PH_SQ = 0, PH_PACK, PH_GRAM, PH_JOIN, PH_CHAIN, PH_APPLY, PHASES };
 
 // One batch element's area: doubles parts[kMaxParts], int exponents[kMaxSteps + 1], then the split matrices.
-__host__ __device__ inline long split_bytes(long rows, long cols) { return rows * cols * 4; }
-enum { BUF_X0 = 0, BUF_X1, BUF_A, BUF_W, BUF_P0, BUF_P1, BUF_Q0, BUF_Q1, BUF_PART };
+// Bytes from a row to the next: an odd number of lines, so that a column of lines (the rows of a tile) lies in all the memory channels
+// and not, as with 4096 columns, 16 KB apart in one of them.
+__host__ __device__ inline long pitch(int cols) { return ((cols / 32) | 1) * 128l; }
+__host__ __device__ inline long split_bytes(int rows, int cols) { return rows * pitch(cols); }
+enum { BUF_X0 = 0, BUF_X1, BUF_A, BUF_W, BUF_P0, BUF_P1, BUF_Q0, BUF_Q1, BUF_END };
 constexpr int kMaxSteps = 32;
 constexpr long kHead = kMaxParts * 8 + 256;      // (a multiple of 256, at least 4 * (kMaxSteps + 1) past the sums)
 __host__ __device__ inline long buf_at(int which, int mp, int np)
@@ -76,17 +80,20 @@ __host__ __device__ inline long buf_at(int which, int mp, int np)
 struct Table { const Mat *mats; int count; };
 
 // The work item of a workgroup: consecutive ones — tiles that read the same rows — go to ONE of the 8 XCDs (workgroups are dealt to
-// them in turn), so that a matrix is read into one L2 instead of all eight.
-__device__ inline int work_item()
+// them in turn), so that a matrix is read into one L2 instead of all eight.  The first `whole` items (a multiple of 8) are
+// dealt on their own: they take longer than the rest.
+__device__ inline int work_item(int whole = 0)
 {
-    const int total = gridDim.x * gridDim.y, lin = blockIdx.y * gridDim.x + blockIdx.x, xcd = lin & 7, each = total >> 3, more = total & 7;
-    return xcd * each + (xcd < more ? xcd : more) + (lin >> 3);
+    const int id = blockIdx.x, from = id < whole ? 0 : whole, total = id < whole ? whole : gridDim.x - whole;
+    const int lin = id - from, xcd = lin & 7, each = total >> 3, more = total & 7;
+    return from + xcd * each + (xcd < more ? xcd : more) + (lin >> 3);
 }
 // Which matrix an item of a phase belongs to: `first` is ascending, the wave looks at up to 64 of them at once.
-__device__ inline int find(const Table &t, int phase, int item)
+__device__ inline int find(const Table &t, int phase, int item, int products = 1)
 {
+    if (t.count == 1) return 0;
     const int lane = threadIdx.x & 63;
-    const int f = lane < t.count ? t.mats[lane].first[phase] : 0x7fffffff;
+    const int f = lane < t.count ? t.mats[lane].first[phase] * products : 0x7fffffff;
     return __popcll(__ballot(f <= item)) - 1;
 }
 
@@ -104,6 +111,26 @@ __device__ inline void split(float v, _Float16 &hi, _Float16 &lo)
 {
     hi = (_Float16)v;
     lo = (_Float16)(v - (float)hi);      // (infinite hi: NaN, as an overflow should show)
+}
+
+// eight neighbouring values of a split matrix's row
+__device__ inline _Float16 *split_at(char *base, int cols, long row, int col)
+{
+    return reinterpret_cast<_Float16 *>(base + row * pitch(cols) + (col >> 5) * 128) + (col & 31);
+}
+__device__ inline void put_split(char *base, int cols, long row, int col, const float (&f)[8])
+{
+    _Float16 *p = split_at(base, cols, row, col);
+    half8 hi, lo;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        _Float16 h, l;
+        split(f[k], h, l);
+        hi[k] = h;
+        lo[k] = l;
+    }
+    *reinterpret_cast<half8 *>(p) = hi;
+    *reinterpret_cast<half8 *>(p + 32) = lo;
 }
 
 __device__ inline double block_sum(double s, double *red)
@@ -272,17 +299,9 @@ template <typename T, bool STEP> __global__ __launch_bounds__(kThreads) void ort
         }
     }
     if (j0 + c >= M.np) return;
-    half8 hi, lo;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        _Float16 h, l;
-        split((float)((double)f[k] * mul), h, l);
-        hi[k] = h;
-        lo[k] = l;
-    }
-    _Float16 *x = reinterpret_cast<_Float16 *>(area + buf_at(BUF_X0, M.mp, M.np)) + ((long)(i0 + r) * M.np + j0 + (c & ~31)) * 2 + (c & 31);
-    *reinterpret_cast<half8 *>(x) = hi;
-    *reinterpret_cast<half8 *>(x + 32) = lo;
+    for (int k = 0; k < 8; ++k) f[k] = (float)((double)f[k] * mul);
+    put_split(area + buf_at(BUF_X0, M.mp, M.np), M.np, i0 + r, j0 + c, f);
 }
 
 // ---- the products -----------------------------------------------------------------------------------------------------------
@@ -488,26 +507,6 @@ template <int TS> __device__ inline float *to_tile_upper(const Acc<TS> &acc, cha
     return tile;
 }
 
-// eight neighbouring values of a split matrix's row
-__device__ inline _Float16 *split_at(char *base, long cols, long row, int col)
-{
-    return reinterpret_cast<_Float16 *>(base) + (row * cols + (col & ~31)) * 2 + (col & 31);
-}
-__device__ inline void put_split(char *base, long cols, long row, int col, const float (&f)[8])
-{
-    _Float16 *p = split_at(base, cols, row, col);
-    half8 hi, lo;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        _Float16 h, l;
-        split(f[k], h, l);
-        hi[k] = h;
-        lo[k] = l;
-    }
-    *reinterpret_cast<half8 *>(p) = hi;
-    *reinterpret_cast<half8 *>(p + 32) = lo;
-}
-
 // Writes rows row0 .. of the tile in LDS to the split matrix `out`, from column col0 on: mul * value + (POLY: the rest of
 // P = a I + b A + c A A).
 template <int TS, bool POLY>
@@ -548,56 +547,102 @@ __device__ inline void put_symmetric(const Acc<TS> &acc, char *lds, char *out, i
     if (i0 != j0) put_tile<TS, POLY>(to_tile<TS, true>(acc, lds), out, mp, mp, j0, i0, mul, A, pa, pb);
 }
 
-// tile number -> (i, j), j >= i, of a symmetric matrix of T x T tiles
+// tile number -> (i, j), j >= i, of a symmetric matrix of T x T tiles: eight columns at a time, so that 64 consecutive tiles, which run
+// side by side on one XCD, read 8 + 8 blocks of rows
 __device__ inline void triangle(int t, int T, int &i, int &j)
 {
-    i = 0;
-    while (t >= T - i) { t -= T - i; ++i; }
-    j = i + t;
+    int j0 = 0;
+    for (;;) {
+        const int w = T - j0 < 8 ? T - j0 : 8, n = w * j0 + w * (w + 1) / 2;
+        if (t < n) {
+            if (t < w * j0) { i = t / w; j = j0 + t % w; return; }
+            t -= w * j0;
+            i = 0;
+            while (t >= w - i) { t -= w - i; ++i; }
+            j = j0 + i + t;
+            i += j0;
+            return;
+        }
+        t -= n;
+        j0 += 8;
+    }
 }
 
-// ---- phase 2: A = X X^T, k in pieces when there are few tiles; the pieces' sums go to the workspace as the threads hold them ----
-template <int TS> __global__ __launch_bounds__(kThreads, 2) void ortho_gram(Table t, char *ws, int seg)
+// ---- phases 2 and 3: the symmetric products A = X X^T (k the long side) and those of the m x m matrices ------------------------------
+// A launch computes one or two of them (`products`, of every matrix).  Where their tiles do not fill the machine evenly some are
+// cut along k: `splits` pieces of every tile from number `whole` on (0 splits: the matrix's own number of pieces, all tiles); a
+// piece's fp32 sums go to the workspace as the threads hold them and ortho_join adds them up in order.
+struct Sym {
+    int l[2], r[2], out[2];            // buffers
+    float mul[2];
+    int products;
+    int poly;                          // product 0 is A A, its result P = a I + b A + c A A
+    float pa, pb;
+    int gram, seg;                     // product 0 is X X^T of this segment's X
+    int whole, splits;
+};
+struct Piece { int w, bi, ti, tj, slot, piece, pieces; };
+template <int TS> __device__ inline Piece piece_of(const Mat &M, const Sym &c, int local, bool join)
+{
+    const int T = (M.mp + TS - 1) / TS, tiles = T * (T + 1) / 2, total = tiles * M.batch * c.products;
+    Piece p;
+    const int cut = c.splits ? c.splits : M.splits;
+    int tile;
+    if (join) {
+        p.slot = local; tile = c.whole + local; p.piece = 0; p.pieces = cut;
+    } else if (local < c.whole) {
+        p.slot = 0; tile = local; p.piece = 0; p.pieces = 1;
+    } else {
+        const int n = total - c.whole;      // (the tiles of one piece of k next to each other: they read the same lines)
+        p.slot = (local - c.whole) % n; tile = c.whole + p.slot; p.piece = (local - c.whole) / n; p.pieces = cut;
+    }
+    p.w = tile / (tiles * M.batch);
+    tile %= tiles * M.batch;
+    p.bi = tile / tiles;
+    triangle(tile % tiles, T, p.ti, p.tj);
+    return p;
+}
+template <int TS> __device__ inline void finish(const Acc<TS> &acc, char *lds, const Mat &M, char *area, const Sym &c, const Piece &p)
+{
+    char *out = area + buf_at(c.out[p.w], M.mp, M.np);
+    if (c.poly) {
+        put_symmetric<TS, true>(acc, lds, out, M.mp, p.ti * TS, p.tj * TS, c.mul[p.w], area + buf_at(c.l[p.w], M.mp, M.np), c.pa, c.pb);
+    } else {
+        const float mul = c.gram ? ldexpf(1.0f, kExpA - 2 * reinterpret_cast<const int *>(area + kMaxParts * 8)[c.seg]) : c.mul[p.w];
+        put_symmetric<TS, false>(acc, lds, out, M.mp, p.ti * TS, p.tj * TS, mul, nullptr, 0.0f, 0.0f);
+    }
+}
+// DEEP: at most one workgroup a CU, which then has the registers for twice the lines in flight.
+template <int TS, bool DEEP> __global__ __launch_bounds__(kThreads, DEEP ? 1 : 2) void ortho_symmetric(Table t, char *ws, Sym c)
 {
     __shared__ __attribute__((aligned(16))) char lds[Geo<TS>::LDS];
-    const int item = work_item();
-    const Mat &M = t.mats[find(t, PH_GRAM, item)];
-    const int T = (M.mp + TS - 1) / TS, tiles = T * (T + 1) / 2;
-    // (the tiles of one piece of k next to each other: they read the same lines of X)
-    const int wg = item - M.first[PH_GRAM], bi = wg / (tiles * M.splits), rest = wg % (tiles * M.splits), tile = rest % tiles, piece = rest / tiles;
-    int ti, tj;
-    triangle(tile, T, ti, tj);
-    char *area = ws + M.ws + bi * M.area;
-    const char *X = area + buf_at(seg & 1 ? BUF_X1 : BUF_X0, M.mp, M.np);
-    const int lines = M.np / 32, k0 = (int)((long)lines * piece / M.splits), k1 = (int)((long)lines * (piece + 1) / M.splits);
+    const int item = work_item(c.splits > 1 ? c.whole : 0), phase = c.gram ? PH_GRAM : PH_CHAIN;
+    const Mat &M = t.mats[find(t, phase, item, c.products)];
+    const Piece p = piece_of<TS>(M, c, item - M.first[phase] * c.products, false);
+    char *area = ws + M.ws + p.bi * M.area;
+    const char *L = area + buf_at(c.l[p.w], M.mp, M.np), *R = area + buf_at(c.r[p.w], M.mp, M.np);
+    const int side = c.gram ? M.np : M.mp, lines = side / 32;
+    const int k0 = (int)((long)lines * p.piece / p.pieces), k1 = (int)((long)lines * (p.piece + 1) / p.pieces);
     Acc<TS> acc;
-    product<TS, TS == 64 ? 4 : 2, false>(acc, lds, X, (long)M.np * 4, ti * TS, M.mp, X, (long)M.np * 4, tj * TS, M.mp, k0, k1);
-    if (M.splits > 1) {
-        float *part = reinterpret_cast<float *>(area + buf_at(BUF_PART, M.mp, M.np)) + ((long)tile * M.splits + piece) * TS * TS;
+    product<TS, (TS == 64 ? 4 : 2) * (DEEP ? 2 : 1), false>(acc, lds, L, pitch(side), p.ti * TS, M.mp, R, pitch(side), p.tj * TS, M.mp, k0, k1);
+    if (p.pieces == 1) return finish<TS>(acc, lds, M, area, c, p);
+    float *part = reinterpret_cast<float *>(ws + M.part) + ((long)p.slot * p.pieces + p.piece) * TS * TS;
 #pragma unroll
-        for (int i = 0; i < Geo<TS>::FR; ++i)
+    for (int i = 0; i < Geo<TS>::FR; ++i)
 #pragma unroll
-            for (int j = 0; j < Geo<TS>::FR; ++j)
+        for (int j = 0; j < Geo<TS>::FR; ++j)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) part[((i * Geo<TS>::FR + j) * 16 + e) * kThreads + threadIdx.x] = acc.v[i][j][e];
-        return;
-    }
-    const int e = reinterpret_cast<const int *>(area + kMaxParts * 8)[seg];
-    put_symmetric<TS, false>(acc, lds, area + buf_at(BUF_A, M.mp, M.np), M.mp, ti * TS, tj * TS, ldexpf(1.0f, kExpA - 2 * e), nullptr, 0.0f, 0.0f);
+            for (int e = 0; e < 16; ++e) part[((i * Geo<TS>::FR + j) * 16 + e) * kThreads + threadIdx.x] = acc.v[i][j][e];
 }
 
-template <int TS> __global__ __launch_bounds__(kThreads) void ortho_join(Table t, char *ws, int seg)
+template <int TS> __global__ __launch_bounds__(kThreads) void ortho_join(Table t, char *ws, Sym c)
 {
     __shared__ __attribute__((aligned(16))) char lds[Geo<TS>::LDS];
     const int item = work_item();
     const Mat &M = t.mats[find(t, PH_JOIN, item)];
-    if (M.splits == 1) return;
-    const int T = (M.mp + TS - 1) / TS, tiles = T * (T + 1) / 2;
-    const int wg = item - M.first[PH_JOIN], bi = wg / tiles, tile = wg % tiles;
-    int ti, tj;
-    triangle(tile, T, ti, tj);
-    char *area = ws + M.ws + bi * M.area;
-    const float *part = reinterpret_cast<const float *>(area + buf_at(BUF_PART, M.mp, M.np)) + (long)tile * M.splits * TS * TS;
+    const Piece p = piece_of<TS>(M, c, item - (t.count == 1 ? 0 : M.first[PH_JOIN]), true);
+    if (p.pieces == 1) return;
+    const float *part = reinterpret_cast<const float *>(ws + M.part) + (long)p.slot * p.pieces * TS * TS;
     Acc<TS> acc;
 #pragma unroll
     for (int i = 0; i < Geo<TS>::FR; ++i)
@@ -605,41 +650,14 @@ template <int TS> __global__ __launch_bounds__(kThreads) void ortho_join(Table t
         for (int j = 0; j < Geo<TS>::FR; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc.v[i][j][e] = 0.0f;
-    for (int s = 0; s < M.splits; ++s)
+    for (int s = 0; s < p.pieces; ++s)
 #pragma unroll
         for (int i = 0; i < Geo<TS>::FR; ++i)
 #pragma unroll
             for (int j = 0; j < Geo<TS>::FR; ++j)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc.v[i][j][e] += part[(long)s * TS * TS + ((i * Geo<TS>::FR + j) * 16 + e) * kThreads + threadIdx.x];
-    const int e = reinterpret_cast<const int *>(area + kMaxParts * 8)[seg];
-    put_symmetric<TS, false>(acc, lds, area + buf_at(BUF_A, M.mp, M.np), M.mp, ti * TS, tj * TS, ldexpf(1.0f, kExpA - 2 * e), nullptr, 0.0f, 0.0f);
-}
-
-// ---- phase 3: products of the m x m matrices ----------------------------------------------------------------------------------
-struct Chain {
-    int l[2], r[2], out[2];            // buffers of the (up to two, gridDim.y) products of this launch
-    float mul[2];
-    int poly;                          // product 0 is A A, its result P
-    float pa, pb;
-};
-// DEEP: at most one workgroup a CU, which then has the registers for twice the lines in flight.
-template <int TS, bool DEEP> __global__ __launch_bounds__(kThreads, DEEP ? 1 : 2) void ortho_chain(Table t, char *ws, Chain c)
-{
-    __shared__ __attribute__((aligned(16))) char lds[Geo<TS>::LDS];
-    const int item = work_item(), w = item / (int)gridDim.x;
-    const Mat &M = t.mats[find(t, PH_CHAIN, item % (int)gridDim.x)];
-    const int T = (M.mp + TS - 1) / TS, tiles = T * (T + 1) / 2;
-    const int wg = item % (int)gridDim.x - M.first[PH_CHAIN], bi = wg / tiles;
-    int ti, tj;
-    triangle(wg % tiles, T, ti, tj);
-    char *area = ws + M.ws + bi * M.area;
-    char *L = area + buf_at(c.l[w], M.mp, M.np), *R = area + buf_at(c.r[w], M.mp, M.np);
-    Acc<TS> acc;
-    product<TS, (TS == 64 ? 4 : 2) * (DEEP ? 2 : 1), false>(acc, lds, L, (long)M.mp * 4, ti * TS, M.mp, R, (long)M.mp * 4, tj * TS, M.mp, 0, M.mp / 32);
-    char *out = area + buf_at(c.out[w], M.mp, M.np);
-    if (c.poly) put_symmetric<TS, true>(acc, lds, out, M.mp, ti * TS, tj * TS, c.mul[w], L, c.pa, c.pb);
-    else put_symmetric<TS, false>(acc, lds, out, M.mp, ti * TS, tj * TS, c.mul[w], nullptr, 0.0f, 0.0f);
+    finish<TS>(acc, lds, M, ws + M.ws + p.bi * M.area, c, p);
 }
 
 // ---- phase 4: X' = Q X, into the other X, the caller's matrix, or the parameters -------------------------------------------------
@@ -650,13 +668,14 @@ template <int TS, typename T, int DEST> __global__ __launch_bounds__(kThreads, 2
     const int item = work_item();
     const Mat &M = t.mats[find(t, PH_APPLY, item)];
     const int Ti = (M.mp + TS - 1) / TS, Tj = (M.np + TS - 1) / TS;
-    const int wg = item - M.first[PH_APPLY], bi = wg / (Ti * Tj), ti = wg % (Ti * Tj) % Ti, tj = wg % (Ti * Tj) / Ti;
+    const int wg = item - M.first[PH_APPLY], bi = wg / (Ti * Tj), r = wg % (Ti * Tj);
+    const int j8 = r / (8 * Ti) * 8, w8 = Tj - j8 < 8 ? Tj - j8 : 8, ti = (r - j8 * Ti) / w8, tj = j8 + (r - j8 * Ti) % w8;      // (as in triangle())
     char *area = ws + M.ws + bi * M.area;
     const char *X = area + buf_at(seg & 1 ? BUF_X1 : BUF_X0, M.mp, M.np);
     const int *ex = reinterpret_cast<const int *>(area + kMaxParts * 8);
     const int e0 = ex[seg], e1 = ex[seg + 1];
     Acc<TS> acc;
-    product<TS, TS == 64 ? 4 : 2, true>(acc, lds, area + buf_at(q, M.mp, M.np), (long)M.mp * 4, ti * TS, M.mp, X, (long)M.np * 4, tj * TS, M.np / 32, 0, M.mp / 32);
+    product<TS, TS == 64 ? 4 : 2, true>(acc, lds, area + buf_at(q, M.mp, M.np), pitch(M.mp), ti * TS, M.mp, X, pitch(M.np), tj * TS, M.np / 32, 0, M.mp / 32);
     if constexpr (DEST == TO_X) {
         put_tile<TS, false>(to_tile<TS, false>(acc, lds), area + buf_at(seg & 1 ? BUF_X0 : BUF_X1, M.mp, M.np), M.mp, M.np, ti * TS, tj * TS, ldexpf(1.0f, e1 - e0 - qexp), nullptr, 0.0f, 0.0f);
         return;
@@ -755,65 +774,115 @@ bool bounded(Poly &p)
     return tef::fail("orthogonalisation: these coefficients grow too fast");
 }
 
+struct Cut { int whole, splits; long items, joins; };
 struct Group {
     Mat m[kGroup];
     int n;
     long bytes;                        // workspace
     int grid[PHASES];
     int ts_gram, ts_chain, ts_apply;
-    bool joined;
+    Cut gram, chain[2];                // one, two products
 };
 
 inline int round32(long v) { return (int)((v + 31) & ~31l); }
 
+inline long triangle_tiles(int mp, int ts)
+{
+    const long T = (mp + ts - 1) / ts;
+    return T * (T + 1) / 2;
+}
+
+// How the tiles of ONE matrix's product are dealt to 256 CUs: as many as are a multiple of 256 whole, the rest cut along k so that the
+// pieces, too, are about 256 (512 when there is nothing else to run beside them), of at least 8 lines: a piece's sums have to be
+// written and read again, and joining takes a launch of its own (about 10 us), so products of fewer than 32 lines are left alone.
+// 4096 x 4096: 528 tiles take 280 us whole — two on every CU, then the last 16 — and 180 us with those 16 in pieces.
+Cut cut_one(long tiles, long lines)
+{
+    Cut c{(int)tiles, 1, tiles, 0};
+    const long rest = tiles % 256;
+    if (lines < 32 || tiles > (1l << 24) || !rest) return c;
+    long s = tiles < 256 ? 512 / tiles : 256 / rest;
+    if (s > lines / 8) s = lines / 8;
+    if (s < 2) return c;
+    if (s > 64) s = 64;
+    c.whole = (int)(tiles - rest);
+    c.splits = (int)s;
+    c.items = c.whole + rest * s;
+    c.joins = rest;
+    return c;
+}
+
 // Tile sizes: 128 where the launch then still covers the 256 CUs, else 64 (a quarter of the work each, so that four times as many
-// workgroups share it).  The Gram product is cut along k until there are about two workgroups a CU, in pieces of at least
-// eight lines, since a piece's fp32 sums have to be written and read again.
+// workgroups share it).
 void plan(Group &g)
 {
     long chain128 = 0, apply128 = 0, steps128 = 0;
     for (int k = 0; k < g.n; ++k) {
         const Mat &M = g.m[k];
         const long T = (M.mp + 127) / 128;
-        chain128 += (long)M.batch * T * (T + 1) / 2;
+        chain128 += (long)M.batch * triangle_tiles(M.mp, 128);
         apply128 += (long)M.batch * T * ((M.np + 127) / 128);
-        steps128 += (long)M.batch * T * (T + 1) / 2 * (M.np / 32);
+        steps128 += (long)M.batch * triangle_tiles(M.mp, 128) * (M.np / 32);
     }
-    g.ts_chain = chain128 >= 256 ? 128 : 64;
+    g.ts_chain = chain128 >= 256 || (g.n == 1 && chain128 >= 64 && g.m[0].mp >= 1024) ? 128 : 64;
     g.ts_gram = steps128 >= 256 * 16 ? 128 : 64;
     g.ts_apply = apply128 >= 256 ? 128 : 64;
-    long steps = 0;
-    for (int k = 0; k < g.n; ++k) {
-        const Mat &M = g.m[k];
-        const long T = (M.mp + g.ts_gram - 1) / g.ts_gram;
-        steps += (long)M.batch * T * (T + 1) / 2 * (M.np / 32);
-    }
-    const long piece = steps / 512 > 8 ? steps / 512 : 8;
-    long at = 0, first[PHASES] = {};
-    g.joined = false;
-    at = (long)((sizeof(Mat) * kGroup + 255) & ~255ul);
+    // a list: every tile of the Gram products in pieces of one length, the shortest that gives no more pieces than run at once
+    long piece = 8, slots = g.ts_gram == 128 ? 512 : 1024;
+    if (g.n > 1)
+        for (;; piece += piece / 8) {
+            long items = 0, longest = 0;
+            for (int k = 0; k < g.n; ++k) {
+                const long lines = g.m[k].np / 32;
+                items += (long)g.m[k].batch * triangle_tiles(g.m[k].mp, g.ts_gram) * ((lines + piece - 1) / piece);
+                longest = longest > lines ? longest : lines;
+            }
+            if (items <= slots || piece >= longest) break;
+        }
+    long first[PHASES] = {};
+    long at = (long)((sizeof(Mat) * kGroup + 255) & ~255ul);
+    g.gram = Cut{0, 0, 0, 0};
     for (int k = 0; k < g.n; ++k) {
         Mat &M = g.m[k];
-        const long T = (M.mp + g.ts_gram - 1) / g.ts_gram, tiles = T * (T + 1) / 2, lines = M.np / 32;
-        long splits = (lines + piece - 1) / piece;
-        M.splits = (int)(splits < 1 ? 1 : splits > 64 ? 64 : splits);
-        if (M.splits > 1) g.joined = true;
+        const long tiles = triangle_tiles(M.mp, g.ts_gram), lines = M.np / 32;
+        long splits = (lines + piece - 1) / piece, parts = 0;
+        if (g.n == 1) {
+            g.gram = cut_one(tiles * M.batch, lines);
+            parts = g.gram.joins * g.gram.splits * g.ts_gram * g.ts_gram;
+            splits = 1;
+            for (int w = 0; w < 2; ++w) {
+                g.chain[w] = cut_one(triangle_tiles(M.mp, g.ts_chain) * M.batch * (w + 1), M.mp / 32);
+                const long p = g.chain[w].joins * g.chain[w].splits * g.ts_chain * g.ts_chain;
+                parts = parts > p ? parts : p;
+            }
+        } else {
+            splits = splits > 64 ? 64 : splits;
+            if (splits > 1) {
+                parts = tiles * M.batch * splits * g.ts_gram * g.ts_gram;
+                g.gram.joins = 1;
+            }
+        }
+        M.splits = (int)splits;
         const long total = (long)M.m * M.n;
-        long parts = (total + 16383) / 16384;
-        M.parts = (int)(parts < 1 ? 1 : parts > kMaxParts ? kMaxParts : parts);
-        M.area = buf_at(BUF_PART, M.mp, M.np) + (M.splits > 1 ? tiles * M.splits * g.ts_gram * g.ts_gram * 4 : 0);
-        M.area = (M.area + 255) & ~255l;
+        long sums = (total + 16383) / 16384;
+        M.parts = (int)(sums < 1 ? 1 : sums > kMaxParts ? kMaxParts : sums);
+        M.area = (buf_at(BUF_END, M.mp, M.np) + 255) & ~255l;
         M.ws = at;
-        at += M.area * M.batch;
+        M.part = at + M.area * M.batch;
+        at = M.part + ((parts * 4 + 255) & ~255l);
         const long Ta = (M.mp + g.ts_apply - 1) / g.ts_apply, Tb = (M.np + g.ts_apply - 1) / g.ts_apply;
-        const long Tc = (M.mp + g.ts_chain - 1) / g.ts_chain;
-        const long per[PHASES] = {M.parts, (M.mp / 32) * ((M.np + 63l) / 64), tiles * M.splits, tiles, Tc * (Tc + 1) / 2, Ta * Tb};
+        const long per[PHASES] = {M.parts, (M.mp / 32) * ((M.np + 63l) / 64), tiles * splits, tiles, triangle_tiles(M.mp, g.ts_chain), Ta * Tb};
         for (int f = 0; f < PHASES; ++f) {
             M.first[f] = (int)first[f];
             first[f] += per[f] * M.batch;
         }
     }
-    for (int f = 0; f < PHASES; ++f) g.grid[f] = first[f] > 0x7fffffff ? -1 : (int)first[f];
+    if (g.n > 1) {
+        g.gram.items = first[PH_GRAM];
+        if (g.gram.joins) g.gram.joins = first[PH_JOIN];
+        for (int w = 0; w < 2; ++w) g.chain[w] = Cut{0, 1, first[PH_CHAIN] * (w + 1), 0};
+    }
+    for (int f = 0; f < PHASES; ++f) g.grid[f] = first[f] > 0x3fffffff ? -1 : (int)first[f];
     g.bytes = at;
 }
 
@@ -848,38 +917,44 @@ int iterate(Group &g, const Poly &p, double eps, char *ws, const Step &st, hipSt
     }
     const Table t{table, g.n};
     hipLaunchKernelGGL((ortho_pack<T, STEP>), dim3((unsigned)g.grid[PH_PACK]), block, 0, stream, t, ws, eps, st);
-    const dim3 gram((unsigned)g.grid[PH_GRAM]), apply((unsigned)g.grid[PH_APPLY]);
+    const dim3 apply((unsigned)g.grid[PH_APPLY]);
+    auto symmetric = [&](Sym c, int products, int ts, const Cut &cut) {
+        c.products = products;
+        c.whole = cut.whole;
+        c.splits = cut.splits;
+        const dim3 grid((unsigned)cut.items);
+        const bool deep = cut.items <= 256;
+        if (ts == 128) {
+            if (deep) hipLaunchKernelGGL((ortho_symmetric<128, true>), grid, block, 0, stream, t, ws, c);
+            else hipLaunchKernelGGL((ortho_symmetric<128, false>), grid, block, 0, stream, t, ws, c);
+        } else {
+            if (deep) hipLaunchKernelGGL((ortho_symmetric<64, true>), grid, block, 0, stream, t, ws, c);
+            else hipLaunchKernelGGL((ortho_symmetric<64, false>), grid, block, 0, stream, t, ws, c);
+        }
+        if (cut.joins)
+            TS_LAUNCH(ts, hipLaunchKernelGGL(ortho_join<128>, dim3((unsigned)cut.joins), block, 0, stream, t, ws, c),
+                      hipLaunchKernelGGL(ortho_join<64>, dim3((unsigned)cut.joins), block, 0, stream, t, ws, c));
+    };
     // steps in segments of nearly equal length (5: 3 + 2)
     const int segs = (p.steps + p.seg_len - 1) / p.seg_len;
     int done = 0;
     for (int s = 0; s < segs; ++s) {
         const int len = (p.steps - done + segs - s - 1) / (segs - s);
         done += len;
-        TS_LAUNCH(g.ts_gram, hipLaunchKernelGGL(ortho_gram<128>, gram, block, 0, stream, t, ws, s), hipLaunchKernelGGL(ortho_gram<64>, gram, block, 0, stream, t, ws, s));
-        if (g.joined)
-            TS_LAUNCH(g.ts_gram, hipLaunchKernelGGL(ortho_join<128>, dim3((unsigned)g.grid[PH_JOIN]), block, 0, stream, t, ws, s),
-                      hipLaunchKernelGGL(ortho_join<64>, dim3((unsigned)g.grid[PH_JOIN]), block, 0, stream, t, ws, s));
+        Sym x{};
+        x.gram = 1; x.seg = s;
+        x.l[0] = x.r[0] = s & 1 ? BUF_X1 : BUF_X0; x.out[0] = BUF_A;
+        symmetric(x, 1, g.ts_gram, g.gram);
         int q = -1;
         for (int k = 0; k < len; ++k) {
             const int P = k & 1 ? BUF_P1 : BUF_P0;
-            auto chain = [&](const Chain &c, int products) {
-                const dim3 grid((unsigned)g.grid[PH_CHAIN], (unsigned)products);
-                const bool deep = (long)g.grid[PH_CHAIN] * products <= 256;
-                if (g.ts_chain == 128) {
-                    if (deep) hipLaunchKernelGGL((ortho_chain<128, true>), grid, block, 0, stream, t, ws, c);
-                    else hipLaunchKernelGGL((ortho_chain<128, false>), grid, block, 0, stream, t, ws, c);
-                } else {
-                    if (deep) hipLaunchKernelGGL((ortho_chain<64, true>), grid, block, 0, stream, t, ws, c);
-                    else hipLaunchKernelGGL((ortho_chain<64, false>), grid, block, 0, stream, t, ws, c);
-                }
-            };
             // P = a I + b A + c A A
-            Chain c{};
+            Sym c{};
             c.l[0] = c.r[0] = BUF_A; c.out[0] = P; c.poly = 1;
             c.mul[0] = ldexpf(p.c, kExpP - 2 * kExpA); c.pa = ldexpf(p.a, kExpP); c.pb = ldexpf(p.b, kExpP - kExpA);
-            chain(c, 1);
+            symmetric(c, 1, g.ts_chain, g.chain[0]);
             // W = A P and Q' = Q P, then A' = W P
-            Chain d{};
+            Sym d{};
             int products = 0;
             if (k + 1 < len) {
                 d.l[products] = BUF_A; d.r[products] = P; d.out[products] = BUF_W; d.mul[products] = ldexpf(1.0f, kExpA - kExpA - kExpP);
@@ -894,11 +969,11 @@ int iterate(Group &g, const Poly &p, double eps, char *ws, const Step &st, hipSt
             } else {
                 q = P;
             }
-            if (products) chain(d, products);
+            if (products) symmetric(d, products, g.ts_chain, g.chain[products - 1]);
             if (k + 1 < len) {
-                Chain e{};
+                Sym e{};
                 e.l[0] = BUF_W; e.r[0] = P; e.out[0] = BUF_A; e.mul[0] = ldexpf(1.0f, kExpA - kExpA - kExpP);
-                chain(e, 1);
+                symmetric(e, 1, g.ts_chain, g.chain[0]);
             }
         }
         const bool last = s + 1 == segs;
