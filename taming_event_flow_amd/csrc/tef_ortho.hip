@@ -650,14 +650,103 @@ template <int TS> __global__ __launch_bounds__(kThreads) void ortho_join(Table t
         for (int j = 0; j < Geo<TS>::FR; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc.v[i][j][e] = 0.0f;
-    for (int s = 0; s < p.pieces; ++s)
+    for (int s = 0; s < p.pieces; s += 2) {      // two pieces' sums in flight
+        constexpr int N = Geo<TS>::FR * Geo<TS>::FR * 16;
+        const float *q = part + (long)s * TS * TS + threadIdx.x;
+        const bool two = s + 1 < p.pieces;
+        float f[2][N];
 #pragma unroll
-        for (int i = 0; i < Geo<TS>::FR; ++i)
+        for (int k = 0; k < N; ++k) {
+            f[0][k] = q[k * kThreads];
+            f[1][k] = q[(two ? TS * TS : 0) + k * kThreads];
+        }
 #pragma unroll
-            for (int j = 0; j < Geo<TS>::FR; ++j)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) acc.v[i][j][e] += part[(long)s * TS * TS + ((i * Geo<TS>::FR + j) * 16 + e) * kThreads + threadIdx.x];
+        for (int k = 0; k < N; ++k) {
+            auto &v = acc.v[k / 16 / Geo<TS>::FR][k / 16 % Geo<TS>::FR];
+            v[k % 16] += f[0][k];
+            v[k % 16] += two ? f[1][k] : 0.0f;
+        }
+    }
     finish<TS>(acc, lds, M, ws + M.ws + p.bi * M.area, c, p);
+}
+
+// The same for m x m products of few and short tiles, where a launch is latency: 32 x 32 tiles, k dealt line by line to the four waves,
+// fragments straight from memory (no LDS, no barrier; four lines of a wave in flight), the waves' sums joined in order in LDS.
+__global__ __launch_bounds__(kThreads) void ortho_symmetric32(Table t, char *ws, Sym c)
+{
+    constexpr int TS = 32, PITCH = 36, BATCH = 4;
+    typedef float float4v __attribute__((ext_vector_type(4)));
+    __shared__ __attribute__((aligned(16))) float sums[4][TS * PITCH];
+    __shared__ float done[TS * (TS + 1)];
+    const int item = work_item();
+    const Mat &M = t.mats[find(t, PH_CHAIN, item, c.products)];
+    const int T = M.mp / TS, tiles = T * (T + 1) / 2;
+    int tile = item - M.first[PH_CHAIN] * c.products, ti, tj;
+    const int w = tile / (tiles * M.batch), bi = tile % (tiles * M.batch) / tiles;
+    triangle(tile % tiles, T, ti, tj);
+    char *area = ws + M.ws + bi * M.area;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lines = M.mp / 32;
+    const long ld = pitch(M.mp), at = (lane >> 5) * 16;
+    const char *L = area + buf_at(c.l[w], M.mp, M.np) + (ti * TS + (lane & 31)) * ld + at, *R = area + buf_at(c.r[w], M.mp, M.np) + (tj * TS + (lane & 31)) * ld + at;
+    const int r = threadIdx.x >> 3, q = (threadIdx.x & 7) * 4, row = ti * TS + r, col = tj * TS + q;
+    half4 ahi, alo;
+    if (c.poly) {
+        const _Float16 *p = split_at(area + buf_at(c.l[w], M.mp, M.np), M.mp, row, col);
+        ahi = *reinterpret_cast<const half4 *>(p);
+        alo = *reinterpret_cast<const half4 *>(p + 32);
+    }
+    float16v acc;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e] = 0.0f;
+    for (int l0 = wave; l0 < lines; l0 += 4 * BATCH) {
+        half8 a[BATCH][2][2], b[BATCH][2][2];
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+            const int l = l0 + 4 * k < lines ? l0 + 4 * k : lines - 1;
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int pl = 0; pl < 2; ++pl) {
+                    a[k][s][pl] = *reinterpret_cast<const half8 *>(L + l * 128l + pl * 64 + s * 32);
+                    b[k][s][pl] = *reinterpret_cast<const half8 *>(R + l * 128l + pl * 64 + s * 32);
+                }
+        }
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k)
+            if (l0 + 4 * k < lines)
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int x = 0; x < 3; ++x) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[k][s][x == 0], b[k][s][x == 1], acc, 0, 0, 0);
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sums[wave][(8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * PITCH + (lane & 31)] = acc[e];
+    __syncthreads();
+    float4v f = *reinterpret_cast<const float4v *>(&sums[0][r * PITCH + q]);
+#pragma unroll
+    for (int k = 1; k < 4; ++k) f += *reinterpret_cast<const float4v *>(&sums[k][r * PITCH + q]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        f[k] *= c.mul[w];
+        if (c.poly) f[k] += c.pb * ((float)ahi[k] + (float)alo[k]) + (row == col + k ? c.pa : 0.0f);
+        done[r * (TS + 1) + q + k] = f[k];
+    }
+    __syncthreads();
+    char *out = area + buf_at(c.out[w], M.mp, M.np);
+    for (int mirror = 0; mirror < (ti == tj ? 1 : 2); ++mirror) {
+        half4 hi, lo;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {      // (the diagonal tile: its upper triangle for both, see put_symmetric)
+            const bool turn = mirror || (ti == tj && r > q + k);
+            _Float16 h, lw;
+            split(turn ? done[(q + k) * (TS + 1) + r] : f[k], h, lw);
+            hi[k] = h;
+            lo[k] = lw;
+        }
+        _Float16 *p = split_at(out, M.mp, mirror ? tj * TS + r : row, mirror ? ti * TS + q : col);
+        *reinterpret_cast<half4 *>(p) = hi;
+        *reinterpret_cast<half4 *>(p + 32) = lo;
+    }
 }
 
 // ---- phase 4: X' = Q X, into the other X, the caller's matrix, or the parameters -------------------------------------------------
@@ -666,7 +755,7 @@ template <int TS, typename T, int DEST> __global__ __launch_bounds__(kThreads, 2
 {
     __shared__ __attribute__((aligned(16))) char lds[Geo<TS>::LDS];
     const int item = work_item();
-    const Mat &M = t.mats[find(t, PH_APPLY, item)];
+    const Mat M = t.mats[find(t, PH_APPLY, item)];      // (a copy: the stores below could be to the table, as far as the compiler knows)
     const int Ti = (M.mp + TS - 1) / TS, Tj = (M.np + TS - 1) / TS;
     const int wg = item - M.first[PH_APPLY], bi = wg / (Ti * Tj), r = wg % (Ti * Tj);
     const int j8 = r / (8 * Ti) * 8, w8 = Tj - j8 < 8 ? Tj - j8 : 8, ti = (r - j8 * Ti) / w8, tj = j8 + (r - j8 * Ti) % w8;      // (as in triangle())
@@ -719,6 +808,182 @@ template <int TS, typename T, int DEST> __global__ __launch_bounds__(kThreads, 2
         }
     }
 }
+
+// ---- small matrices: the whole iteration in one workgroup --------------------------------------------------------------------------
+// m <= 64 and at most 32 LINES columns: X, A, P and Q stay in LDS as split matrices (line l: 64 rows of 128 bytes, permuted as the
+// stages above) and one launch does what the general path spreads over twenty, each a few microseconds of latency whatever the
+// size.  A product's values are in registers when its operands have been read, so it overwrites one of them: W = A P goes to A's
+// place, Q P to Q's, A' = W P to W's.
+__device__ inline char *line_at(char *m, int line) { return m + line * (64 * 128); }
+// acc = L R^T over `lines` lines (this wave's 32 x 32 block)
+__device__ inline void small_rows(Acc<64> &acc, const char *L, const char *R, int lines)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = (wave >> 1) * 32, wj = (wave & 1) * 32;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc.v[0][0][e] = 0.0f;
+    for (int l = 0; l < lines; ++l)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            half8 a[2], b[2];
+#pragma unroll
+            for (int pl = 0; pl < 2; ++pl) {
+                a[pl] = frag_rows(L + l * 8192, wi + (lane & 31), s, pl);
+                b[pl] = frag_rows(R + l * 8192, wj + (lane & 31), s, pl);
+            }
+#pragma unroll
+            for (int t = 0; t < 3; ++t) acc.v[0][0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[t == 0], b[t == 1], acc.v[0][0], 0, 0, 0);
+        }
+}
+// acc = Q X over `lines` lines of Q, for the two lines of X from `X` on (64 columns; X's rows are k)
+__device__ inline void small_cols(Acc<64> &acc, const char *Q, const char *X, int lines)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = (wave >> 1) * 32, g = lane >> 4, src = lane & 15;
+    const char *x = X + (wave & 1) * 8192;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc.v[0][0][e] = 0.0f;
+    for (int l = 0; l < lines; ++l)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            half8 a[2], b[2];
+#pragma unroll
+            for (int pl = 0; pl < 2; ++pl) {
+                a[pl] = frag_rows(Q + l * 8192, wi + (lane & 31), s, pl);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {      // four k of this lane's column: see frag_cols
+                    const int row = l * 32 + s * 16 + (g >> 1) * 8 + h * 4 + (src >> 2), col = (g & 1) * 16 + (src & 3) * 4;
+                    const char *p = x + row * 128 + (((pl * 4 + (col >> 3)) ^ (row >> 1 & 7)) << 4) + (col & 4) * 2;
+                    const half4 f = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v *)p));
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) b[pl][h * 4 + k] = f[k];
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 3; ++t) acc.v[0][0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[t == 0], b[t == 1], acc.v[0][0], 0, 0, 0);
+        }
+}
+__device__ inline char *small_at(char *m, int row, int col, int plane)      // 16 bytes: eight columns from `col` on
+{
+    return line_at(m, col >> 5) + row * 128 + (((plane * 4 + ((col & 31) >> 3)) ^ (row >> 1 & 7)) << 4);
+}
+// 64 x 64 values of the tile to the split matrix `out` (two lines); POLY as in put_tile, A and out may not be the same
+template <bool POLY> __device__ inline void small_put(const float *tile, char *out, float mul, char *A, float pa, float pb)
+{
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int q = threadIdx.x + i * kThreads, r = q >> 3, c = (q & 7) * 8;
+        half8 hi, lo;
+        if (POLY) {
+            hi = *reinterpret_cast<const half8 *>(small_at(A, r, c, 0));
+            lo = *reinterpret_cast<const half8 *>(small_at(A, r, c, 1));
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            float f = mul * tile[r * Geo<64>::PITCH + c + k];
+            if (POLY) f += pb * ((float)hi[k] + (float)lo[k]) + (r == c + k ? pa : 0.0f);
+            _Float16 h, l;
+            split(f, h, l);
+            hi[k] = h;
+            lo[k] = l;
+        }
+        *reinterpret_cast<half8 *>(small_at(out, r, c, 0)) = hi;
+        *reinterpret_cast<half8 *>(small_at(out, r, c, 1)) = lo;
+    }
+    __syncthreads();
+}
+
+struct Small { Mat m[kChunk]; int first[kChunk]; int n; };
+struct SmallPoly { float a, b, c; int steps, seg_len; double eps; };
+template <typename T, int LINES> __global__ __launch_bounds__(kThreads) void ortho_small(Small list, SmallPoly p)
+{
+    __shared__ __attribute__((aligned(16))) char mats[3 * 16384];
+    __shared__ __attribute__((aligned(16))) char X[LINES * 8192];
+    __shared__ __attribute__((aligned(16))) char scratch[64 * Geo<64>::PITCH * 4];
+    __shared__ double red[4];
+    int k = 0;
+    while (k + 1 < list.n && list.first[k + 1] <= (int)blockIdx.x) ++k;
+    const Mat &M = list.m[k];
+    const int bi = blockIdx.x - list.first[k], cols = M.tall ? M.m : M.n, m = M.m, n = M.n, klines = m > 32 ? 2 : 1;
+    const T *src = reinterpret_cast<const T *>(M.src) + bi * M.src_stride;
+    double s = 0.0;
+    for (int i = threadIdx.x; i < m * n; i += kThreads) {
+        const float v = to_f<T>(src[(long)(i / cols) * M.src_ld + i % cols]);
+        s += (double)v * v;
+    }
+    s = sqrt(block_sum(s, red));
+    const double div = s < p.eps ? p.eps : s, rho = s / div;
+    int up = 0;
+    if (rho < 1.0 && rho > 0.0) {
+        up = -ilogb(rho);
+        up = up > 100 ? 100 : up;
+    }
+    const double mul = ldexp(1.0 / div, kExpX + up);
+    const int xlines = 2 * ((n + 63) / 64);      // (whole 64-column tiles; LINES is even)
+    for (int q = threadIdx.x; q < xlines * 256; q += kThreads) {      // eight columns of a row; a wave along the source's rows
+        const int per = xlines * 4, r = M.tall ? q & 63 : q / per, c = (M.tall ? q >> 6 : q % per) * 8;
+        half8 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const bool in = r < m && c + e < n;
+            const long off = M.tall ? (long)(c + e) * M.src_ld + r : (long)r * M.src_ld + c + e;
+            const float v = in ? (float)((double)to_f<T>(src[in ? off : 0]) * mul) : 0.0f;
+            _Float16 h, l;
+            split(v, h, l);
+            hi[e] = h;
+            lo[e] = l;
+        }
+        *reinterpret_cast<half8 *>(small_at(X, r, c, 0)) = hi;
+        *reinterpret_cast<half8 *>(small_at(X, r, c, 1)) = lo;
+    }
+    __syncthreads();
+    Acc<64> acc;
+    int done = 0;
+    const int segs = (p.steps + p.seg_len - 1) / p.seg_len;
+    for (int seg = 0; seg < segs; ++seg) {
+        const int len = (p.steps - done + segs - seg - 1) / (segs - seg);
+        done += len;
+        char *A = mats, *P = mats + 16384, *Q = mats + 32768;
+        small_rows(acc, X, X, xlines);
+        small_put<false>(to_tile_upper<64>(acc, scratch), A, ldexpf(1.0f, kExpA - 2 * (kExpX + up)), nullptr, 0.0f, 0.0f);
+        int qexp = kExpP;
+        for (int j = 0; j < len; ++j) {
+            small_rows(acc, A, A, klines);
+            small_put<true>(to_tile_upper<64>(acc, scratch), P, ldexpf(p.c, kExpP - 2 * kExpA), A, ldexpf(p.a, kExpP), ldexpf(p.b, kExpP - kExpA));
+            if (j + 1 < len) {
+                small_rows(acc, A, P, klines);
+                small_put<false>(to_tile_upper<64>(acc, scratch), A, ldexpf(1.0f, -kExpP), nullptr, 0.0f, 0.0f);
+                small_rows(acc, A, P, klines);
+                small_put<false>(to_tile_upper<64>(acc, scratch), A, ldexpf(1.0f, -kExpP), nullptr, 0.0f, 0.0f);
+            }
+            if (j == 0) {      // Q is P; the next P takes the other place
+                char *other = Q;
+                Q = P;
+                P = other;
+            } else {
+                small_rows(acc, Q, P, klines);
+                small_put<false>(to_tile_upper<64>(acc, scratch), Q, ldexpf(1.0f, kExpQ - qexp - kExpP), nullptr, 0.0f, 0.0f);
+                qexp = kExpQ;
+            }
+        }
+        const int e0 = kExpX + up;
+        up = up > 6 ? up - 6 : 0;
+        for (int x = 0; x < xlines; x += 2) {
+            small_cols(acc, Q, line_at(X, x), klines);
+            if (seg + 1 < segs) {
+                small_put<false>(to_tile<64, false>(acc, scratch), line_at(X, x), ldexpf(1.0f, kExpX + up - e0 - qexp), nullptr, 0.0f, 0.0f);
+                continue;
+            }
+            const float *tile = M.tall ? to_tile<64, true>(acc, scratch) : to_tile<64, false>(acc, scratch);
+            const float out = ldexpf(1.0f, -(e0 + qexp));
+            T *dst = reinterpret_cast<T *>(M.dst) + bi * M.dst_stride;
+            const int c0 = x * 32;      // columns of X: rows of a tall result
+            for (int q = threadIdx.x; q < 64 * 64; q += kThreads) {
+                const int r = q >> 6, c = q & 63, row = M.tall ? c0 + r : r, col = M.tall ? c : c0 + c;
+                if (row < (M.tall ? n : m) && col < cols) dst[(long)row * M.dst_ld + col] = from_f<T>(out * tile[r * Geo<64>::PITCH + c]);
+            }
+        }
+    }
+}
+constexpr int kSmallSide = 64, kSmallLong = 320;      // (10 lines of X: 148 KB of LDS with A, P, Q and the tile)
 
 // ---- Adam for the vectors (the same arithmetic as tef_adam_clip_step, over a list of ranges of the flat buffers) --------------------
 constexpr int kRanges = 96;
@@ -793,15 +1058,15 @@ inline long triangle_tiles(int mp, int ts)
 }
 
 // How the tiles of ONE matrix's product are dealt to 256 CUs: as many as are a multiple of 256 whole, the rest cut along k so that the
-// pieces, too, are about 256 (512 when there is nothing else to run beside them), of at least 8 lines: a piece's sums have to be
+// pieces, too, are about 256 (512 of the large tiles when there is nothing else to run beside them), of at least 8 lines: a piece's sums have to be
 // written and read again, and joining takes a launch of its own (about 10 us), so products of fewer than 32 lines are left alone.
 // 4096 x 4096: 528 tiles take 280 us whole — two on every CU, then the last 16 — and 180 us with those 16 in pieces.
-Cut cut_one(long tiles, long lines)
+Cut cut_one(long tiles, long lines, int ts)
 {
     Cut c{(int)tiles, 1, tiles, 0};
     const long rest = tiles % 256;
     if (lines < 32 || tiles > (1l << 24) || !rest) return c;
-    long s = tiles < 256 ? 512 / tiles : 256 / rest;
+    long s = tiles < 256 ? (ts == 128 ? 512 : 256) / tiles : 256 / rest;
     if (s > lines / 8) s = lines / 8;
     if (s < 2) return c;
     if (s > 64) s = 64;
@@ -825,8 +1090,11 @@ void plan(Group &g)
         steps128 += (long)M.batch * triangle_tiles(M.mp, 128) * (M.np / 32);
     }
     g.ts_chain = chain128 >= 256 || (g.n == 1 && chain128 >= 64 && g.m[0].mp >= 1024) ? 128 : 64;
+    long chain32 = 0;
+    for (int k = 0; k < g.n; ++k) chain32 += (long)g.m[k].batch * triangle_tiles(g.m[k].mp, 32);
+    if (g.ts_chain == 64 && chain32 <= 512) g.ts_chain = 32;
     g.ts_gram = steps128 >= 256 * 16 ? 128 : 64;
-    g.ts_apply = apply128 >= 256 ? 128 : 64;
+    g.ts_apply = apply128 >= 192 ? 128 : 64;
     // a list: every tile of the Gram products in pieces of one length, the shortest that gives no more pieces than run at once
     long piece = 8, slots = g.ts_gram == 128 ? 512 : 1024;
     if (g.n > 1)
@@ -847,11 +1115,12 @@ void plan(Group &g)
         const long tiles = triangle_tiles(M.mp, g.ts_gram), lines = M.np / 32;
         long splits = (lines + piece - 1) / piece, parts = 0;
         if (g.n == 1) {
-            g.gram = cut_one(tiles * M.batch, lines);
+            g.gram = cut_one(tiles * M.batch, lines, g.ts_gram);
             parts = g.gram.joins * g.gram.splits * g.ts_gram * g.ts_gram;
             splits = 1;
             for (int w = 0; w < 2; ++w) {
-                g.chain[w] = cut_one(triangle_tiles(M.mp, g.ts_chain) * M.batch * (w + 1), M.mp / 32);
+                const long all = triangle_tiles(M.mp, g.ts_chain) * M.batch * (w + 1);
+                g.chain[w] = g.ts_chain == 32 ? Cut{(int)all, 1, all, 0} : cut_one(all, M.mp / 32, g.ts_chain);
                 const long p = g.chain[w].joins * g.chain[w].splits * g.ts_chain * g.ts_chain;
                 parts = parts > p ? parts : p;
             }
@@ -924,6 +1193,10 @@ int iterate(Group &g, const Poly &p, double eps, char *ws, const Step &st, hipSt
         c.splits = cut.splits;
         const dim3 grid((unsigned)cut.items);
         const bool deep = cut.items <= 256;
+        if (ts == 32) {
+            hipLaunchKernelGGL(ortho_symmetric32, grid, block, 0, stream, t, ws, c);
+            return;
+        }
         if (ts == 128) {
             if (deep) hipLaunchKernelGGL((ortho_symmetric<128, true>), grid, block, 0, stream, t, ws, c);
             else hipLaunchKernelGGL((ortho_symmetric<128, false>), grid, block, 0, stream, t, ws, c);
@@ -988,6 +1261,34 @@ int iterate(Group &g, const Poly &p, double eps, char *ws, const Step &st, hipSt
         }
     }
     return tef::check_launch("orthogonalisation");
+}
+
+// One workgroup a matrix when every matrix of the group is small enough: 26 us against 85 for a single 64 x 18 one.
+template <typename T> int small(const Group &g, const Poly &p, double eps, hipStream_t stream)
+{
+    const SmallPoly sp{p.a, p.b, p.c, p.steps, p.seg_len, eps};
+    for (int at = 0; at < g.n; at += kChunk) {
+        Small list;
+        list.n = g.n - at < kChunk ? g.n - at : kChunk;
+        int items = 0, longest = 0;
+        for (int k = 0; k < list.n; ++k) {
+            list.m[k] = g.m[at + k];
+            list.first[k] = items;
+            items += g.m[at + k].batch;
+            longest = longest > g.m[at + k].n ? longest : g.m[at + k].n;
+        }
+        const dim3 grid((unsigned)items), block(kThreads);
+        if (longest <= 64) hipLaunchKernelGGL((ortho_small<T, 2>), grid, block, 0, stream, list, sp);
+        else if (longest <= 128) hipLaunchKernelGGL((ortho_small<T, 4>), grid, block, 0, stream, list, sp);
+        else hipLaunchKernelGGL((ortho_small<T, 10>), grid, block, 0, stream, list, sp);
+    }
+    return tef::check_launch("orthogonalisation");
+}
+bool all_small(const Group &g)
+{
+    for (int k = 0; k < g.n; ++k)
+        if (g.m[k].m > kSmallSide || g.m[k].n > kSmallLong) return false;
+    return true;
 }
 
 bool polynomial(Poly &p, int steps, double a, double b, double c, double eps)
@@ -1064,6 +1365,13 @@ int tef_orthogonalize(const tef_ortho_matrix *matrices, int count, int dtype, in
     Group g;
     for (int at = 0; at < count; at += kGroup) {
         if (!group_of(g, matrices, at, count)) return TEF_ERR_INVALID;
+        if (all_small(g)) {
+            const int rc = dtype == TEF_F32 ? small<float>(g, p, eps, (hipStream_t)stream)
+                         : dtype == TEF_F16 ? small<__half>(g, p, eps, (hipStream_t)stream)
+                                            : small<__hip_bfloat16>(g, p, eps, (hipStream_t)stream);
+            if (rc) return rc;
+            continue;
+        }
         const Step none{};
         const int rc = dtype == TEF_F32 ? iterate<float, false>(g, p, eps, (char *)workspace, none, (hipStream_t)stream)
                      : dtype == TEF_F16 ? iterate<__half, false>(g, p, eps, (char *)workspace, none, (hipStream_t)stream)

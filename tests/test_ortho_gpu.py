@@ -93,7 +93,8 @@ def matrix(kind, rows, cols, seed=0):
     raise KeyError(kind)
 
 
-SIZES = [(1, 1), (1, 7), (7, 1), (2, 3), (31, 33), (32, 32), (64, 18), (18, 64), (33, 65), (64, 64), (65, 64), (64, 576), (100, 7), (96, 160),
+# (both sides of every limit of the variants: 64 / 65 rows, 64 / 128 / 320 columns, tiles of 32, 64 and 128)
+SIZES = [(64, 65), (50, 129), (64, 320), (320, 64), (64, 321), (10, 300), (65, 65), (513, 520), (1030, 1100), (1, 1), (1, 7), (7, 1), (2, 3), (31, 33), (32, 32), (64, 18), (18, 64), (33, 65), (64, 64), (65, 64), (64, 576), (100, 7), (96, 160),
          (128, 128), (129, 257), (1, 5000), (300, 2), (257, 130), (512, 1000), (385, 1111), (1111, 385), (640, 640)]
 
 
