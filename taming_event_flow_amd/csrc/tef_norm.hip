@@ -680,7 +680,7 @@ int tef_layer_norm_forward(const tef_norm_desc *d, const void *x, const void *we
     a.x = x; a.res = residual; a.y = y; a.mean = mean; a.rstd = rstd;
     a.v = Vecs{weight, bias, d->wdtype};
     a.rows = (long)d->outer * d->inner; a.inner = d->inner; a.C = d->channels; a.act = d->act; a.eps = d->eps;
-    const long most = 1l << 20;      // (the kernels stride over what a grid of that size leaves)
+    const long most = p.kind <= 1 ? 2048 : 1l << 20;      // rows: a workgroup keeps the weights of its columns over several rows
     launch(*d, p, false, (unsigned)(p.tiles < most ? p.tiles : most), (hipStream_t)stream, a);
     return tef::check_launch("layer norm forward");
 }
