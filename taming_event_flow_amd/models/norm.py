@@ -32,9 +32,14 @@ class _LayerNormFn(torch.autograd.Function):
     def forward(ctx, x, weight, bias, residual, dim, eps, act):
         # a map in channels-last memory is a matrix of rows as it stands; anything else is taken in x's own dimension order
         shape = x.shape
-        last = x if dim == len(shape) - 1 else x.movedim(dim, -1)
-        rows = last.is_contiguous()
-        xc = last if rows else x.contiguous()
+        if dim == len(shape) - 1:
+            xc, rows = x.contiguous(), True
+        elif x.is_contiguous():
+            xc, rows = x, False
+        else:
+            last = x.movedim(dim, -1)
+            rows = last.is_contiguous()
+            xc = last if rows else x.contiguous()
         rc = residual
         if rc is not None:
             rc = (rc.movedim(dim, -1) if rows else rc).contiguous()
@@ -73,7 +78,8 @@ class _LayerNormFn(torch.autograd.Function):
         dr = torch.empty_like(xc) if need_r else None
         lib, dw, db, ws, nbytes = _lib.lib(), None, None, None, 0
         if need_w or need_b:
-            dw, db = torch.empty((2, d.channels), dtype=_TORCH[d.wdtype], device=xc.device).unbind(0)
+            dw = torch.empty((d.channels,), dtype=_TORCH[d.wdtype], device=xc.device) if need_w else None
+            db = torch.empty((d.channels,), dtype=_TORCH[d.wdtype], device=xc.device) if need_b else None
             nbytes = lib.tef_layer_norm_workspace_bytes(ctypes.byref(d))
             ws = torch.empty((nbytes,), dtype=torch.uint8, device=xc.device)
         at = stats.data_ptr()
@@ -83,7 +89,7 @@ class _LayerNormFn(torch.autograd.Function):
         _lib.check(code, "tef_layer_norm_backward")
         if rows:
             dx, dr = (t.movedim(-1, dim) if t is not None else None for t in (dx, dr))
-        return dx, dw if need_w else None, db if need_b else None, dr, None, None, None
+        return dx, dw, db, dr, None, None, None
 
 
 def layer_norm(x, weight=None, bias=None, dim=1, eps=1e-5, activation=None, residual=None):
