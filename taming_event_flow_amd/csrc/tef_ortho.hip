@@ -5,17 +5,25 @@
 //
 //   A = X X^T,  P = a I + b A + c A A,  X <- P X            (the singular values go through  a s + b s^3 + c s^5)
 //
-// is run on the small side: P is a polynomial of A, so A' = X' X'^T = P A P and X_k = Q_k X_0 with Q' = P Q, and a segment of up to
-// three steps needs ONE Gram matrix of X and ONE product Q X; in between all matrices are m x m, symmetric, and commute
-// (products of them are symmetric: half of the tiles are computed, the other half mirrored).  The recurrence for A amplifies
-// its rounding errors by up to a^2 = 12 a step where the direct iteration amplifies them by a: after three steps the Gram
-// matrix is formed anew from X (five steps: 3 + 2), which keeps the result within a small factor of a plain fp32 iteration on
-// rank-deficient matrices too; all five in one segment lose a further digit.  Work for five steps, in multiply-adds
-// with symmetric products counted half: 3 m^2 n + 7 m^3 instead of 7.5 m^2 n + 2.5 m^3.
+// can be run on the small side: P is a polynomial of A, so A' = X' X'^T = P A P and X_k = Q_k X_0 with Q' = P Q, and a segment of
+// steps needs ONE Gram matrix of X and ONE product Q X; in between all matrices are m x m, symmetric, and commute (products of
+// them are symmetric: half of the tiles are computed, the other half mirrored).  Every matrix close to a multiple of the identity is kept as its
+// difference from it — P = a (I + B), B = (b/a) A + (c/a) A A, and Q = q (I + R), q = a^k — so that nothing small is rounded at the size of
+// a diagonal:
+//
+//   W = A (I + B),  A' = a^2 W (I + B),  R' = R (I + B) + B,  X' = q (I + R) X
+//
+// where what the I brings is added to a product's fp32 sums unrounded.  The recurrence
+// for A multiplies its rounding errors by up to a^2 = 12 a step along small singular values, the direct iteration by a; against the plain
+// iteration in fp32, on gradients of rank m / 4 to m, segments of 2, 1, 1, 1 steps are 1.05 to 1.2 times as far from 64 bits
+// (1.4 below 64 rows), 3 + 2 steps 1.5 to 3.5 times.  orthogonalize() takes the former: 12 m^2 n + 8 m^3 / 2
+// multiply-adds (symmetric products at half) where the plain iteration takes 20 m^2 n + 10 m^3 over 2; small matrices go step by step.
+// The optimiser takes the latter, 6 m^2 n + 14 m^3 over 2: its update is scaled by the learning rate and added to fp32 parameters, whose own
+// rounding is as large as that error.
 //
 // Arithmetic.  fp32 matrix instructions run at 1/16 of the fp16 rate, so every operand is held as two fp16 planes, v = hi + lo
 // with hi = fp16(v), lo = fp16(v - hi) — 22 bits — and a product is hi hi + hi lo + lo hi with fp32 accumulation; the dropped lo lo
-// is 2^-22 of the product.  All matrices have bounded entries (|X|, |A|, |P| <= a few; |Q| <= a^3), so a fixed power of two
+// is 2^-22 of the product.  All matrices have bounded entries (|X|, |A|, |B|, |R| of the order of 1), so a fixed power of two
 // per matrix kind puts them into fp16's normal range.  Nothing is rounded to a single fp16 anywhere.
 //
 // Layout.  A split matrix is [rows][cols / 32][hi 32 | lo 32]: a row's 32 columns are one 128-byte line with both planes, so a
@@ -42,8 +50,7 @@ constexpr int kThreads = 256;
 constexpr int kGroup = 64;             // matrices (with their batches) a set of launches takes
 constexpr int kChunk = 16;             // of them per kernel argument
 constexpr int kMaxParts = 512;         // partial sums of a matrix's squares
-constexpr int kSegment = 3;            // steps between two Gram matrices
-constexpr int kExpX = 12, kExpA = 12, kExpP = 12, kExpQ = 10;      // powers of two the split matrices are scaled by
+constexpr int kExpX = 12, kExpA = 12, kExpB = 12;      // powers of two that X, that A and W, that B and R are scaled by
 
 // What the kernels know of a matrix (a batch of equal ones): lives in the workspace, written by the first launch.
 struct Mat {
@@ -68,7 +75,7 @@ enum { PH_SQ = 0, PH_PACK, PH_GRAM, PH_JOIN, PH_CHAIN, PH_APPLY, PHASES };
 // and not, as with 4096 columns, 16 KB apart in one of them.
 __host__ __device__ inline long pitch(int cols) { return ((cols / 32) | 1) * 128l; }
 __host__ __device__ inline long split_bytes(int rows, int cols) { return rows * pitch(cols); }
-enum { BUF_X0 = 0, BUF_X1, BUF_A, BUF_W, BUF_P0, BUF_P1, BUF_Q0, BUF_Q1, BUF_END };
+enum { BUF_X0 = 0, BUF_X1, BUF_A, BUF_W, BUF_B0, BUF_B1, BUF_R0, BUF_R1, BUF_END };
 constexpr int kMaxSteps = 32;
 constexpr long kHead = kMaxParts * 8 + 256;      // (a multiple of 256, at least 4 * (kMaxSteps + 1) past the sums)
 __host__ __device__ inline long buf_at(int which, int mp, int np)
@@ -109,6 +116,9 @@ template <typename T, int V> struct __attribute__((packed, aligned(sizeof(T)))) 
 
 __device__ inline void split(float v, _Float16 &hi, _Float16 &lo)
 {
+    // v as ONE rounded number: without this the compiler forms a product's hi in one instruction from the unrounded product where hi is
+    // stored, and from the rounded one where it is subtracted; near a tie the two differ by a unit of hi and lo belongs to the other
+    asm("" : "+v"(v));
     hi = (_Float16)v;
     lo = (_Float16)(v - (float)hi);      // (infinite hi: NaN, as an overflow should show)
 }
@@ -223,7 +233,7 @@ template <typename T, bool STEP> __global__ __launch_bounds__(kThreads) void ort
 // ---- phase 1: normalise and split ---------------------------------------------------------------------------------------------
 // A workgroup writes 32 rows x 64 columns of the padded X (8 values a thread).  The scale is kExpX plus, where |U| < eps leaves
 // X small, the power of two that brings it back up: what is multiplied later always has 22 good bits.
-template <typename T, bool STEP> __global__ __launch_bounds__(kThreads) void ortho_pack(Table t, char *ws, double eps, Step st)
+template <typename T, bool STEP> __global__ __launch_bounds__(kThreads) void ortho_pack(Table t, char *ws, double eps, int grow_first, int grow_rest, Step st)
 {
     __shared__ double red[4];
     __shared__ float turn[64][33];
@@ -244,8 +254,9 @@ template <typename T, bool STEP> __global__ __launch_bounds__(kThreads) void ort
     if (wg % tiles == 0 && threadIdx.x == 0) {
         int *e = reinterpret_cast<int *>(area + kMaxParts * 8);
         e[0] = kExpX + up;
-        for (int k = 1; k <= kMaxSteps; ++k) {      // a segment multiplies X by at most 2^6
-            up = up > 6 ? up - 6 : 0;
+        for (int k = 1; k <= kMaxSteps; ++k) {      // a segment multiplies X by at most 2^grow
+            up -= k == 1 ? grow_first : grow_rest;
+            up = up > 0 ? up : 0;
             e[k] = kExpX + up;
         }
         up = e[0] - kExpX;
@@ -382,6 +393,16 @@ template <int TS> __device__ inline half8 frag_cols(const char *lds, int col0, i
 
 template <int TS> struct Acc { float16v v[Geo<TS>::FR][Geo<TS>::FR]; };
 
+// the identity's 32 x 16 block s (rows or columns this lane's, k = 16 s + 8 (lane >> 5) ..), times v
+__device__ inline half8 identity(int s, _Float16 v)
+{
+    const int lane = threadIdx.x & 63, at = (lane & 31) - s * 16 - (lane >> 5) * 8;
+    half8 f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = at == k ? v : (_Float16)0.0f;
+    return f;
+}
+
 // acc = L (rows li0 ..) times R (rows rj0 .. as columns, or, COLS, the 32-column blocks rj0 / 32 ..), k lines k0 .. k1
 template <int TS, int AHEAD, bool COLS>
 __device__ inline void product(Acc<TS> &acc, char *lds, const char *L, long ldL, int li0, int rowsL, const char *R, long ldR, int rj0, int limR, int k0, int k1)
@@ -456,6 +477,29 @@ __device__ inline void product(Acc<TS> &acc, char *lds, const char *L, long ldL,
 #undef TEF_PUT
 }
 
+// acc += one * M, the tile (i0, j0) of a split matrix, straight from memory: M's rows times an identity, exact (one: a power of two)
+template <int TS> __device__ inline void add_tile(Acc<TS> &acc, const char *M, int rows, int cols, int i0, int j0, float one)
+{
+    using G = Geo<TS>;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = (wave >> 1) * (TS / 2), wj = (wave & 1) * (TS / 2);
+#pragma unroll
+    for (int i = 0; i < G::FR; ++i)
+#pragma unroll
+        for (int j = 0; j < G::FR; ++j) {
+            const int row = i0 + wi + i * 32 + (lane & 31), line = ((j0 + wj) >> 5) + j, lines = cols / 32;
+            const char *p = M + (row < rows ? row : rows - 1) * pitch(cols) + (line < lines ? line : lines - 1) * 128 + (lane >> 5) * 16;
+            half8 f[2][2];
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int pl = 0; pl < 2; ++pl) f[s][pl] = *reinterpret_cast<const half8 *>(p + pl * 64 + s * 32);
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int pl = 0; pl < 2; ++pl) acc.v[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[s][pl], identity(s, (_Float16)one), acc.v[i][j], 0, 0, 0);
+        }
+}
+
 // The finished tile in LDS, row-major or, TURN, transposed (a lane of a 32 x 32 block holds column lane & 31 and the rows
 // 8 (e / 4) + 4 (lane >> 5) + e % 4: four neighbours of a row of the transposed tile, one 16-byte write); either way free of
 // bank conflicts, and read back in rows.
@@ -507,15 +551,14 @@ template <int TS> __device__ inline float *to_tile_upper(const Acc<TS> &acc, cha
     return tile;
 }
 
-// Writes rows row0 .. of the tile in LDS to the split matrix `out`, from column col0 on: mul * value + (POLY: the rest of
-// P = a I + b A + c A A).
-template <int TS, bool POLY>
-__device__ inline void put_tile(const float *tile, char *out, int rows, int cols, int row0, int col0, float mul, char *A, float pa, float pb)
+// Writes rows row0 .. of the tile in LDS to the split matrix `out`, from column col0 on: mul * value (+ PLUS: plus * A).
+template <int TS, bool PLUS>
+__device__ inline void put_tile(const float *tile, char *out, int rows, int cols, int row0, int col0, float mul, char *A, float plus)
 {
     constexpr int per = TS / 8, ROUNDS = TS * per / kThreads, BATCH = ROUNDS < 4 ? ROUNDS : 4;
     for (int at = 0; at < ROUNDS; at += BATCH) {
         half8 hi[BATCH], lo[BATCH];
-        if (POLY)
+        if (PLUS)
 #pragma unroll
             for (int i = 0; i < BATCH; ++i) {      // (on their way before the first value is needed)
                 const int q = threadIdx.x + (at + i) * kThreads, row = row0 + q / per, col = col0 + q % per * 8;
@@ -530,7 +573,7 @@ __device__ inline void put_tile(const float *tile, char *out, int rows, int cols
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 f[k] = mul * tile[r * Geo<TS>::PITCH + c + k];
-                if (POLY) f[k] += pb * ((float)hi[i][k] + (float)lo[i][k]) + (row == col + k ? pa : 0.0f);
+                if (PLUS) f[k] += plus * ((float)hi[i][k] + (float)lo[i][k]);
             }
             if (row < rows && col < cols) put_split(out, cols, row, col, f);
         }
@@ -540,11 +583,11 @@ __device__ inline void put_tile(const float *tile, char *out, int rows, int cols
 // ... of a symmetric matrix: the tile (i0, j0) and its mirror image.  A diagonal tile holds both triangles, the same products added
 // up in another order: the upper one is taken for both.  (The iteration relies on it: an asymmetry of one rounding grows with every step and
 // cost a factor of twelve in the result of a 40 x 300 matrix of rank one.)
-template <int TS, bool POLY>
-__device__ inline void put_symmetric(const Acc<TS> &acc, char *lds, char *out, int mp, int i0, int j0, float mul, char *A, float pa, float pb)
+template <int TS, bool PLUS>
+__device__ inline void put_symmetric(const Acc<TS> &acc, char *lds, char *out, int mp, int i0, int j0, float mul, char *A, float plus)
 {
-    put_tile<TS, POLY>(i0 == j0 ? to_tile_upper<TS>(acc, lds) : to_tile<TS, false>(acc, lds), out, mp, mp, i0, j0, mul, A, pa, pb);
-    if (i0 != j0) put_tile<TS, POLY>(to_tile<TS, true>(acc, lds), out, mp, mp, j0, i0, mul, A, pa, pb);
+    put_tile<TS, PLUS>(i0 == j0 ? to_tile_upper<TS>(acc, lds) : to_tile<TS, false>(acc, lds), out, mp, mp, i0, j0, mul, A, plus);
+    if (i0 != j0) put_tile<TS, PLUS>(to_tile<TS, true>(acc, lds), out, mp, mp, j0, i0, mul, A, plus);
 }
 
 // tile number -> (i, j), j >= i, of a symmetric matrix of T x T tiles: eight columns at a time, so that 64 consecutive tiles, which run
@@ -574,10 +617,11 @@ __device__ inline void triangle(int t, int T, int &i, int &j)
 // piece's fp32 sums go to the workspace as the threads hold them and ortho_join adds them up in order.
 struct Sym {
     int l[2], r[2], out[2];            // buffers
-    float mul[2];
+    float mul[2];                      // of the values
+    int plus_l[2], plus_r[2];          // add L, add R to the product (at the scale of B: the other factor is I + ..)
     int products;
-    int poly;                          // product 0 is A A, its result P = a I + b A + c A A
-    float pa, pb;
+    int poly;                          // product 0 is A A, its result B
+    float plus;
     int gram, seg;                     // product 0 is X X^T of this segment's X
     int whole, splits;
 };
@@ -606,10 +650,10 @@ template <int TS> __device__ inline void finish(const Acc<TS> &acc, char *lds, c
 {
     char *out = area + buf_at(c.out[p.w], M.mp, M.np);
     if (c.poly) {
-        put_symmetric<TS, true>(acc, lds, out, M.mp, p.ti * TS, p.tj * TS, c.mul[p.w], area + buf_at(c.l[p.w], M.mp, M.np), c.pa, c.pb);
+        put_symmetric<TS, true>(acc, lds, out, M.mp, p.ti * TS, p.tj * TS, c.mul[p.w], area + buf_at(c.l[p.w], M.mp, M.np), c.plus);
     } else {
         const float mul = c.gram ? ldexpf(1.0f, kExpA - 2 * reinterpret_cast<const int *>(area + kMaxParts * 8)[c.seg]) : c.mul[p.w];
-        put_symmetric<TS, false>(acc, lds, out, M.mp, p.ti * TS, p.tj * TS, mul, nullptr, 0.0f, 0.0f);
+        put_symmetric<TS, false>(acc, lds, out, M.mp, p.ti * TS, p.tj * TS, mul, nullptr, 0.0f);
     }
 }
 // DEEP: at most one workgroup a CU, which then has the registers for twice the lines in flight.
@@ -625,6 +669,10 @@ template <int TS, bool DEEP> __global__ __launch_bounds__(kThreads, DEEP ? 1 : 2
     const int k0 = (int)((long)lines * p.piece / p.pieces), k1 = (int)((long)lines * (p.piece + 1) / p.pieces);
     Acc<TS> acc;
     product<TS, (TS == 64 ? 4 : 2) * (DEEP ? 2 : 1), false>(acc, lds, L, pitch(side), p.ti * TS, M.mp, R, pitch(side), p.tj * TS, M.mp, k0, k1);
+    if (p.piece == 0) {
+        if (c.plus_l[p.w]) add_tile<TS>(acc, L, M.mp, M.mp, p.ti * TS, p.tj * TS, (float)(1 << kExpB));
+        if (c.plus_r[p.w]) add_tile<TS>(acc, R, M.mp, M.mp, p.ti * TS, p.tj * TS, (float)(1 << kExpB));
+    }
     if (p.pieces == 1) return finish<TS>(acc, lds, M, area, c, p);
     float *part = reinterpret_cast<float *>(ws + M.part) + ((long)p.slot * p.pieces + p.piece) * TS * TS;
 #pragma unroll
@@ -689,12 +737,14 @@ __global__ __launch_bounds__(kThreads) void ortho_symmetric32(Table t, char *ws,
     const long ld = pitch(M.mp), at = (lane >> 5) * 16;
     const char *L = area + buf_at(c.l[w], M.mp, M.np) + (ti * TS + (lane & 31)) * ld + at, *R = area + buf_at(c.r[w], M.mp, M.np) + (tj * TS + (lane & 31)) * ld + at;
     const int r = threadIdx.x >> 3, q = (threadIdx.x & 7) * 4, row = ti * TS + r, col = tj * TS + q;
-    half4 ahi, alo;
-    if (c.poly) {
-        const _Float16 *p = split_at(area + buf_at(c.l[w], M.mp, M.np), M.mp, row, col);
-        ahi = *reinterpret_cast<const half4 *>(p);
-        alo = *reinterpret_cast<const half4 *>(p + 32);
-    }
+    half4 hi[2], lo[2];      // this thread's part of L and R, where they are added
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+        if (k ? c.plus_r[w] : c.plus_l[w] | c.poly) {
+            const _Float16 *p = split_at(area + buf_at(k ? c.r[w] : c.l[w], M.mp, M.np), M.mp, row, col);
+            hi[k] = *reinterpret_cast<const half4 *>(p);
+            lo[k] = *reinterpret_cast<const half4 *>(p + 32);
+        }
     float16v acc;
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[e] = 0.0f;
@@ -727,31 +777,33 @@ __global__ __launch_bounds__(kThreads) void ortho_symmetric32(Table t, char *ws,
     for (int k = 1; k < 4; ++k) f += *reinterpret_cast<const float4v *>(&sums[k][r * PITCH + q]);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
+        if (c.plus_l[w]) f[k] += (float)(1 << kExpB) * ((float)hi[0][k] + (float)lo[0][k]);
+        if (c.plus_r[w]) f[k] += (float)(1 << kExpB) * ((float)hi[1][k] + (float)lo[1][k]);
         f[k] *= c.mul[w];
-        if (c.poly) f[k] += c.pb * ((float)ahi[k] + (float)alo[k]) + (row == col + k ? c.pa : 0.0f);
+        if (c.poly) f[k] += c.plus * ((float)hi[0][k] + (float)lo[0][k]);
         done[r * (TS + 1) + q + k] = f[k];
     }
     __syncthreads();
     char *out = area + buf_at(c.out[w], M.mp, M.np);
     for (int mirror = 0; mirror < (ti == tj ? 1 : 2); ++mirror) {
-        half4 hi, lo;
+        half4 vhi, vlo;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {      // (the diagonal tile: its upper triangle for both, see put_symmetric)
             const bool turn = mirror || (ti == tj && r > q + k);
             _Float16 h, lw;
             split(turn ? done[(q + k) * (TS + 1) + r] : f[k], h, lw);
-            hi[k] = h;
-            lo[k] = lw;
+            vhi[k] = h;
+            vlo[k] = lw;
         }
         _Float16 *p = split_at(out, M.mp, mirror ? tj * TS + r : row, mirror ? ti * TS + q : col);
-        *reinterpret_cast<half4 *>(p) = hi;
-        *reinterpret_cast<half4 *>(p + 32) = lo;
+        *reinterpret_cast<half4 *>(p) = vhi;
+        *reinterpret_cast<half4 *>(p + 32) = vlo;
     }
 }
 
-// ---- phase 4: X' = Q X, into the other X, the caller's matrix, or the parameters -------------------------------------------------
+// ---- phase 4: X' = q (I + R) X, into the other X, the caller's matrix, or the parameters -------------------------------------------------
 enum { TO_X = 0, TO_DST, TO_PARAM };
-template <int TS, typename T, int DEST> __global__ __launch_bounds__(kThreads, 2) void ortho_apply(Table t, char *ws, int seg, int q, int qexp, Step st)
+template <int TS, typename T, int DEST> __global__ __launch_bounds__(kThreads, 2) void ortho_apply(Table t, char *ws, int seg, int r_buf, float q, Step st)
 {
     __shared__ __attribute__((aligned(16))) char lds[Geo<TS>::LDS];
     const int item = work_item();
@@ -764,13 +816,14 @@ template <int TS, typename T, int DEST> __global__ __launch_bounds__(kThreads, 2
     const int *ex = reinterpret_cast<const int *>(area + kMaxParts * 8);
     const int e0 = ex[seg], e1 = ex[seg + 1];
     Acc<TS> acc;
-    product<TS, TS == 64 ? 4 : 2, true>(acc, lds, area + buf_at(q, M.mp, M.np), pitch(M.mp), ti * TS, M.mp, X, pitch(M.np), tj * TS, M.np / 32, 0, M.mp / 32);
+    product<TS, TS == 64 ? 4 : 2, true>(acc, lds, area + buf_at(r_buf, M.mp, M.np), pitch(M.mp), ti * TS, M.mp, X, pitch(M.np), tj * TS, M.np / 32, 0, M.mp / 32);
+    add_tile<TS>(acc, X, M.mp, M.np, ti * TS, tj * TS, (float)(1 << kExpB));
     if constexpr (DEST == TO_X) {
-        put_tile<TS, false>(to_tile<TS, false>(acc, lds), area + buf_at(seg & 1 ? BUF_X0 : BUF_X1, M.mp, M.np), M.mp, M.np, ti * TS, tj * TS, ldexpf(1.0f, e1 - e0 - qexp), nullptr, 0.0f, 0.0f);
+        put_tile<TS, false>(to_tile<TS, false>(acc, lds), area + buf_at(seg & 1 ? BUF_X0 : BUF_X1, M.mp, M.np), M.mp, M.np, ti * TS, tj * TS, ldexpf(q, e1 - e0 - kExpB), nullptr, 0.0f);
         return;
     }
     // the result, in the caller's orientation: row r of the output tile, four neighbours of it
-    const float mul = ldexpf(1.0f, -(e0 + qexp));
+    const float mul = ldexpf(q, -(e0 + kExpB));
     float keep = 1.0f, step = 1.0f;
     if constexpr (DEST == TO_PARAM) {
         keep = (float)(1.0 - st.hp[0] * st.hp[2]);
@@ -810,10 +863,10 @@ template <int TS, typename T, int DEST> __global__ __launch_bounds__(kThreads, 2
 }
 
 // ---- small matrices: the whole iteration in one workgroup --------------------------------------------------------------------------
-// m <= 64 and at most 32 LINES columns: X, A, P and Q stay in LDS as split matrices (line l: 64 rows of 128 bytes, permuted as the
+// m <= 64 and at most 32 LINES columns: X, A, B and R stay in LDS as split matrices (line l: 64 rows of 128 bytes, permuted as the
 // stages above) and one launch does what the general path spreads over twenty, each a few microseconds of latency whatever the
-// size.  A product's values are in registers when its operands have been read, so it overwrites one of them: W = A P goes to A's
-// place, Q P to Q's, A' = W P to W's.
+// size.  X <- q (I + R) X goes to X's own place (a tile's values are in registers when its columns have been read), and so does every
+// other product to one of its operands'.
 __device__ inline char *line_at(char *m, int line) { return m + line * (64 * 128); }
 // acc = L R^T over `lines` lines (this wave's 32 x 32 block)
 __device__ inline void small_rows(Acc<64> &acc, const char *L, const char *R, int lines)
@@ -834,8 +887,8 @@ __device__ inline void small_rows(Acc<64> &acc, const char *L, const char *R, in
             for (int t = 0; t < 3; ++t) acc.v[0][0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[t == 0], b[t == 1], acc.v[0][0], 0, 0, 0);
         }
 }
-// acc = Q X over `lines` lines of Q, for the two lines of X from `X` on (64 columns; X's rows are k)
-__device__ inline void small_cols(Acc<64> &acc, const char *Q, const char *X, int lines)
+// acc = (B + one I) X over `lines` lines of B, for the two lines of X from `X` on (64 columns; X's rows are k)
+__device__ inline void small_cols(Acc<64> &acc, const char *B, const char *X, int lines, _Float16 one)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = (wave >> 1) * 32, g = lane >> 4, src = lane & 15;
     const char *x = X + (wave & 1) * 8192;
@@ -847,7 +900,7 @@ __device__ inline void small_cols(Acc<64> &acc, const char *Q, const char *X, in
             half8 a[2], b[2];
 #pragma unroll
             for (int pl = 0; pl < 2; ++pl) {
-                a[pl] = frag_rows(Q + l * 8192, wi + (lane & 31), s, pl);
+                a[pl] = frag_rows(B + l * 8192, wi + (lane & 31), s, pl);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {      // four k of this lane's column: see frag_cols
                     const int row = l * 32 + s * 16 + (g >> 1) * 8 + h * 4 + (src >> 2), col = (g & 1) * 16 + (src & 3) * 4;
@@ -859,27 +912,36 @@ __device__ inline void small_cols(Acc<64> &acc, const char *Q, const char *X, in
             }
 #pragma unroll
             for (int t = 0; t < 3; ++t) acc.v[0][0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[t == 0], b[t == 1], acc.v[0][0], 0, 0, 0);
+            if (l * 32 == wi)
+#pragma unroll
+                for (int pl = 0; pl < 2; ++pl) acc.v[0][0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(identity(s, one), b[pl], acc.v[0][0], 0, 0, 0);
         }
 }
 __device__ inline char *small_at(char *m, int row, int col, int plane)      // 16 bytes: eight columns from `col` on
 {
     return line_at(m, col >> 5) + row * 128 + (((plane * 4 + ((col & 31) >> 3)) ^ (row >> 1 & 7)) << 4);
 }
-// 64 x 64 values of the tile to the split matrix `out` (two lines); POLY as in put_tile, A and out may not be the same
-template <bool POLY> __device__ inline void small_put(const float *tile, char *out, float mul, char *A, float pa, float pb)
+// mul times the 64 x 64 values of the tile, PLUS: plus * A (+ B), to the split matrix `out` (two lines; A's own place too: a thread
+// writes the values that it has read)
+template <bool PLUS> __device__ inline void small_put(const float *tile, char *out, float mul, char *A, float plus, char *B = nullptr)
 {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int q = threadIdx.x + i * kThreads, r = q >> 3, c = (q & 7) * 8;
-        half8 hi, lo;
-        if (POLY) {
+        half8 hi, lo, bhi, blo;
+        if (PLUS) {
             hi = *reinterpret_cast<const half8 *>(small_at(A, r, c, 0));
             lo = *reinterpret_cast<const half8 *>(small_at(A, r, c, 1));
+            if (B) {
+                bhi = *reinterpret_cast<const half8 *>(small_at(B, r, c, 0));
+                blo = *reinterpret_cast<const half8 *>(small_at(B, r, c, 1));
+            }
         }
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             float f = mul * tile[r * Geo<64>::PITCH + c + k];
-            if (POLY) f += pb * ((float)hi[k] + (float)lo[k]) + (r == c + k ? pa : 0.0f);
+            if (PLUS) f += plus * ((float)hi[k] + (float)lo[k]);
+            if (PLUS && B) f += (float)bhi[k] + (float)blo[k];
             _Float16 h, l;
             split(f, h, l);
             hi[k] = h;
@@ -892,7 +954,7 @@ template <bool POLY> __device__ inline void small_put(const float *tile, char *o
 }
 
 struct Small { Mat m[kChunk]; int first[kChunk]; int n; };
-struct SmallPoly { float a, b, c; int steps, seg_len; double eps; };
+struct SmallPoly { float a, b, c; int steps, first, grow_first, grow_rest; double eps; };      // b, c: over a
 template <typename T, int LINES> __global__ __launch_bounds__(kThreads) void ortho_small(Small list, SmallPoly p)
 {
     __shared__ __attribute__((aligned(16))) char mats[3 * 16384];
@@ -936,44 +998,37 @@ template <typename T, int LINES> __global__ __launch_bounds__(kThreads) void ort
     }
     __syncthreads();
     Acc<64> acc;
-    int done = 0;
-    const int segs = (p.steps + p.seg_len - 1) / p.seg_len;
-    for (int seg = 0; seg < segs; ++seg) {
-        const int len = (p.steps - done + segs - seg - 1) / (segs - seg);
-        done += len;
-        char *A = mats, *P = mats + 16384, *Q = mats + 32768;
+    for (int done = 0; done < p.steps;) {
+        const bool two = done == 0 && p.first == 2 && p.steps > 1;      // the first segment; the rest goes step by step
+        char *A = mats, *B = mats + 16384, *R = B;
         small_rows(acc, X, X, xlines);
-        small_put<false>(to_tile_upper<64>(acc, scratch), A, ldexpf(1.0f, kExpA - 2 * (kExpX + up)), nullptr, 0.0f, 0.0f);
-        int qexp = kExpP;
-        for (int j = 0; j < len; ++j) {
+        small_put<false>(to_tile_upper<64>(acc, scratch), A, ldexpf(1.0f, kExpA - 2 * (kExpX + up)), nullptr, 0.0f);
+        small_rows(acc, A, A, klines);
+        small_put<true>(to_tile_upper<64>(acc, scratch), B, ldexpf(p.c, kExpB - 2 * kExpA), A, ldexpf(p.b, kExpB - kExpA));
+        if (two) {
+            small_rows(acc, A, B, klines);      // W = A + A B, in A's place
+            small_put<true>(to_tile_upper<64>(acc, scratch), A, ldexpf(1.0f, -kExpB), A, 1.0f);
+            small_rows(acc, A, B, klines);      // A' = a^2 (W + W B)
+            small_put<true>(to_tile_upper<64>(acc, scratch), A, p.a * p.a * ldexpf(1.0f, -kExpB), A, p.a * p.a);
+            B = mats + 32768;
             small_rows(acc, A, A, klines);
-            small_put<true>(to_tile_upper<64>(acc, scratch), P, ldexpf(p.c, kExpP - 2 * kExpA), A, ldexpf(p.a, kExpP), ldexpf(p.b, kExpP - kExpA));
-            if (j + 1 < len) {
-                small_rows(acc, A, P, klines);
-                small_put<false>(to_tile_upper<64>(acc, scratch), A, ldexpf(1.0f, -kExpP), nullptr, 0.0f, 0.0f);
-                small_rows(acc, A, P, klines);
-                small_put<false>(to_tile_upper<64>(acc, scratch), A, ldexpf(1.0f, -kExpP), nullptr, 0.0f, 0.0f);
-            }
-            if (j == 0) {      // Q is P; the next P takes the other place
-                char *other = Q;
-                Q = P;
-                P = other;
-            } else {
-                small_rows(acc, Q, P, klines);
-                small_put<false>(to_tile_upper<64>(acc, scratch), Q, ldexpf(1.0f, kExpQ - qexp - kExpP), nullptr, 0.0f, 0.0f);
-                qexp = kExpQ;
-            }
+            small_put<true>(to_tile_upper<64>(acc, scratch), B, ldexpf(p.c, kExpB - 2 * kExpA), A, ldexpf(p.b, kExpB - kExpA));
+            small_rows(acc, R, B, klines);      // R' = R + B + R B
+            small_put<true>(to_tile_upper<64>(acc, scratch), R, ldexpf(1.0f, -kExpB), R, 1.0f, B);
         }
+        done += two ? 2 : 1;
         const int e0 = kExpX + up;
-        up = up > 6 ? up - 6 : 0;
+        up -= two || done == 1 ? p.grow_first : p.grow_rest;
+        up = up > 0 ? up : 0;
+        const float q = two ? p.a * p.a : p.a;
         for (int x = 0; x < xlines; x += 2) {
-            small_cols(acc, Q, line_at(X, x), klines);
-            if (seg + 1 < segs) {
-                small_put<false>(to_tile<64, false>(acc, scratch), line_at(X, x), ldexpf(1.0f, kExpX + up - e0 - qexp), nullptr, 0.0f, 0.0f);
+            small_cols(acc, R, line_at(X, x), klines, (_Float16)(float)(1 << kExpB));
+            if (done < p.steps) {
+                small_put<false>(to_tile<64, false>(acc, scratch), line_at(X, x), ldexpf(q, kExpX + up - e0 - kExpB), nullptr, 0.0f);
                 continue;
             }
             const float *tile = M.tall ? to_tile<64, true>(acc, scratch) : to_tile<64, false>(acc, scratch);
-            const float out = ldexpf(1.0f, -(e0 + qexp));
+            const float out = ldexpf(q, -(e0 + kExpB));
             T *dst = reinterpret_cast<T *>(M.dst) + bi * M.dst_stride;
             const int c0 = x * 32;      // columns of X: rows of a tall result
             for (int q = threadIdx.x; q < 64 * 64; q += kThreads) {
@@ -983,7 +1038,7 @@ template <typename T, int LINES> __global__ __launch_bounds__(kThreads) void ort
         }
     }
 }
-constexpr int kSmallSide = 64, kSmallLong = 320;      // (10 lines of X: 148 KB of LDS with A, P, Q and the tile)
+constexpr int kSmallSide = 64, kSmallLong = 320;      // (10 lines of X: 148 KB of LDS with A, B, R and the tile)
 
 // ---- Adam for the vectors (the same arithmetic as tef_adam_clip_step, over a list of ranges of the flat buffers) --------------------
 constexpr int kRanges = 96;
@@ -1013,30 +1068,31 @@ __global__ __launch_bounds__(kThreads) void muon_vectors(Ranges rg, float *p, fl
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------------------
-struct Poly { float a, b, c; int steps; int seg_len; };
+struct Poly { double a, b, c; int steps, first, rest, grow_first, grow_rest; };      // steps of the first segment and of the following ones; the powers of two X grows by in them
 
 // The bounds that the fixed scales rely on, for singular values that start anywhere in [0, 1]: X and A stay below 2^2 (s < 4 would
-// square to 16: 2^12 * 16 = 65536 overflows fp16), P below 15, and Q of a segment below 60.
+// square to 16: 2^12 * 16 = 65536 overflows fp16), B and R below 15, and a segment's q below 2^6 (the exponents of X).
 bool bounded(Poly &p)
 {
-    double a = p.a, b = p.b, c = p.c;
-    if (!(isfinite(a) && isfinite(b) && isfinite(c))) return tef::fail("orthogonalisation: coefficients are not finite");
-    for (p.seg_len = kSegment; p.seg_len >= 1; --p.seg_len) {
-        bool ok = true;
-        for (int g = 0; g <= 512 && ok; ++g) {
-            double s = g / 512.0, q = 1.0;
-            for (int k = 0; k < p.steps && ok; ++k) {
-                const double l = s * s, poly = a + b * l + c * l * l;
-                if (k % p.seg_len == 0) q = 1.0;
-                q *= poly;
-                s *= poly;
-                if (!(fabs(poly) < 15.0 && fabs(s) < 3.9)) return tef::fail("orthogonalisation: these coefficients let a singular value grow past what the iteration can hold (|s| < 3.9, |p(s)/s| < 15)");
-                ok = fabs(q) < 60.0;
-            }
+    if (!(isfinite(p.a) && isfinite(p.b) && isfinite(p.c)) || fabs(p.a) < 1e-3) return tef::fail("orthogonalisation: the coefficients have to be finite, the first one not 0");
+    double first = 1.0, rest = 1.0;
+    for (int g = 0; g <= 512; ++g) {
+        double s = g / 512.0, q = 1.0, size = 1.0;
+        for (int k = 0, left = p.first; k < p.steps; ++k, --left) {
+            if (left == 0) { left = p.rest; q = size = 1.0; }
+            const double l = s * s, poly = 1.0 + (p.b * l + p.c * l * l) / p.a;
+            q *= poly;
+            size *= p.a;
+            s *= p.a * poly;
+            if (!(fabs(s) < 3.9 && fabs(poly - 1.0) < 15.0 && fabs(q - 1.0) < 15.0 && fabs(size) < 64.0 && fabs(size * q) < 64.0))
+                return tef::fail("orthogonalisation: these coefficients let the iteration grow past what it can hold (singular values below 3.9)");
+            double &most = k < p.first ? first : rest;
+            most = fabs(size * q) > most ? fabs(size * q) : most;
         }
-        if (ok) return true;
     }
-    return tef::fail("orthogonalisation: these coefficients grow too fast");
+    p.grow_first = (int)ceil(log2(first));
+    p.grow_rest = (int)ceil(log2(rest));
+    return true;
 }
 
 struct Cut { int whole, splits; long items, joins; };
@@ -1185,7 +1241,7 @@ int iterate(Group &g, const Poly &p, double eps, char *ws, const Step &st, hipSt
         hipLaunchKernelGGL((ortho_squares<T, STEP>), dim3((unsigned)(end - ch.m[0].first[PH_SQ])), block, 0, stream, ch, table, ws, st);
     }
     const Table t{table, g.n};
-    hipLaunchKernelGGL((ortho_pack<T, STEP>), dim3((unsigned)g.grid[PH_PACK]), block, 0, stream, t, ws, eps, st);
+    hipLaunchKernelGGL((ortho_pack<T, STEP>), dim3((unsigned)g.grid[PH_PACK]), block, 0, stream, t, ws, eps, p.grow_first, p.grow_rest, st);
     const dim3 apply((unsigned)g.grid[PH_APPLY]);
     auto symmetric = [&](Sym c, int products, int ts, const Cut &cut) {
         c.products = products;
@@ -1208,56 +1264,54 @@ int iterate(Group &g, const Poly &p, double eps, char *ws, const Step &st, hipSt
             TS_LAUNCH(ts, hipLaunchKernelGGL(ortho_join<128>, dim3((unsigned)cut.joins), block, 0, stream, t, ws, c),
                       hipLaunchKernelGGL(ortho_join<64>, dim3((unsigned)cut.joins), block, 0, stream, t, ws, c));
     };
-    // steps in segments of nearly equal length (5: 3 + 2)
-    const int segs = (p.steps + p.seg_len - 1) / p.seg_len;
-    int done = 0;
-    for (int s = 0; s < segs; ++s) {
-        const int len = (p.steps - done + segs - s - 1) / (segs - s);
-        done += len;
+    for (int s = 0, done = 0; done < p.steps; ++s) {
+        int len = s ? p.rest : p.first;
+        if (len > p.steps - done) len = p.steps - done;
         Sym x{};
         x.gram = 1; x.seg = s;
         x.l[0] = x.r[0] = s & 1 ? BUF_X1 : BUF_X0; x.out[0] = BUF_A;
         symmetric(x, 1, g.ts_gram, g.gram);
-        int q = -1;
+        int R = -1;
+        double q = 1.0;
         for (int k = 0; k < len; ++k) {
-            const int P = k & 1 ? BUF_P1 : BUF_P0;
-            // P = a I + b A + c A A
-            Sym c{};
-            c.l[0] = c.r[0] = BUF_A; c.out[0] = P; c.poly = 1;
-            c.mul[0] = ldexpf(p.c, kExpP - 2 * kExpA); c.pa = ldexpf(p.a, kExpP); c.pb = ldexpf(p.b, kExpP - kExpA);
+            const int B = k & 1 ? BUF_B1 : BUF_B0;
+            Sym c{};      // B = (b/a) A + (c/a) A A
+            c.l[0] = c.r[0] = BUF_A; c.out[0] = B; c.poly = 1;
+            c.mul[0] = (float)ldexp(p.c / p.a, kExpB - 2 * kExpA); c.plus = (float)ldexp(p.b / p.a, kExpB - kExpA);
             symmetric(c, 1, g.ts_chain, g.chain[0]);
-            // W = A P and Q' = Q P, then A' = W P
+            // W = A (I + B) and R' = R (I + B) + B
             Sym d{};
             int products = 0;
             if (k + 1 < len) {
-                d.l[products] = BUF_A; d.r[products] = P; d.out[products] = BUF_W; d.mul[products] = ldexpf(1.0f, kExpA - kExpA - kExpP);
-                ++products;
+                d.l[0] = BUF_A; d.r[0] = B; d.out[0] = BUF_W; d.mul[0] = ldexpf(1.0f, -kExpB); d.plus_l[0] = 1;
+                products = 1;
             }
             if (k > 0) {
-                const int out = q == BUF_Q0 ? BUF_Q1 : BUF_Q0;
-                d.l[products] = q; d.r[products] = P; d.out[products] = out;
-                d.mul[products] = ldexpf(1.0f, kExpQ - (q == BUF_Q0 || q == BUF_Q1 ? kExpQ : kExpP) - kExpP);
+                const int out = R == BUF_R0 ? BUF_R1 : BUF_R0;
+                d.l[products] = R; d.r[products] = B; d.out[products] = out; d.mul[products] = ldexpf(1.0f, -kExpB);
+                d.plus_l[products] = d.plus_r[products] = 1;
                 ++products;
-                q = out;
+                R = out;
             } else {
-                q = P;
+                R = B;
             }
             if (products) symmetric(d, products, g.ts_chain, g.chain[products - 1]);
             if (k + 1 < len) {
-                Sym e{};
-                e.l[0] = BUF_W; e.r[0] = P; e.out[0] = BUF_A; e.mul[0] = ldexpf(1.0f, kExpA - kExpA - kExpP);
+                Sym e{};      // A' = a^2 W (I + B)
+                e.l[0] = BUF_W; e.r[0] = B; e.out[0] = BUF_A; e.mul[0] = (float)ldexp(p.a * p.a, -kExpB); e.plus_l[0] = 1;
                 symmetric(e, 1, g.ts_chain, g.chain[0]);
             }
+            q *= p.a;
         }
-        const bool last = s + 1 == segs;
-        const int qexp = q == BUF_Q0 || q == BUF_Q1 ? kExpQ : kExpP;
-        if (!last) {
-            TS_LAUNCH(g.ts_apply, hipLaunchKernelGGL((ortho_apply<128, float, TO_X>), apply, block, 0, stream, t, ws, s, q, qexp, st),
-                      hipLaunchKernelGGL((ortho_apply<64, float, TO_X>), apply, block, 0, stream, t, ws, s, q, qexp, st));
+        done += len;
+        const float qf = (float)q;
+        if (done < p.steps) {
+            TS_LAUNCH(g.ts_apply, hipLaunchKernelGGL((ortho_apply<128, float, TO_X>), apply, block, 0, stream, t, ws, s, R, qf, st),
+                      hipLaunchKernelGGL((ortho_apply<64, float, TO_X>), apply, block, 0, stream, t, ws, s, R, qf, st));
         } else {
             constexpr int D = STEP ? TO_PARAM : TO_DST;
-            TS_LAUNCH(g.ts_apply, hipLaunchKernelGGL((ortho_apply<128, T, D>), apply, block, 0, stream, t, ws, s, q, qexp, st),
-                      hipLaunchKernelGGL((ortho_apply<64, T, D>), apply, block, 0, stream, t, ws, s, q, qexp, st));
+            TS_LAUNCH(g.ts_apply, hipLaunchKernelGGL((ortho_apply<128, T, D>), apply, block, 0, stream, t, ws, s, R, qf, st),
+                      hipLaunchKernelGGL((ortho_apply<64, T, D>), apply, block, 0, stream, t, ws, s, R, qf, st));
         }
     }
     return tef::check_launch("orthogonalisation");
@@ -1266,7 +1320,7 @@ int iterate(Group &g, const Poly &p, double eps, char *ws, const Step &st, hipSt
 // One workgroup a matrix when every matrix of the group is small enough: 26 us against 85 for a single 64 x 18 one.
 template <typename T> int small(const Group &g, const Poly &p, double eps, hipStream_t stream)
 {
-    const SmallPoly sp{p.a, p.b, p.c, p.steps, p.seg_len, eps};
+    const SmallPoly sp{(float)p.a, (float)(p.b / p.a), (float)(p.c / p.a), p.steps, p.first, p.grow_first, p.grow_rest, eps};
     for (int at = 0; at < g.n; at += kChunk) {
         Small list;
         list.n = g.n - at < kChunk ? g.n - at : kChunk;
@@ -1291,11 +1345,11 @@ bool all_small(const Group &g)
     return true;
 }
 
-bool polynomial(Poly &p, int steps, double a, double b, double c, double eps)
+bool polynomial(Poly &p, int steps, double a, double b, double c, double eps, int first, int rest)
 {
     if (steps < 1 || steps > kMaxSteps) return tef::fail("orthogonalisation: 1 to 32 steps");
     if (!(eps > 0.0 && eps < 1e30)) return tef::fail("orthogonalisation: eps must be positive");
-    p = Poly{(float)a, (float)b, (float)c, steps, kSegment};
+    p = Poly{a, b, c, steps, first, rest, 0, 0};
     return bounded(p);
 }
 
@@ -1353,7 +1407,7 @@ int tef_orthogonalize(const tef_ortho_matrix *matrices, int count, int dtype, in
                       void *workspace, size_t workspace_bytes, void *stream)
 {
     Poly p;
-    if (!polynomial(p, steps, a, b, c, eps)) return TEF_ERR_INVALID;
+    if (!polynomial(p, steps, a, b, c, eps, 2, 1)) return TEF_ERR_INVALID;
     if (dtype < TEF_F32 || dtype > TEF_BF16) return tef::fail("tef_orthogonalize: type"), TEF_ERR_INVALID;
     const size_t need = workspace_of(matrices, count);
     if (!need) return TEF_ERR_INVALID;
@@ -1388,7 +1442,7 @@ int tef_muon_step(float *p, float *g, float *m, float *v, const tef_muon_matrix 
                   double c, double eps, void *workspace, size_t workspace_bytes, void *stream)
 {
     Poly poly;
-    if (!polynomial(poly, steps, a, b, c, eps)) return TEF_ERR_INVALID;
+    if (!polynomial(poly, steps, a, b, c, eps, steps % 3 == 1 && steps > 1 ? 2 : 3, 3)) return TEF_ERR_INVALID;
     if (!p || !g || !m || !norm || !hp || !step || nvectors < 0 || (nvectors && (!vectors || !v)))
         return tef::fail("tef_muon_step: null pointer"), TEF_ERR_INVALID;
     long total = 0;

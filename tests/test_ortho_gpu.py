@@ -2,17 +2,17 @@
 
 Tolerance of the orthogonalisation.  The iteration amplifies any rounding of its matrices (a factor 3.4 a step along small singular
 values), by how much depends on the spectrum, so the bar is the error that the plain iteration X <- a X + (b A + c A A) X makes in
-fp32 ON THE SAME MATRIX, measured against 64 bits here: the kernels' operands carry 22 bits (half a step 2^-23) against fp32's 24, four
-times as much, and forming A from the previous A instead of from X doubles what reaches the result: 8 times the plain error.  On top of
-that stands what rounding costs where plain fp32 has nothing to amplify (a matrix of equal elements: one singular value 1, all rounding errors
-alike).  A segment of L steps is applied as X <- Q X, and Q = P_L .. P_1 reaches |q| = a^L = 41 (L = 3) on small singular
-values, so its diagonal is that large too.  In a row of Q X the elements' own roundings, 2^-23 relative, add up to at most 2^-23 sum_j |Q_ij x_j|
-<= 2^-23 2 |q| max|x| when the row is q on the diagonal and -q spread over the rest (the strong direction's share), and each of the L factors of
-Q brings the same again: 2^-23 times the sum over segments of 2 L |q|, relative to the largest element (five steps: 293 * 2^-23 = 3.5e-5).
-In that matrix the fp32 sums count as well, where other matrices' terms of both signs keep them small: a row of Q X, and of each factor of Q,
-is 3 m / 16 additions (the matrix instruction takes 16 products at a time, three plane pairs) to a running sum that reaches
-|q| max|x|, each off by 2^-24 of it: (L + 1) 3 m / 16 |q| 2^-24 a segment.  The bar for matrices of equal elements holds both terms.
-A result stored in 16 bits is off by half a step of its own on top."""
+fp32 ON THE SAME MATRIX, measured against 64 bits here, times 4: the kernels' operands carry 22 bits (half a step 2^-23) against fp32's 24
+(2^-25 when a value is stored, 2^-24 in every sum, which both sides share).  On top stands what rounding costs where plain fp32 has
+nothing to amplify: in each of five steps X, A and B are stored with half a step 2^-23 each, 15 of them, rounded up to 16,
+relative to the largest element.  In a matrix of equal elements all terms of a sum have one sign and all rows round alike: there the fp32 sums
+count in full, 2^-24 for each of the 3 n / 16 additions of an element of A (the matrix instruction takes 16 products at a time, three
+pairs of planes) and the 3 m / 16 of one of A A and one of B X, in each step, and p'(s) is at most 3.4 along the one direction.
+A result stored in 16 bits is off by half a step of its own on top.
+
+The optimiser takes three steps between Gram matrices (X' = q (X + R X), q up to a^3 = 41): a row of R is of the size of 1, its roundings
+bring q 2^-23 max|x| on each side of the diagonal, and each of the L factors of I + R the same again: 2^-23 times the sum over
+segments of 2 L |q|, and the recurrence for A doubles the plain error's factor of 4 to 8."""
 import math
 
 import pytest
@@ -23,16 +23,19 @@ pytestmark = pytest.mark.gpu
 ABC = (3.4445, -4.7750, 2.0315)
 
 
-def floor(steps, abc, m=0):
-    """2^-23 sum over the segments (three steps at most, of nearly equal length) of 2 L max|q|; m: with the sums over m products."""
+FLOOR = 16 * 2.0 ** -23
+
+
+def segments_floor(steps, abc):
+    """2^-23 sum over segments of three steps of 2 L max|q|."""
     a, b, c = abc
-    s, total, segments, done = torch.linspace(0, 1, 2001, dtype=torch.float64), 0.0, -(-steps // 3), 0
-    for k in range(segments):
-        length, q = -(-(steps - done) // (segments - k)), 1.0
+    s, total, done = torch.linspace(0, 1, 2001, dtype=torch.float64), 0.0, 0
+    while done < steps:
+        length, q = min(3, steps - done), 1.0
         for _ in range(length):
             p = a + b * s ** 2 + c * s ** 4
             q, s = q * p, s * p
-        total += (2 * length + (length + 1) * 3 * m / 16 / 2) * q.abs().max().item()
+        total += 2 * length * q.abs().max().item()
         done += length
     return total * 2.0 ** -23
 
@@ -68,7 +71,8 @@ def check(got, u, steps=5, abc=ABC, eps=1e-7, equal=False):
     T = torch.finfo(u.dtype).eps / 2 if u.dtype != torch.float32 else 0.0
     tiny = T * torch.finfo(u.dtype).smallest_normal
     err = (got.detach().double().cpu() - want).abs() - T * want.abs() - tiny
-    assert err.max().item() <= 8 * plain + floor(steps, abc, min(u.shape) if equal else 0) * top, (tuple(u.shape), err.max().item() / max(top, 1e-300), plain / max(top, 1e-300))
+    sums = steps * 3.4 * (3 * max(u.shape) + 6 * min(u.shape)) / 16 * 2.0 ** -24 if equal else 0.0
+    assert err.max().item() <= 4 * plain + (FLOOR + sums) * top, (tuple(u.shape), err.max().item() / max(top, 1e-300), plain / max(top, 1e-300))
 
 
 def matrix(kind, rows, cols, seed=0):
@@ -260,7 +264,7 @@ def muon_reference(params, moments, squares, grads, t, k, vectors=()):
             rows, cols = u.shape
             scale = math.sqrt(max(1, rows / cols)) if k["adjust_lr"] == "original" else 0.2 * math.sqrt(max(rows, cols))
             p.mul_(1 - k["lr"] * k["weight_decay"]).sub_(k["lr"] * scale * o.view(p.shape))
-            bars.append(k["lr"] * scale * (8 * plain + (floor(5, ABC) + 2e-6) * o.abs().max().item()))      # u itself: a few roundings of fp32
+            bars.append(k["lr"] * scale * (8 * plain + (segments_floor(5, ABC) + 2e-6) * o.abs().max().item()))      # u itself: a few roundings of fp32
         else:
             v = squares[i]
             m.add_(0.1 * (g - m))
