@@ -868,12 +868,14 @@ template <int TS, typename T, int DEST> __global__ __launch_bounds__(kThreads, 2
 // size.  X <- q (I + R) X goes to X's own place (a tile's values are in registers when its columns have been read), and so does every
 // other product to one of its operands'.
 __device__ inline char *line_at(char *m, int line) { return m + line * (64 * 128); }
-// acc = L R^T over `lines` lines (this wave's 32 x 32 block)
+// acc = L R^T over `lines` lines (this wave's 32 x 32 block); hi lo and lo hi have a sum of their own, 2^-11 of the other's size: a third of
+// the additions round at the size of the result
 __device__ inline void small_rows(Acc<64> &acc, const char *L, const char *R, int lines)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = (wave >> 1) * 32, wj = (wave & 1) * 32;
+    float16v cross;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) acc.v[0][0][e] = 0.0f;
+    for (int e = 0; e < 16; ++e) acc.v[0][0][e] = cross[e] = 0.0f;
     for (int l = 0; l < lines; ++l)
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
@@ -884,16 +886,20 @@ __device__ inline void small_rows(Acc<64> &acc, const char *L, const char *R, in
                 b[pl] = frag_rows(R + l * 8192, wj + (lane & 31), s, pl);
             }
 #pragma unroll
-            for (int t = 0; t < 3; ++t) acc.v[0][0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[t == 0], b[t == 1], acc.v[0][0], 0, 0, 0);
+            for (int t = 0; t < 2; ++t) cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[t == 0], b[t == 1], cross, 0, 0, 0);
+            acc.v[0][0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], b[0], acc.v[0][0], 0, 0, 0);
         }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc.v[0][0][e] += cross[e];
 }
 // acc = (B + one I) X over `lines` lines of B, for the two lines of X from `X` on (64 columns; X's rows are k)
 __device__ inline void small_cols(Acc<64> &acc, const char *B, const char *X, int lines, _Float16 one)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = (wave >> 1) * 32, g = lane >> 4, src = lane & 15;
     const char *x = X + (wave & 1) * 8192;
+    float16v cross;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) acc.v[0][0][e] = 0.0f;
+    for (int e = 0; e < 16; ++e) acc.v[0][0][e] = cross[e] = 0.0f;
     for (int l = 0; l < lines; ++l)
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
@@ -911,11 +917,14 @@ __device__ inline void small_cols(Acc<64> &acc, const char *B, const char *X, in
                 }
             }
 #pragma unroll
-            for (int t = 0; t < 3; ++t) acc.v[0][0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[t == 0], b[t == 1], acc.v[0][0], 0, 0, 0);
+            for (int t = 0; t < 2; ++t) cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[t == 0], b[t == 1], cross, 0, 0, 0);
+            acc.v[0][0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], b[0], acc.v[0][0], 0, 0, 0);
             if (l * 32 == wi)
 #pragma unroll
                 for (int pl = 0; pl < 2; ++pl) acc.v[0][0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(identity(s, one), b[pl], acc.v[0][0], 0, 0, 0);
         }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc.v[0][0][e] += cross[e];
 }
 __device__ inline char *small_at(char *m, int row, int col, int plane)      // 16 bytes: eight columns from `col` on
 {
