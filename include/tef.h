@@ -566,8 +566,8 @@ int tef_layer_norm_backward(const tef_norm_desc *d, const void *x, const void *w
  * row's elements contiguous) X = U / max(|U|_F, eps), then `steps` times X <- a X + (b A + c A A) X with A = X X^T (X^T X for tall
  * ones: same result), written to dst (which may be src).  All matrices of a call go through the same launches.
  * src and dst have type `dtype` (TEF_F32 / F16 / BF16) and the alignment of their elements; the arithmetic is fp32-grade
- * whatever the type.  1 <= steps <= 32; coefficients under which a singular value in [0, 1] would leave |s| < 3.9 are
- * refused.  The matrix list is read during the call only.  Workspace: 256-byte aligned, the caller's, of the size asked for with the same
+ * whatever the type.  1 <= steps <= 32, 1e-200 <= eps < 1e30; a first coefficient of 0 and coefficients under which a singular value in
+ * [0, 1] would leave |s| < 3.9 are refused.  The matrix list is read during the call only.  Workspace: 256-byte aligned, the caller's, of the size asked for with the same
  * list; two calls that may run at once need two. */
 typedef struct tef_ortho_matrix {
     const void *src;

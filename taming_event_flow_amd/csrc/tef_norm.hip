@@ -651,7 +651,16 @@ void launch(const tef_norm_desc &d, const Plan &p, bool bwd, unsigned blocks, hi
     else go<__hip_bfloat16>(p, bwd, grid, st, a);
 }
 
-unsigned bwd_blocks(const Plan &p) { return (unsigned)(p.tiles < kMaxBlocks ? p.tiles : kMaxBlocks); }
+// (rows too long for the registers: fewer workgroups, since each has a partial row of that length in the workspace)
+unsigned bwd_blocks(const Plan &p, int channels)
+{
+    long most = kMaxBlocks;
+    if (p.kind == 3) {
+        most = (1l << 23) / channels;
+        most = most < 64 ? 64 : most > kMaxBlocks ? kMaxBlocks : most;
+    }
+    return (unsigned)(p.tiles < most ? p.tiles : most);
+}
 
 bool valid(const tef_norm_desc *d)
 {
@@ -689,7 +698,7 @@ size_t tef_layer_norm_workspace_bytes(const tef_norm_desc *d)
 {
     if (!valid(d)) return 0;
     if (d->outer == 0) return 16;
-    return (size_t)bwd_blocks(make_plan(*d)) * 2 * (size_t)d->channels * sizeof(float);
+    return (size_t)bwd_blocks(make_plan(*d), d->channels) * 2 * (size_t)d->channels * sizeof(float);
 }
 
 int tef_layer_norm_backward(const tef_norm_desc *d, const void *x, const void *weight, const void *bias, const void *residual,
@@ -715,7 +724,7 @@ int tef_layer_norm_backward(const tef_norm_desc *d, const void *x, const void *w
     a.part = sums ? (float *)workspace : nullptr;
     a.v = Vecs{weight, bias, d->wdtype};
     a.rows = (long)d->outer * d->inner; a.inner = d->inner; a.C = d->channels; a.act = d->act; a.eps = d->eps;
-    const unsigned blocks = bwd_blocks(p);
+    const unsigned blocks = bwd_blocks(p, d->channels);
     launch(*d, p, true, blocks, st, a);
     if (sums)
         hipLaunchKernelGGL(norm_join, dim3((unsigned)((2l * d->channels + 63) / 64)), dim3(64 * kJoinWaves), 0, st, (const float *)workspace, (int)blocks,

@@ -1357,7 +1357,7 @@ bool all_small(const Group &g)
 bool polynomial(Poly &p, int steps, double a, double b, double c, double eps, int first, int rest)
 {
     if (steps < 1 || steps > kMaxSteps) return tef::fail("orthogonalisation: 1 to 32 steps");
-    if (!(eps > 0.0 && eps < 1e30)) return tef::fail("orthogonalisation: eps must be positive");
+    if (!(eps >= 1e-200 && eps < 1e30)) return tef::fail("orthogonalisation: eps must be positive (1e-200 at least: 1 / eps is formed)");
     p = Poly{a, b, c, steps, first, rest, 0, 0};
     return bounded(p);
 }
@@ -1394,14 +1394,15 @@ bool group_of(Group &g, const tef_muon_matrix *m, int at, int count)
     return true;
 }
 
-template <typename D> size_t workspace_of(const D *m, int count)
+// (one workgroup a matrix needs none; the optimiser's step does not go that way)
+template <typename D> size_t workspace_of(const D *m, int count, bool small_ones)
 {
     if (count < 0 || (count && !m)) return tef::fail("orthogonalisation: null matrix list"), 0;
     size_t most = 256;
     Group g;
     for (int at = 0; at < count; at += kGroup) {
         if (!group_of(g, m, at, count)) return 0;
-        if ((size_t)g.bytes > most) most = (size_t)g.bytes;
+        if (!(small_ones && all_small(g)) && (size_t)g.bytes > most) most = (size_t)g.bytes;
     }
     return most;
 }
@@ -1410,7 +1411,7 @@ template <typename D> size_t workspace_of(const D *m, int count)
 
 extern "C" {
 
-size_t tef_orthogonalize_workspace_bytes(const tef_ortho_matrix *matrices, int count) { return workspace_of(matrices, count); }
+size_t tef_orthogonalize_workspace_bytes(const tef_ortho_matrix *matrices, int count) { return workspace_of(matrices, count, true); }
 
 int tef_orthogonalize(const tef_ortho_matrix *matrices, int count, int dtype, int steps, double a, double b, double c, double eps,
                       void *workspace, size_t workspace_bytes, void *stream)
@@ -1418,7 +1419,7 @@ int tef_orthogonalize(const tef_ortho_matrix *matrices, int count, int dtype, in
     Poly p;
     if (!polynomial(p, steps, a, b, c, eps, 2, 1)) return TEF_ERR_INVALID;
     if (dtype < TEF_F32 || dtype > TEF_BF16) return tef::fail("tef_orthogonalize: type"), TEF_ERR_INVALID;
-    const size_t need = workspace_of(matrices, count);
+    const size_t need = workspace_of(matrices, count, true);
     if (!need) return TEF_ERR_INVALID;
     if (count == 0) return 0;
     for (int k = 0; k < count; ++k)
@@ -1444,7 +1445,7 @@ int tef_orthogonalize(const tef_ortho_matrix *matrices, int count, int dtype, in
     return 0;
 }
 
-size_t tef_muon_workspace_bytes(const tef_muon_matrix *matrices, int count) { return workspace_of(matrices, count); }
+size_t tef_muon_workspace_bytes(const tef_muon_matrix *matrices, int count) { return workspace_of(matrices, count, false); }
 
 int tef_muon_step(float *p, float *g, float *m, float *v, const tef_muon_matrix *matrices, int nmatrices, const tef_muon_vector *vectors,
                   int nvectors, const float *norm, const double *hp, const float *step, int nesterov, int steps, double a, double b,
@@ -1460,7 +1461,7 @@ int tef_muon_step(float *p, float *g, float *m, float *v, const tef_muon_matrix 
         total += vectors[k].size;
     }
     if (total > 0x3fffffff) return tef::fail("tef_muon_step: more than 2^30 vector elements"), TEF_ERR_INVALID;
-    const size_t need = workspace_of(matrices, nmatrices);
+    const size_t need = workspace_of(matrices, nmatrices, false);
     if (!need) return TEF_ERR_INVALID;
     if (nmatrices && (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < need))
         return tef::fail("tef_muon_step: workspace too small or not 256-byte aligned"), TEF_ERR_WORKSPACE;

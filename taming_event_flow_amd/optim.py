@@ -33,8 +33,8 @@ def _polynomial(steps, coefficients, eps):
         raise ValueError(f"steps = {steps}: 1 to 32")
     if len(coefficients) != 3 or not all(math.isfinite(c) for c in coefficients):
         raise ValueError(f"coefficients = {coefficients!r}: three finite numbers")
-    if not (math.isfinite(eps) and 0.0 < eps < 1e30):
-        raise ValueError(f"eps = {eps}: positive")
+    if not 1e-200 <= eps < 1e30:
+        raise ValueError(f"eps = {eps}: positive (at least 1e-200)")
     return (int(steps),) + tuple(float(c) for c in coefficients) + (float(eps),)
 
 
@@ -120,6 +120,7 @@ class FusedMuon(FusedAdam):
         if bucket.flat.dtype != torch.float32:
             raise TypeError(f"FusedMuon: float32 parameters (got {bucket.flat.dtype})")
         self._poly = _polynomial(steps, coefficients, eps)
+        _lib.require_device_tensor(bucket.flat, "FusedMuon gradient bucket")
         self.nesterov = bool(nesterov)
         super().__init__(bucket, lr, betas=betas, eps=adam_eps)
         self.param_groups[0].update(momentum=float(momentum), weight_decay=float(weight_decay), adam_lr=None if adam_lr is None else float(adam_lr))
@@ -166,6 +167,11 @@ class FusedMuon(FusedAdam):
         for k, v in sd["param_groups"][0].items():
             if k != "params":
                 self.param_groups[0][k] = tuple(v) if k == "betas" else v
+
+    def step(self, max_norm=None):
+        """One step on the (already reduced) flat gradient, see FusedAdam.step: clip to `max_norm`, update, clear -> the norm before clipping."""
+        with torch.cuda.device_of(self.flat_p):
+            return super().step(max_norm)
 
     def _update(self, stream):
         code = self._lib.lib().tef_muon_step(self.flat_p.data_ptr(), self.bucket.flat.data_ptr(), self.m.data_ptr(), self.v.data_ptr(),

@@ -43,6 +43,8 @@ def test_optimiser_refusals(lib_):
                dict(coefficients=(9.0, 0.0, 0.0, 1.0)), dict(eps=0.0)):
         with pytest.raises(ValueError):
             optim.FusedMuon(bucket, **dict(dict(lr=0.1), **kw))
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        optim.FusedMuon(bucket, 0.1)
     with pytest.raises(TypeError):
         optim.FusedMuon(parallel.FlatGradBucket([torch.nn.Parameter(torch.zeros(4, 6).double())]), 0.1)
 
@@ -68,7 +70,7 @@ def test_c_refusals(lib_):
         assert call(mats(**kw)) == -1, kw
     assert call(mats(src=None)) == -1 and call(mats(dst=None)) == -1
     assert call(n=-1) == -1 and call(dtype=3) == -1 and call(dtype=-1) == -1
-    assert call(steps=0) == -1 and call(steps=33) == -1 and call(eps=0.0) == -1 and call(eps=float("nan")) == -1
+    assert call(steps=0) == -1 and call(steps=33) == -1 and call(eps=0.0) == -1 and call(eps=1e-300) == -1 and call(eps=float("nan")) == -1
     for abc in ((float("nan"), 0, 0), (16.0, 0, 0), (4.0, 0.0, 0.0), (0.0, 0.0, 5.0), (-20.0, 0.0, 0.0)):
         assert call(abc=abc) == -1, abc
         assert b"coefficients" in lib.tef_last_error()
@@ -91,8 +93,10 @@ def test_c_refusals(lib_):
 def test_workspace_of_many_matrices(lib_):
     """The list is worked through in groups: the workspace is the largest group's, not the sum."""
     lib = lib_.lib()
-    one = lib_.OrthoMatrix(1, 1, 64, 64, 64, 64, 1, 0, 0)
+    one = lib_.OrthoMatrix(1, 1, 80, 80, 80, 80, 1, 0, 0)
     size = lambda n: lib.tef_orthogonalize_workspace_bytes((lib_.OrthoMatrix * n)(*[one] * n), n)  # noqa: E731
     assert size(1) < size(64) == size(128) == size(1000)
     big = lib_.OrthoMatrix(1, 1, 2 ** 15, 2 ** 17, 2 ** 17, 2 ** 17, 1, 0, 0)
     assert lib.tef_orthogonalize_workspace_bytes((lib_.OrthoMatrix * 1)(big), 1) > 2 * 4 * 2 ** 32      # 64-bit sizes
+    small = lib_.OrthoMatrix(1, 1, 64, 320, 320, 320, 1 << 20, 0, 0)      # one workgroup each: nothing in memory
+    assert lib.tef_orthogonalize_workspace_bytes((lib_.OrthoMatrix * 1)(small), 1) == 256

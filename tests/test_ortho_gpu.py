@@ -149,10 +149,11 @@ def test_scales(dev, size):
         check(orthogonalize(u, eps=1e-3), u, eps=1e-3)
 
 
-def test_zero_nan_inf_stay_in_their_matrix(dev):
+@pytest.mark.parametrize("shape", [(40, 60), (70, 400), (400, 70), (300, 300)])
+def test_zero_nan_inf_stay_in_their_matrix(dev, shape):
     from taming_event_flow_amd.optim import orthogonalize
 
-    u = matrix("normal", 40, 60).float().to(dev).repeat(5, 1, 1)
+    u = matrix("normal", *shape).float().to(dev).repeat(5, 1, 1)
     clean = orthogonalize(u)
     u[1] = 0
     u[2, 3, 4], u[3, 0, 59] = float("nan"), float("-inf")
@@ -306,6 +307,39 @@ def test_muon_steps(dev, kw):
             got = opt.m[at:at + m.numel()].double().cpu().view(m.shape)
             assert (got - m).abs().max() <= t * 4 * 2.0 ** -23 * max(m.abs().max().item(), 0.04)
             at += m.numel()
+
+
+def test_muon_many_parameters(dev):
+    """More matrices and vectors than one set of launches takes."""
+    from taming_event_flow_amd import optim, parallel
+
+    gen = torch.Generator().manual_seed(2)
+    shapes = [(6, 10)] * 70 + [(80, 90)] * 3 + [(5,)] * 110
+    start = [torch.randn(s, generator=gen) * 0.1 for s in shapes]
+    params = [torch.nn.Parameter(p.clone().to(dev)) for p in start]
+    bucket = parallel.FlatGradBucket(params)
+    opt = optim.FusedMuon(bucket, 0.02, adam_lr=1e-3)
+    grads = [torch.randn(s, generator=gen) * 0.01 for s in shapes]
+    for p, g in zip(params, grads):
+        p.grad.copy_(g)
+    opt.step()
+    p64 = [p.double() for p in start]
+    k = dict(lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, adjust_lr="original", adam_lr=1e-3, max_norm=None)
+    _, bars = muon_reference(p64, [torch.zeros_like(p) for p in p64], [torch.zeros_like(p) for p in p64], [g.double() for g in grads], 1, k)
+    for p, q, bar in zip(params, p64, bars):
+        assert (p.detach().double().cpu() - q).abs().max() <= bar + 2.0 ** -23 * q.abs().max()
+
+
+@pytest.mark.parametrize("shapes", [[(4, 5), (7, 3)], [(4,), (9,)]])
+def test_muon_without_vectors_or_matrices(dev, shapes):
+    from taming_event_flow_amd import optim, parallel
+
+    params = [torch.nn.Parameter(torch.ones(s, device=dev)) for s in shapes]
+    bucket = parallel.FlatGradBucket(params)
+    opt = optim.FusedMuon(bucket, 0.02)
+    bucket.flat.fill_(0.1)
+    opt.step()
+    assert torch.isfinite(opt.flat_p).all() and (opt.flat_p < 1).all() and not bucket.flat.any()
 
 
 def test_muon_state_dict_and_param_views(dev):
