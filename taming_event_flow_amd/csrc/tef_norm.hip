@@ -118,7 +118,8 @@ struct Args {
 // ---- rows: C contiguous --------------------------------------------------------------------------------------------------
 // A row belongs to L lanes (a power of two, at most one wave: no barrier, several short rows a wave) or, WG, to the whole
 // workgroup.  Lane l holds the elements V * (l + L * i) .. + V - 1, i < NV, in registers, and keeps the weights of its
-// columns over all rows that it takes.
+// columns over all rows that it takes.  4096 x 4096 bf16: 29 us forward, 42 backward (2.3, 2.4 TB/s; one row a workgroup at a time,
+// two joins of its waves each: latency, hidden by eight workgroups a CU).
 constexpr int V = 4;
 
 template <bool WG> __device__ inline float row_sum(float s, int L, float *red)
@@ -278,6 +279,7 @@ template <typename T, int NV, bool WG, bool EVEN> __global__ __launch_bounds__(k
 // ---- maps: the channels of a position lie `inner` elements apart --------------------------------------------------------
 // A workgroup takes LX * P neighbouring positions (P per lane: 4 when inner is a multiple of 4, so that a lane's positions
 // are one load; else 1) and all channels: lane group g of G = 256 / LX holds the channels g, g + G, ... in registers.
+// 80 x 32 x 128 x 128 f32 with tanh: 84 us forward, 110 backward (4.0, 4.6 TB/s of a copy's 4.9).
 template <int P> __device__ inline void map_sum(float (&s)[P], int LX, float *red)      // over the lane groups
 {
     const int lx = threadIdx.x & (LX - 1), wave = threadIdx.x >> 6;

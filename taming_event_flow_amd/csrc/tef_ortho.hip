@@ -169,6 +169,7 @@ __device__ inline float clip_scale(const float *norm, double max_norm)
 }
 
 // ---- phase 0: sums of squares (double: no overflow or underflow of a square for any fp32 input) -----------------------------
+// Bound by memory: 31 million parameters, momentum updated on the way (g, m read, m written), 65 us = 5.8 TB/s.
 struct Chunk { Mat m[kChunk]; int n, at; };
 
 template <typename T, bool STEP> __global__ __launch_bounds__(kThreads) void ortho_squares(Chunk ch, Mat *table, char *ws, Step st)
@@ -231,7 +232,8 @@ template <typename T, bool STEP> __global__ __launch_bounds__(kThreads) void ort
 }
 
 // ---- phase 1: normalise and split ---------------------------------------------------------------------------------------------
-// A workgroup writes 32 rows x 64 columns of the padded X (8 values a thread).  The scale is kExpX plus, where |U| < eps leaves
+// A workgroup writes 32 rows x 64 columns of the padded X (8 values a thread); bound by memory: g, m read, X written and g cleared for 31
+// million parameters in 100 us = 5 TB/s.  The scale is kExpX plus, where |U| < eps leaves
 // X small, the power of two that brings it back up: what is multiplied later always has 22 good bits.
 template <typename T, bool STEP> __global__ __launch_bounds__(kThreads) void ortho_pack(Table t, char *ws, double eps, int grow_first, int grow_rest, Step st)
 {
@@ -320,6 +322,11 @@ template <typename T, bool STEP> __global__ __launch_bounds__(kThreads) void ort
 // by one line of 32 a stage, from global memory through registers (AHEAD stages in flight) into LDS while the previous stage is
 // multiplied: two buffers, one barrier a stage.  The 16-byte chunks of a row are permuted by the row, chunk ^ (row / 2 & 7):
 // sixteen lanes that read the same chunk of sixteen neighbouring rows (128 bytes each) meet all 64 banks once.
+//
+// What bounds them: large tiles (128) the way from L2 into the CU, 32 KB a line and workgroup, at 8 to 11 TB/s over the chip — 1.0 to 1.05
+// PFLOP/s of fp16 products on 4096 x 4096, the matrix pipes 0.56 of the time busy; deeper prefetch, priorities and other instruction orders change
+// nothing.  Small ones (64: 32 KB for a quarter of the work) the same on many CUs, latency on few.  A line's three plane products
+// share its loads, which is why a line of 128 x 128 costs two thirds of the traffic per product that plain fp16 operands would.
 template <int TS> struct Geo {
     static constexpr int FR = TS / 64;                       // 32 x 32 blocks of a wave along each side
     static constexpr int STAGE = TS * 128;                   // bytes of an operand's stage
@@ -718,7 +725,8 @@ template <int TS> __global__ __launch_bounds__(kThreads) void ortho_join(Table t
     finish<TS>(acc, lds, M, ws + M.ws + p.bi * M.area, c, p);
 }
 
-// The same for m x m products of few and short tiles, where a launch is latency: 32 x 32 tiles, k dealt line by line to the four waves,
+// The same for m x m products of few and short tiles, where a launch is latency (385 x 385: 8.4 us with 64 x 64 tiles, 6.9 with these; past some
+// 500 tiles the operands' re-reading costs more: 27 us against 15 for nine matrices of 512): 32 x 32 tiles, k dealt line by line to the four waves,
 // fragments straight from memory (no LDS, no barrier; four lines of a wave in flight), the waves' sums joined in order in LDS.
 __global__ __launch_bounds__(kThreads) void ortho_symmetric32(Table t, char *ws, Sym c)
 {
@@ -802,6 +810,8 @@ __global__ __launch_bounds__(kThreads) void ortho_symmetric32(Table t, char *ws,
 }
 
 // ---- phase 4: X' = q (I + R) X, into the other X, the caller's matrix, or the parameters -------------------------------------------------
+// 4096 x 4096: 410 us = 1.0 PFLOP/s of fp16 products; the default network's matrices: 141 us into X, 168 into the parameters (0.6 PFLOP/s, 16
+// lines a tile: a third of the time is the tile's way out).
 enum { TO_X = 0, TO_DST, TO_PARAM };
 template <int TS, typename T, int DEST> __global__ __launch_bounds__(kThreads, 2) void ortho_apply(Table t, char *ws, int seg, int r_buf, float q, Step st)
 {
