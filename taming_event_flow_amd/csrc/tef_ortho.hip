@@ -1226,7 +1226,8 @@ void plan(Group &g)
         if (g.gram.joins) g.gram.joins = first[PH_JOIN];
         for (int w = 0; w < 2; ++w) g.chain[w] = Cut{0, 1, first[PH_CHAIN] * (w + 1), 0};
     }
-    for (int f = 0; f < PHASES; ++f) g.grid[f] = first[f] > 0x3fffffff ? -1 : (int)first[f];
+    // (a launch holds less than 2^32 threads: 2^24 workgroups of 256, and a launch of two products has twice the items)
+    for (int f = 0; f < PHASES; ++f) g.grid[f] = first[f] > 0x7fffff ? -1 : (int)first[f];
     g.bytes = at;
 }
 
@@ -1340,15 +1341,15 @@ int iterate(Group &g, const Poly &p, double eps, char *ws, const Step &st, hipSt
 template <typename T> int small(const Group &g, const Poly &p, double eps, hipStream_t stream)
 {
     const SmallPoly sp{(float)p.a, (float)(p.b / p.a), (float)(p.c / p.a), p.steps, p.first, p.grow_first, p.grow_rest, eps};
-    for (int at = 0; at < g.n; at += kChunk) {
+    for (int at = 0; at < g.n;) {
         Small list;
-        list.n = g.n - at < kChunk ? g.n - at : kChunk;
         int items = 0, longest = 0;
-        for (int k = 0; k < list.n; ++k) {
-            list.m[k] = g.m[at + k];
-            list.first[k] = items;
-            items += g.m[at + k].batch;
-            longest = longest > g.m[at + k].n ? longest : g.m[at + k].n;
+        // (batches hold up to 2^20 matrices, a launch up to 2^24 workgroups)
+        for (list.n = 0; list.n < kChunk && at < g.n && items <= 0x700000; ++list.n, ++at) {
+            list.m[list.n] = g.m[at];
+            list.first[list.n] = items;
+            items += g.m[at].batch;
+            longest = longest > g.m[at].n ? longest : g.m[at].n;
         }
         const dim3 grid((unsigned)items), block(kThreads);
         if (longest <= 64) hipLaunchKernelGGL((ortho_small<T, 2>), grid, block, 0, stream, list, sp);
