@@ -940,27 +940,23 @@ __device__ inline char *small_at(char *m, int row, int col, int plane)      // 1
 {
     return line_at(m, col >> 5) + row * 128 + (((plane * 4 + ((col & 31) >> 3)) ^ (row >> 1 & 7)) << 4);
 }
-// mul times the 64 x 64 values of the tile, PLUS: plus * A (+ B), to the split matrix `out` (two lines; A's own place too: a thread
-// writes the values that it has read)
-template <bool PLUS> __device__ inline void small_put(const float *tile, char *out, float mul, char *A, float plus, char *B = nullptr)
+// mul times the 64 x 64 values of the tile, plus (ADD 1) plus * A, plus (ADD 2) B too — this thread's 16 values of them as they were
+// before they were split: B's linear term would otherwise carry A's rounding, the largest one in small matrices — to the split matrix
+// `out` of two lines and, unsplit, back
+struct Kept { float v[16]; };
+template <int ADD> __device__ inline Kept small_put(const float *tile, char *out, float mul, const Kept &A, float plus, const Kept &B)
 {
+    Kept kept;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int q = threadIdx.x + i * kThreads, r = q >> 3, c = (q & 7) * 8;
-        half8 hi, lo, bhi, blo;
-        if (PLUS) {
-            hi = *reinterpret_cast<const half8 *>(small_at(A, r, c, 0));
-            lo = *reinterpret_cast<const half8 *>(small_at(A, r, c, 1));
-            if (B) {
-                bhi = *reinterpret_cast<const half8 *>(small_at(B, r, c, 0));
-                blo = *reinterpret_cast<const half8 *>(small_at(B, r, c, 1));
-            }
-        }
+        half8 hi, lo;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             float f = mul * tile[r * Geo<64>::PITCH + c + k];
-            if (PLUS) f += plus * ((float)hi[k] + (float)lo[k]);
-            if (PLUS && B) f += (float)bhi[k] + (float)blo[k];
+            if (ADD > 0) f += plus * A.v[i * 8 + k];
+            if (ADD > 1) f += B.v[i * 8 + k];
+            kept.v[i * 8 + k] = f;
             _Float16 h, l;
             split(f, h, l);
             hi[k] = h;
@@ -970,6 +966,7 @@ template <bool PLUS> __device__ inline void small_put(const float *tile, char *o
         *reinterpret_cast<half8 *>(small_at(out, r, c, 1)) = lo;
     }
     __syncthreads();
+    return kept;
 }
 
 struct Small { Mat m[kChunk]; int first[kChunk]; int n; };
@@ -1020,20 +1017,22 @@ template <typename T, int LINES> __global__ __launch_bounds__(kThreads) void ort
     for (int done = 0; done < p.steps;) {
         const bool two = done == 0 && p.first == 2 && p.steps > 1;      // the first segment; the rest goes step by step
         char *A = mats, *B = mats + 16384, *R = B;
+        const float b1 = ldexpf(p.b, kExpB - kExpA), c1 = ldexpf(p.c, kExpB - 2 * kExpA), unit = ldexpf(1.0f, -kExpB);
+        const Kept none{};
         small_rows(acc, X, X, xlines);
-        small_put<false>(to_tile_upper<64>(acc, scratch), A, ldexpf(1.0f, kExpA - 2 * (kExpX + up)), nullptr, 0.0f);
+        Kept a = small_put<0>(to_tile_upper<64>(acc, scratch), A, ldexpf(1.0f, kExpA - 2 * (kExpX + up)), none, 0.0f, none);
         small_rows(acc, A, A, klines);
-        small_put<true>(to_tile_upper<64>(acc, scratch), B, ldexpf(p.c, kExpB - 2 * kExpA), A, ldexpf(p.b, kExpB - kExpA));
+        const Kept b = small_put<1>(to_tile_upper<64>(acc, scratch), B, c1, a, b1, none);
         if (two) {
             small_rows(acc, A, B, klines);      // W = A + A B, in A's place
-            small_put<true>(to_tile_upper<64>(acc, scratch), A, ldexpf(1.0f, -kExpB), A, 1.0f);
+            a = small_put<1>(to_tile_upper<64>(acc, scratch), A, unit, a, 1.0f, none);
             small_rows(acc, A, B, klines);      // A' = a^2 (W + W B)
-            small_put<true>(to_tile_upper<64>(acc, scratch), A, p.a * p.a * ldexpf(1.0f, -kExpB), A, p.a * p.a);
+            a = small_put<1>(to_tile_upper<64>(acc, scratch), A, p.a * p.a * unit, a, p.a * p.a, none);
             B = mats + 32768;
             small_rows(acc, A, A, klines);
-            small_put<true>(to_tile_upper<64>(acc, scratch), B, ldexpf(p.c, kExpB - 2 * kExpA), A, ldexpf(p.b, kExpB - kExpA));
+            const Kept b2 = small_put<1>(to_tile_upper<64>(acc, scratch), B, c1, a, b1, none);
             small_rows(acc, R, B, klines);      // R' = R + B + R B
-            small_put<true>(to_tile_upper<64>(acc, scratch), R, ldexpf(1.0f, -kExpB), R, 1.0f, B);
+            small_put<2>(to_tile_upper<64>(acc, scratch), R, unit, b, 1.0f, b2);
         }
         done += two ? 2 : 1;
         const int e0 = kExpX + up;
@@ -1043,7 +1042,7 @@ template <typename T, int LINES> __global__ __launch_bounds__(kThreads) void ort
         for (int x = 0; x < xlines; x += 2) {
             small_cols(acc, R, line_at(X, x), klines, (_Float16)(float)(1 << kExpB));
             if (done < p.steps) {
-                small_put<false>(to_tile<64, false>(acc, scratch), line_at(X, x), ldexpf(q, kExpX + up - e0 - kExpB), nullptr, 0.0f);
+                small_put<0>(to_tile<64, false>(acc, scratch), line_at(X, x), ldexpf(q, kExpX + up - e0 - kExpB), Kept{}, 0.0f, Kept{});
                 continue;
             }
             const float *tile = M.tall ? to_tile<64, true>(acc, scratch) : to_tile<64, false>(acc, scratch);
