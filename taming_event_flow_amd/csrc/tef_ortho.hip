@@ -1056,6 +1056,71 @@ template <typename T, int LINES> __global__ __launch_bounds__(kThreads) void ort
         }
     }
 }
+
+// ---- tiny matrices: m <= 8, in plain fp32 --------------------------------------------------------------------------------------
+// A matrix instruction would be idle for the most part, and with so few terms the planes' 22 bits show (up to five times plain fp32's
+// error on 2 x 3; 25 us either way): X in LDS, one workgroup, A's m^2 elements with 256 / m^2 threads each, then every thread its columns of a X + B X.
+constexpr int kTinySide = 8, kTinyLong = 960;
+template <typename T> __global__ __launch_bounds__(kThreads) void ortho_tiny(Small list, SmallPoly p)
+{
+    __shared__ float X[kTinySide * (kTinyLong + 1)];
+    __shared__ float A[kTinySide * kTinySide], B[kTinySide * kTinySide];
+    __shared__ double red[4];
+    int k = 0;
+    while (k + 1 < list.n && list.first[k + 1] <= (int)blockIdx.x) ++k;
+    const Mat &M = list.m[k];
+    const int bi = blockIdx.x - list.first[k], cols = M.tall ? M.m : M.n, m = M.m, n = M.n, ld = n | 1, E = m * m;
+    const T *src = reinterpret_cast<const T *>(M.src) + bi * M.src_stride;
+    double s = 0.0;
+    for (int i = threadIdx.x; i < m * n; i += kThreads) {
+        const float v = to_f<T>(src[(long)(i / cols) * M.src_ld + i % cols]);
+        s += (double)v * v;
+    }
+    s = sqrt(block_sum(s, red));
+    const double mul = 1.0 / (s < p.eps ? p.eps : s);
+    for (int i = threadIdx.x; i < m * n; i += kThreads) {
+        const int r = i / cols, c = i % cols;
+        X[M.tall ? c * ld + r : r * ld + c] = (float)((double)to_f<T>(src[(long)r * M.src_ld + c]) * mul);
+    }
+    int per = 1;      // threads of an element of A
+    while (per < 64 && 2 * per * E <= kThreads) per <<= 1;
+    const int e = threadIdx.x / per, slice = threadIdx.x & (per - 1), i = e / m, j = e % m;
+    __syncthreads();
+    for (int step = 0; step < p.steps; ++step) {
+        float f = 0.0f;
+        if (e < E)
+            for (int c = slice; c < n; c += per) f = fmaf(X[i * ld + c], X[j * ld + c], f);
+        for (int o = per >> 1; o > 0; o >>= 1) f += __shfl_xor(f, o, 64);
+        if (e < E && slice == 0) A[e] = f;
+        __syncthreads();
+        if ((int)threadIdx.x < E) {
+            const int r = threadIdx.x / m, c = threadIdx.x % m;
+            float g = 0.0f;
+            for (int x = 0; x < m; ++x) g = fmaf(A[r * m + x], A[x * m + c], g);
+            B[threadIdx.x] = p.b * A[threadIdx.x] + p.c * g;
+        }
+        __syncthreads();
+        for (int c = threadIdx.x; c < n; c += kThreads) {
+            float x[kTinySide];
+#pragma unroll
+            for (int r = 0; r < kTinySide; ++r) x[r] = r < m ? X[r * ld + c] : 0.0f;
+            for (int r = 0; r < m; ++r) {
+                float g = 0.0f;
+#pragma unroll
+                for (int q = 0; q < kTinySide; ++q)
+                    if (q < m) g = fmaf(B[r * m + q], x[q], g);
+                X[r * ld + c] = p.a * (X[r * ld + c] + g);      // (b, c are over a)
+            }
+        }
+        __syncthreads();
+    }
+    T *dst = reinterpret_cast<T *>(M.dst) + bi * M.dst_stride;
+    for (int q = threadIdx.x; q < m * n; q += kThreads) {
+        const int r = q / cols, c = q % cols;
+        dst[(long)r * M.dst_ld + c] = from_f<T>(X[M.tall ? c * ld + r : r * ld + c]);
+    }
+}
+
 constexpr int kSmallSide = 64, kSmallLong = 320;      // (10 lines of X: 148 KB of LDS with A, B, R and the tile)
 
 // ---- Adam for the vectors (the same arithmetic as tef_adam_clip_step, over a list of ranges of the flat buffers) --------------------
@@ -1336,7 +1401,16 @@ int iterate(Group &g, const Poly &p, double eps, char *ws, const Step &st, hipSt
     return tef::check_launch("orthogonalisation");
 }
 
-// One workgroup a matrix when every matrix of the group is small enough: 26 us against 85 for a single 64 x 18 one.
+bool within(const Group &g, int side, int length)
+{
+    for (int k = 0; k < g.n; ++k)
+        if (g.m[k].m > side || g.m[k].n > length) return false;
+    return true;
+}
+bool all_small(const Group &g) { return within(g, kTinySide, kTinyLong) || within(g, kSmallSide, kSmallLong); }
+
+// One workgroup a matrix when every matrix of the group is small enough: 26 us against 85 for a single 64 x 18 one, 82 against 96 at
+// the limit of 64 x 320.
 template <typename T> int small(const Group &g, const Poly &p, double eps, hipStream_t stream)
 {
     const SmallPoly sp{(float)p.a, (float)(p.b / p.a), (float)(p.c / p.a), p.steps, p.first, p.grow_first, p.grow_rest, eps};
@@ -1351,17 +1425,12 @@ template <typename T> int small(const Group &g, const Poly &p, double eps, hipSt
             longest = longest > g.m[at].n ? longest : g.m[at].n;
         }
         const dim3 grid((unsigned)items), block(kThreads);
-        if (longest <= 64) hipLaunchKernelGGL((ortho_small<T, 2>), grid, block, 0, stream, list, sp);
+        if (within(g, kTinySide, kTinyLong)) hipLaunchKernelGGL(ortho_tiny<T>, grid, block, 0, stream, list, sp);
+        else if (longest <= 64) hipLaunchKernelGGL((ortho_small<T, 2>), grid, block, 0, stream, list, sp);
         else if (longest <= 128) hipLaunchKernelGGL((ortho_small<T, 4>), grid, block, 0, stream, list, sp);
         else hipLaunchKernelGGL((ortho_small<T, 10>), grid, block, 0, stream, list, sp);
     }
     return tef::check_launch("orthogonalisation");
-}
-bool all_small(const Group &g)
-{
-    for (int k = 0; k < g.n; ++k)
-        if (g.m[k].m > kSmallSide || g.m[k].n > kSmallLong) return false;
-    return true;
 }
 
 bool polynomial(Poly &p, int steps, double a, double b, double c, double eps, int first, int rest)
