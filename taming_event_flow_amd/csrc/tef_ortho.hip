@@ -16,9 +16,9 @@
 // where what the I brings is added to a product's fp32 sums unrounded.  The recurrence
 // for A multiplies its rounding errors by up to a^2 = 12 a step along small singular values, the direct iteration by a; against the plain
 // iteration in fp32, on gradients of rank m / 4 to m, segments of 2, 1, 1, 1 steps are 1.05 to 1.2 times as far from 64 bits
-// (1.4 below 64 rows), 3 + 2 steps 1.5 to 3.5 times.  orthogonalize() takes the former: 12 m^2 n + 8 m^3 / 2
-// multiply-adds (symmetric products at half) where the plain iteration takes 20 m^2 n + 10 m^3 over 2; small matrices go step by step.
-// The optimiser takes the latter, 6 m^2 n + 14 m^3 over 2: its update is scaled by the learning rate and added to fp32 parameters, whose own
+// (1.4 below 64 rows), 3 + 2 steps 1.5 to 3.5 times.  orthogonalize() takes the former: 6 m^2 n + 4 m^3
+// multiply-adds (symmetric products at half) where the plain iteration takes 10 m^2 n + 5 m^3.  Small matrices take the same segments in
+// one workgroup; tiny ones go step by step, without planes.  The optimiser takes the latter, 3 m^2 n + 7 m^3: its update is scaled by the learning rate and added to fp32 parameters, whose own
 // rounding is as large as that error.
 //
 // Arithmetic.  fp32 matrix instructions run at 1/16 of the fp16 rate, so every operand is held as two fp16 planes, v = hi + lo
@@ -1057,15 +1057,18 @@ template <typename T, int LINES> __global__ __launch_bounds__(kThreads) void ort
     }
 }
 
-// ---- tiny matrices: m <= 8, in plain fp32 --------------------------------------------------------------------------------------
-// A matrix instruction would be idle for the most part, and with so few terms the planes' 22 bits show (up to five times plain fp32's
-// error on 2 x 3; 25 us either way): X in LDS, one workgroup, A's m^2 elements with 256 / m^2 threads each, then every thread its columns of a X + B X.
+// ---- tiny matrices: m <= 8, X in fp32, sums in 64 bits -----------------------------------------------------------------------------
+// A matrix instruction would be idle for the most part, and with so few terms the planes' 22 bits show: X in LDS, one workgroup,
+// A's m^2 elements with up to 256 / m^2 threads each, then every thread its columns of a (X + B X).  Only X is rounded, once a step.
+// Largest distance from 64 bits over twelve gradients, here / in planes / the plain fp32 iteration: 2 x 3 1.2e-6 / 3.8e-6 / 1.2e-6,
+// 4 x 4 2.3e-6 / 8.6e-6 / 5.1e-6, 8 x 100 2.4e-6 / 5.1e-6 / 4.4e-6 (with fp32 sums 2.2e-6, 4.3e-6, 3.8e-6).  Time, here against in
+// planes: 25 us and 25 for 2 x 3, 26 and 33 for 8 x 100, 56 and 55 for 8 x 320, 132 and 103 at the limit of 8 x 960: taken for the
+// accuracy.  Bound by the latency of its passes over LDS and their barriers.
 constexpr int kTinySide = 8, kTinyLong = 960;
 template <typename T> __global__ __launch_bounds__(kThreads) void ortho_tiny(Small list, SmallPoly p)
 {
     __shared__ float X[kTinySide * (kTinyLong + 1)];
-    __shared__ float A[kTinySide * kTinySide], B[kTinySide * kTinySide];
-    __shared__ double red[4];
+    __shared__ double A[kTinySide * kTinySide], B[kTinySide * kTinySide], red[4];
     int k = 0;
     while (k + 1 < list.n && list.first[k + 1] <= (int)blockIdx.x) ++k;
     const Mat &M = list.m[k];
@@ -1087,29 +1090,29 @@ template <typename T> __global__ __launch_bounds__(kThreads) void ortho_tiny(Sma
     const int e = threadIdx.x / per, slice = threadIdx.x & (per - 1), i = e / m, j = e % m;
     __syncthreads();
     for (int step = 0; step < p.steps; ++step) {
-        float f = 0.0f;
+        double f = 0.0;
         if (e < E)
-            for (int c = slice; c < n; c += per) f = fmaf(X[i * ld + c], X[j * ld + c], f);
+            for (int c = slice; c < n; c += per) f = fma((double)X[i * ld + c], (double)X[j * ld + c], f);
         for (int o = per >> 1; o > 0; o >>= 1) f += __shfl_xor(f, o, 64);
         if (e < E && slice == 0) A[e] = f;
         __syncthreads();
         if ((int)threadIdx.x < E) {
             const int r = threadIdx.x / m, c = threadIdx.x % m;
-            float g = 0.0f;
-            for (int x = 0; x < m; ++x) g = fmaf(A[r * m + x], A[x * m + c], g);
+            double g = 0.0;
+            for (int x = 0; x < m; ++x) g = fma(A[r * m + x], A[x * m + c], g);
             B[threadIdx.x] = p.b * A[threadIdx.x] + p.c * g;
         }
         __syncthreads();
         for (int c = threadIdx.x; c < n; c += kThreads) {
-            float x[kTinySide];
+            double x[kTinySide];
 #pragma unroll
-            for (int r = 0; r < kTinySide; ++r) x[r] = r < m ? X[r * ld + c] : 0.0f;
+            for (int r = 0; r < kTinySide; ++r) x[r] = r < m ? (double)X[r * ld + c] : 0.0;
             for (int r = 0; r < m; ++r) {
-                float g = 0.0f;
+                double g = X[r * ld + c];
 #pragma unroll
                 for (int q = 0; q < kTinySide; ++q)
-                    if (q < m) g = fmaf(B[r * m + q], x[q], g);
-                X[r * ld + c] = p.a * (X[r * ld + c] + g);      // (b, c are over a)
+                    if (q < m) g = fma(B[r * m + q], x[q], g);
+                X[r * ld + c] = (float)(p.a * g);      // (b, c are over a)
             }
         }
         __syncthreads();
@@ -1409,8 +1412,8 @@ bool within(const Group &g, int side, int length)
 }
 bool all_small(const Group &g) { return within(g, kTinySide, kTinyLong) || within(g, kSmallSide, kSmallLong); }
 
-// One workgroup a matrix when every matrix of the group is small enough: 26 us against 85 for a single 64 x 18 one, 82 against 96 at
-// the limit of 64 x 320.
+// One workgroup a matrix when every matrix of the group is small enough: 27 us against the tiled launches' 71 for a single 64 x 18 one,
+// 81 against 94 at the limit of 64 x 320, 63 against 185 for 512 of 64 x 64.
 template <typename T> int small(const Group &g, const Poly &p, double eps, hipStream_t stream)
 {
     const SmallPoly sp{(float)p.a, (float)(p.b / p.a), (float)(p.c / p.a), p.steps, p.first, p.grow_first, p.grow_rest, eps};
