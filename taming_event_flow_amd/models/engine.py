@@ -669,8 +669,7 @@ class _EncLowFn(torch.autograd.Function):
             # the upper levels' backward (other stream: the last thing issued there — autograd walks the nodes newest first, the
             # upper range of pass t - 1 comes after this node) left a gradient for state split - 1 in the arena
             # (through the caller's stream, which idles during BPTT: on this stack hipStreamEndCapture crashes on a capture in
-            # which the low stream waits for the high one after the high one has waited for the low one —
-            # tools/experiments/capture_topology_probe.py)
+            # which the low stream waits for the high one after the high one has waited for the low one)
             if rec.high_stream is not None:
                 if rec.hub is not None and rec.hub != cur:
                     rec.hub.wait_stream(rec.high_stream)

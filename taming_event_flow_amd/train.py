@@ -155,8 +155,8 @@ class CapturedWindow:
         is decremented by one and another, 736 bytes on, is zeroed (the signature of a completion signal).  If that memory
         has been handed to a new allocation by then, the writes land there: observed in the first 4.6 KB of the NEXT
         trainer's parameter buffer (two weights of its first convolution changed, one by an ulp, one to 0.0: 6 % of the
-        iterations of tools/interference_trace.py; 0 of 100 with this wait there but still 1 of 24 in the longer test
-        sequence of tools/pytest_sequence_probe.py; 0 of 90 when graphs are never destroyed) and, in round 3, as glibc
+        iterations that looked for it; 0 of 100 with this wait there but still 1 of 24 in a longer sequence of
+        trainers; 0 of 90 when graphs are never destroyed) and, in round 3, as glibc
         heap-corruption aborts when the recycled memory was the host's.  Hence the default below: retire, do not destroy."""
         if self.graph is None and self.graph_tail is None:
             return
