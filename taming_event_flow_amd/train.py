@@ -228,6 +228,19 @@ class WindowRunner:
         return True
 
 
+def _held_by_a_graph(params):
+    """The parameters whose gradient accumulator is kept alive by an autograd graph.  The accumulator belongs to whatever graph
+    refers to it: a mark left on one that nothing else holds is gone when the accumulator is asked for again."""
+    held = []
+    for p in params:
+        if not p.requires_grad:
+            continue
+        torch.autograd.graph.get_gradient_edge(p).node.metadata["tef_mark"] = True
+        if torch.autograd.graph.get_gradient_edge(p).node.metadata.pop("tef_mark", None):
+            held.append(p)
+    return held
+
+
 class Trainer:
     """model + loss + optimiser wired like reference train_flow.py:60-70, plus the DP gradient bucket."""
 
@@ -398,6 +411,12 @@ class Trainer:
                 cw.replay()
                 self.warmup_losses.append(float(self.last_loss.item()))
             return cw
+        # (an accumulator that an eager graph keeps alive remembers that graph's stream; the captured backward pass would wait for
+        # it, which ends the process instead of raising)
+        held = _held_by_a_graph(self.model.parameters())
+        if held:
+            raise RuntimeError(f"capture_window: an autograd graph over {len(held)} of the model's parameters is alive; drop the eager "
+                               "outputs (flows, losses, states) that still refer to it first")
         inputs = [{k: v.clone() for k, v in b.items()} for b in batches]          # public static input buffers
         # update() shifts the time stamps of the two event lists in place (loss/flow.py:457-458): those two get a working copy
         # per replay, everything else is read from the static buffers directly (round 6: 70 -> 20 copy launches per window)
