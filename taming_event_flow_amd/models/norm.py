@@ -34,12 +34,15 @@ class _LayerNormFn(torch.autograd.Function):
         shape = x.shape
         if dim == len(shape) - 1:
             xc, rows = x.contiguous(), True
+            like = xc
         elif x.is_contiguous():
             xc, rows = x, False
+            like = x
         else:
             last = x.movedim(dim, -1)
             rows = last.is_contiguous()
             xc = last if rows else x.contiguous()
+            like = x if rows else xc
         rc = residual
         if rc is not None:
             rc = (rc.movedim(dim, -1) if rows else rc).contiguous()
@@ -51,7 +54,8 @@ class _LayerNormFn(torch.autograd.Function):
         vec = w if w is not None else b
         dtype = _DTYPES[x.dtype]
         d = _lib.NormDesc(n // inner if n else 0, inner if n else 1, C, dtype, dtype if vec is None else _DTYPES[vec.dtype], _lib.ACT[act], eps)
-        y = torch.empty_like(xc)
+        # results are tensors of their own in `like`'s shape and order, no views: the caller may change them in place
+        y = torch.empty_strided(shape, like.stride(), dtype=x.dtype, device=x.device)
         keep = any(ctx.needs_input_grad)
         stats = torch.empty((2 * n,), dtype=torch.float32, device=x.device) if keep else None
         at = stats.data_ptr() if keep else None
@@ -63,19 +67,18 @@ class _LayerNormFn(torch.autograd.Function):
             if act is None:      # (only an activation's slope needs them again)
                 b = rc = None
             ctx.save_for_backward(xc, w, b, rc, stats)
-            ctx.info = d, n, rows, dim
-        return y.movedim(-1, dim) if rows else y
+            ctx.info = d, n, rows, dim, shape, like.stride()
+        return y
 
     @staticmethod
     def backward(ctx, dy):
         if torch.is_grad_enabled():      # (create_graph=True)
             raise RuntimeError("layer_norm is differentiable once: its backward pass has no gradient of its own")
         xc, w, b, rc, stats = ctx.saved_tensors
-        d, n, rows, dim = ctx.info
+        d, n, rows, dim, shape, strides = ctx.info
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         dy = (dy.movedim(dim, -1) if rows else dy).contiguous()
-        dx = torch.empty_like(xc) if need_x else None
-        dr = torch.empty_like(xc) if need_r else None
+        dx, dr = (torch.empty_strided(shape, strides, dtype=xc.dtype, device=xc.device) if need else None for need in (need_x, need_r))
         lib, dw, db, ws, nbytes = _lib.lib(), None, None, None, 0
         if need_w or need_b:
             dw = torch.empty((d.channels,), dtype=_TORCH[d.wdtype], device=xc.device) if need_w else None
@@ -87,15 +90,13 @@ class _LayerNormFn(torch.autograd.Function):
             code = lib.tef_layer_norm_backward(ctypes.byref(d), xc.data_ptr(), _ptr(w), _ptr(b), _ptr(rc), at, at + 4 * n, dy.data_ptr(),
                                                _ptr(dx), _ptr(dr), _ptr(dw), _ptr(db), _ptr(ws), nbytes, _lib.stream_ptr())
         _lib.check(code, "tef_layer_norm_backward")
-        if rows:
-            dx, dr = (t.movedim(-1, dim) if t is not None else None for t in (dx, dr))
         return dx, dw, db, dr, None, None, None
 
 
 def layer_norm(x, weight=None, bias=None, dim=1, eps=1e-5, activation=None, residual=None):
     """act(normalise(x) * weight + bias + residual), normalised over the dimension `dim` at every position of the others
     (dim=1: the channels of feature maps [B, C, H, W]; dim=-1: rows).  x: float32, float16 or bfloat16 on a HIP device, any
-    strides (a contiguous or channels-last x is read in place; the result has x's memory order); weight, bias: [C], of x's
+    strides (a contiguous or channels-last x is read in place and the result has its memory order; of any other x it is contiguous); weight, bias: [C], of x's
     type or float32 (both the same), or None; residual: like x, or None; activation: "relu", "tanh", "sigmoid" or None.
     Statistics are fp32 whatever the type.  Differentiable once, with respect to x, weight, bias and residual; the
     gradients of weight and bias are reproducible bit for bit."""
