@@ -29,7 +29,7 @@ _TORCH = {code: dtype for dtype, code in _DTYPES.items()}
 
 class _LayerNormFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, dim, eps, act):
+    def forward(ctx, x, weight, bias, residual, dim, eps, act, keep):
         # a map in channels-last memory is a matrix of rows as it stands; anything else is taken in x's own dimension order
         shape = x.shape
         if dim == len(shape) - 1:
@@ -56,7 +56,6 @@ class _LayerNormFn(torch.autograd.Function):
         d = _lib.NormDesc(n // inner if n else 0, inner if n else 1, C, dtype, dtype if vec is None else _DTYPES[vec.dtype], _lib.ACT[act], eps)
         # results are tensors of their own in `like`'s shape and order, no views: the caller may change them in place
         y = torch.empty_strided(shape, like.stride(), dtype=x.dtype, device=x.device)
-        keep = any(ctx.needs_input_grad)
         stats = torch.empty((2 * n,), dtype=torch.float32, device=x.device) if keep else None
         at = stats.data_ptr() if keep else None
         with torch.cuda.device_of(x):
@@ -90,7 +89,7 @@ class _LayerNormFn(torch.autograd.Function):
             code = lib.tef_layer_norm_backward(ctypes.byref(d), xc.data_ptr(), _ptr(w), _ptr(b), _ptr(rc), at, at + 4 * n, dy.data_ptr(),
                                                _ptr(dx), _ptr(dr), _ptr(dw), _ptr(db), _ptr(ws), nbytes, _lib.stream_ptr())
         _lib.check(code, "tef_layer_norm_backward")
-        return dx, dw, db, dr, None, None, None
+        return dx, dw, db, dr, None, None, None, None
 
 
 def layer_norm(x, weight=None, bias=None, dim=1, eps=1e-5, activation=None, residual=None):
@@ -127,7 +126,9 @@ def layer_norm(x, weight=None, bias=None, dim=1, eps=1e-5, activation=None, resi
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
         raise ValueError(f"layer_norm: residual {tuple(residual.shape)} {residual.dtype} on {residual.device} for an input "
                          f"{tuple(x.shape)} {x.dtype} on {x.device}")
-    return _LayerNormFn.apply(x, weight, bias, residual, dim, float(eps), activation)
+    # (a parameter asks for gradients under no_grad too: what the backward pass needs is kept only where there will be one)
+    keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual))
+    return _LayerNormFn.apply(x, weight, bias, residual, dim, float(eps), activation, keep)
 
 
 class LayerNorm(nn.Module):

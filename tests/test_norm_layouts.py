@@ -63,3 +63,16 @@ def test_memory_order(fake):
         y = layer_norm(x)
         dense = x.is_contiguous() or x.movedim(1, -1).is_contiguous()
         assert y.stride() == (x.stride() if dense else x.contiguous().stride()), name
+
+
+def test_statistics_are_kept_for_a_backward_pass_only(fake):
+    from taming_event_flow_amd.models.norm import LayerNorm
+
+    m, x = LayerNorm(6), LAYOUTS["contiguous"]()
+    with torch.no_grad():
+        m(x)
+    m(x)
+    m.requires_grad_(False)
+    m(x)
+    m(x.requires_grad_(True))
+    assert [s is not None for s in fake.saved] == [False, True, False, True]
