@@ -537,7 +537,7 @@ int tef_adam_clip_step_hp(float *p, float *g, float *m, float *v, size_t n, cons
  * x is [outer][channels][inner], normalised over `channels` (inner = 1: rows; inner = H * W: feature maps):
  *   y = act((x - mean) * rstd * weight[c] + bias[c] + residual)
  * weight, bias, residual may each be NULL.  x, residual, y, dy, dx, dresidual have type `dtype`; weight, bias and their
- * gradients `wdtype`, which is TEF_F32 or dtype.  Statistics and sums are fp32.  Pointers need the alignment of their element
+ * gradients `wdtype`, which is TEF_F32 or dtype.  1 <= channels <= 2^30.  Statistics and sums are fp32 (sums of very long rows 64 bits).  Pointers need the alignment of their element
  * type only.  Forward: mean, rstd [outer * inner] are written for the backward pass (both NULL: not kept).
  * Backward: any of dx, dresidual, dweight, dbias may be NULL; they are WRITTEN, not accumulated.  `bias` and `residual` are
  * the forward pass's (read only when act is not TEF_ACT_NONE).  The workspace is needed for dweight / dbias; results do not depend on

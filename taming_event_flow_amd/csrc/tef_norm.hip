@@ -436,21 +436,30 @@ template <typename T, int NC, int P> __global__ __launch_bounds__(kThreads) void
 
 // ---- any C: one workgroup per position, the row read again for every sum ------------------------------------------------
 // For rows and channel counts that do not fit into the registers of a workgroup.
+// Sums are 64 bits: a thread alone adds up to 2^22 values, of which fp32 would drop the last ones' lower half.
+__device__ inline double long_sum(double s, double *red)
+{
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    return (red[0] + red[1]) + (red[2] + red[3]);
+}
+
 template <typename T> __global__ __launch_bounds__(kThreads) void long_fwd(Args a)
 {
-    __shared__ float red[kThreads / 64];
-    const float inv = 1.0f / (float)a.C;
+    __shared__ double red[kThreads / 64];
     for (long r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const long o = r / a.inner, at = o * a.C * a.inner + (r - o * a.inner);
         const T *x = reinterpret_cast<const T *>(a.x) + at;
-        float s = 0.0f, q = 0.0f;
+        double s = 0.0, q = 0.0;
         for (int c = threadIdx.x; c < a.C; c += kThreads) s += to_f<T>(x[(long)c * a.inner]);
-        const float mean = row_sum<true>(s, 64, red) * inv;
+        const float mean = (float)(long_sum(s, red) / a.C);
         for (int c = threadIdx.x; c < a.C; c += kThreads) {
             const float d = to_f<T>(x[(long)c * a.inner]) - mean;
             q += d * d;
         }
-        const float rstd = 1.0f / sqrtf(row_sum<true>(q, 64, red) * inv + a.eps);
+        const float rstd = 1.0f / sqrtf((float)(long_sum(q, red) / a.C) + a.eps);
         if (threadIdx.x == 0 && a.mean) { a.mean[r] = mean; a.rstd[r] = rstd; }
         for (int c = threadIdx.x; c < a.C; c += kThreads) {
             const long off = at + (long)c * a.inner;
@@ -475,17 +484,17 @@ template <typename T> __device__ inline float long_g(const Args &a, long off, in
 
 template <typename T> __global__ __launch_bounds__(kThreads) void long_bwd(Args a)
 {
-    __shared__ float red[kThreads / 64];
-    const float inv = 1.0f / (float)a.C;
+    __shared__ double red[kThreads / 64];
     for (long r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const long o = r / a.inner, at = o * a.C * a.inner + (r - o * a.inner);
         const float mean = a.mean[r], rstd = a.rstd[r];
-        float s1 = 0.0f, s2 = 0.0f, u;
+        double t1 = 0.0, t2 = 0.0;
+        float u;
         for (int c = threadIdx.x; c < a.C; c += kThreads) {
             const long off = at + (long)c * a.inner;
             const float g = long_g<T>(a, off, c, mean, rstd, &u), h = g * vec_at(a.v.w, a.v.dtype, c, 1.0f);
-            s1 += h;
-            s2 += h * u;
+            t1 += h;
+            t2 += h * u;
             if (a.dres) reinterpret_cast<T *>(a.dres)[off] = from_f<T>(g);
             if (a.part) {      // this thread is the only one of the workgroup at channel c
                 float *p = a.part + (long)blockIdx.x * 2 * a.C + c;
@@ -495,8 +504,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void long_bwd(Args 
             }
         }
         if (!a.dx) continue;
-        s1 = row_sum<true>(s1, 64, red) * inv;
-        s2 = row_sum<true>(s2, 64, red) * inv;
+        const float s1 = (float)(long_sum(t1, red) / a.C), s2 = (float)(long_sum(t2, red) / a.C);
         for (int c = threadIdx.x; c < a.C; c += kThreads) {
             const long off = at + (long)c * a.inner;
             const float h = long_g<T>(a, off, c, mean, rstd, &u) * vec_at(a.v.w, a.v.dtype, c, 1.0f);
@@ -511,25 +519,30 @@ constexpr int kJoinWaves = 16;
 __global__ __launch_bounds__(64 * kJoinWaves) void norm_join(const float *__restrict__ part, int parts, int C, void *dw, void *db, int dtype)
 {
     __shared__ float red[kJoinWaves][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.x * 64 + lane;
-    float s[8];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long cols = 2l * C;
+    for (long c0 = blockIdx.x * 64l; c0 < cols; c0 += gridDim.x * 64l) {      // (one round, unless the columns outnumber a launch's threads)
+        const long col = c0 + lane;
+        float s[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s[j] = 0.0f;
-    if (col < 2 * C)
-        for (int k = wave; k < parts; k += 8 * kJoinWaves) {
-            float f[8];
+        for (int j = 0; j < 8; ++j) s[j] = 0.0f;
+        if (col < cols)
+            for (int k = wave; k < parts; k += 8 * kJoinWaves) {
+                float f[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] = part[(long)(k + kJoinWaves * j < parts ? k + kJoinWaves * j : parts - 1) * 2 * C + col];
+                for (int j = 0; j < 8; ++j) f[j] = part[(k + kJoinWaves * j < parts ? k + kJoinWaves * j : parts - 1) * cols + col];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s[j] += k + kJoinWaves * j < parts ? f[j] : 0.0f;
+                for (int j = 0; j < 8; ++j) s[j] += k + kJoinWaves * j < parts ? f[j] : 0.0f;
+            }
+        __syncthreads();
+        red[wave][lane] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+        __syncthreads();
+        if (wave == 0 && col < cols) {
+            float v = 0.0f;
+            for (int k = 0; k < kJoinWaves; ++k) v += red[k][lane];
+            if (col < C) { if (dw) vec_put(dw, dtype, (int)col, v); }
+            else if (db) vec_put(db, dtype, (int)(col - C), v);
         }
-    red[wave][lane] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
-    __syncthreads();
-    if (wave == 0 && col < 2 * C) {
-        float v = 0.0f;
-        for (int k = 0; k < kJoinWaves; ++k) v += red[k][lane];
-        if (col < C) { if (dw) vec_put(dw, dtype, col, v); }
-        else if (db) vec_put(db, dtype, col - C, v);
     }
 }
 
@@ -667,7 +680,8 @@ unsigned bwd_blocks(const Plan &p, int channels)
 bool valid(const tef_norm_desc *d)
 {
     if (!d) return tef::fail("layer norm: null description");
-    const bool ok = d->channels >= 1 && d->outer >= 0 && d->inner >= 1 && d->dtype >= TEF_F32 && d->dtype <= TEF_BF16 &&
+    // (a thread's channel number goes up to 256 past the last one: 32 bits)
+    const bool ok = d->channels >= 1 && d->channels <= (1 << 30) && d->outer >= 0 && d->inner >= 1 && d->dtype >= TEF_F32 && d->dtype <= TEF_BF16 &&
                     (d->wdtype == TEF_F32 || d->wdtype == d->dtype) && d->act >= TEF_ACT_NONE && d->act <= TEF_ACT_SIGMOID &&
                     d->eps >= 0.0f && d->eps < 1e30f;
     if (!ok) return tef::fail("layer norm: invalid description (sizes, types, activation or eps)");
@@ -728,9 +742,11 @@ int tef_layer_norm_backward(const tef_norm_desc *d, const void *x, const void *w
     a.rows = (long)d->outer * d->inner; a.inner = d->inner; a.C = d->channels; a.act = d->act; a.eps = d->eps;
     const unsigned blocks = bwd_blocks(p, d->channels);
     launch(*d, p, true, blocks, st, a);
-    if (sums)
-        hipLaunchKernelGGL(norm_join, dim3((unsigned)((2l * d->channels + 63) / 64)), dim3(64 * kJoinWaves), 0, st, (const float *)workspace, (int)blocks,
+    if (sums) {
+        const long joins = (2l * d->channels + 63) / 64, most = 1l << 21;      // (a launch holds less than 2^32 threads)
+        hipLaunchKernelGGL(norm_join, dim3((unsigned)(joins < most ? joins : most)), dim3(64 * kJoinWaves), 0, st, (const float *)workspace, (int)blocks,
                            d->channels, dweight, dbias, d->wdtype);
+    }
     return tef::check_launch("layer norm backward");
 }
 

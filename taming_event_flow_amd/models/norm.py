@@ -97,7 +97,8 @@ def layer_norm(x, weight=None, bias=None, dim=1, eps=1e-5, activation=None, resi
     (dim=1: the channels of feature maps [B, C, H, W]; dim=-1: rows).  x: float32, float16 or bfloat16 on a HIP device, any
     strides (a contiguous or channels-last x is read in place and the result has its memory order; of any other x it is contiguous); weight, bias: [C], of x's
     type or float32 (both the same), or None; residual: like x, or None; activation: "relu", "tanh", "sigmoid" or None.
-    Statistics are fp32 whatever the type.  Differentiable once, with respect to x, weight, bias and residual; the
+    Statistics are fp32 whatever the type; at most 2^30 elements are
+    normalised together.  Differentiable once, with respect to x, weight, bias and residual; the
     gradients of weight and bias are reproducible bit for bit."""
     _lib.require_device_tensor(x, "layer_norm input")
     if x.dtype not in _DTYPES:
@@ -108,6 +109,8 @@ def layer_norm(x, weight=None, bias=None, dim=1, eps=1e-5, activation=None, resi
     C = x.shape[dim]
     if C == 0:
         raise ValueError("layer_norm: nothing to normalise over (the dimension has size 0)")
+    if C > 2 ** 30:
+        raise ValueError(f"layer_norm: {C} elements to normalise over (2^30 at most)")
     if not (math.isfinite(eps) and 0.0 <= eps < 1e30):
         raise ValueError(f"layer_norm: eps = {eps}")
     if activation not in _lib.ACT:

@@ -76,3 +76,26 @@ def test_statistics_are_kept_for_a_backward_pass_only(fake):
     m(x)
     m(x.requires_grad_(True))
     assert [s is not None for s in fake.saved] == [False, True, False, True]
+
+
+def test_more_channels_than_32_bits_hold(fake):
+    """A size that a 32-bit number of channels would cut down to 8 is refused, by both entry points."""
+    from taming_event_flow_amd import _lib
+    from taming_event_flow_amd.models import norm
+
+    for n in (2 ** 32 + 8, 2 ** 31, 2 ** 30 + 1):
+        x = torch.zeros((), dtype=torch.bfloat16).expand(1, n)
+        with pytest.raises(ValueError, match="at most"):
+            norm.layer_norm(x, dim=-1)
+
+
+def test_channel_limit_of_the_library():
+    import __graft_entry__ as g
+
+    g.build()
+    from taming_event_flow_amd import _lib
+
+    lib = _lib.lib()
+    for n, ok in ((2 ** 30, True), (2 ** 30 + 1, False), (2 ** 31 - 1, False)):
+        d = _lib.NormDesc(1, 1, n, 2, 0, 0, 1e-5)
+        assert (lib.tef_layer_norm_workspace_bytes(ctypes.byref(d)) == 8 * n) == ok
