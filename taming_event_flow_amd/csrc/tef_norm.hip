@@ -280,6 +280,10 @@ template <typename T, int NV, bool WG, bool EVEN> __global__ __launch_bounds__(k
 // A workgroup takes LX * P neighbouring positions (P per lane: 4 when inner is a multiple of 4, so that a lane's positions
 // are one load; else 1) and all channels: lane group g of G = 256 / LX holds the channels g, g + G, ... in registers.
 // 80 x 32 x 128 x 128 f32 with tanh: 84 us forward, 110 backward (4.0, 4.6 TB/s of a copy's 4.9).
+// A thread holds up to 64 values, one position at a time up to 16: 64 channels do not fit the register file (the backward pass spilled 789
+// registers), and 32 leave one wave a SIMD: 32 x 256 x 61 x 63 f32 takes 927 us forward and backward with up to 64, 396 with up to 32, 268 with
+// up to 16 (x 257: 1280, 578, 416).  Past 4096 channels, where a workgroup has one position, up to 32 are better than 16 with a
+// second read of everything (20 x 4097 x 15 x 15: 792 against 1600); past 8192 they are read again (8 x 16000 x 9 x 9: 891, with 64 of them 750).
 template <int P> __device__ inline void map_sum(float (&s)[P], int LX, float *red)      // over the lane groups
 {
     const int lx = threadIdx.x & (LX - 1), wave = threadIdx.x >> 6;
@@ -592,14 +596,14 @@ Plan make_plan(const tef_norm_desc &d)
         }
     } else {
         p.per = d.inner % 4 == 0 ? 4 : 1;
-        // as many lanes along the positions as leave a thread at most 64 values (long runs of memory per channel), then
+        // as many lanes along the positions as leave a thread at most 16 channels (long runs of memory per channel), then
         // fewer while the grid does not cover the 256 CUs and a thread still has more than one channel
-        const int most = 64 / p.per;
+        const int most = 16, last = p.per == 4 ? 16 : 32;      // ... with one lane along the positions: what the registers hold
         int lx = p.per == 4 ? 16 : 64;
         while (lx > 1 && (d.channels + kThreads / lx - 1) / (kThreads / lx) > most) lx >>= 1;
         while (lx > 1 && (rows + lx * p.per - 1) / (lx * p.per) < 256 && (long)d.channels * lx > kThreads) lx >>= 1;
         const int nc = (d.channels + kThreads / lx - 1) / (kThreads / lx);
-        if (nc <= most) {
+        if (nc <= last) {
             p.kind = 2;
             p.lanes = lx;
             p.n = pow2_at_least(nc);
@@ -653,8 +657,7 @@ template <typename T> void go(const Plan &p, bool bwd, dim3 grid, hipStream_t st
     case 4: go_n<T, 4>(p, bwd, grid, st, a); break;
     case 8: go_n<T, 8>(p, bwd, grid, st, a); break;
     case 16: go_n<T, 16>(p, bwd, grid, st, a); break;
-    case 32: go_n<T, 32>(p, bwd, grid, st, a); break;
-    default: go_n<T, 64>(p, bwd, grid, st, a); break;
+    default: go_n<T, 32>(p, bwd, grid, st, a); break;
     }
 }
 
