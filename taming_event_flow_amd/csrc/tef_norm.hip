@@ -119,7 +119,8 @@ struct Args {
 // A row belongs to L lanes (a power of two, at most one wave: no barrier, several short rows a wave) or, WG, to the whole
 // workgroup.  Lane l holds the elements V * (l + L * i) .. + V - 1, i < NV, in registers, and keeps the weights of its
 // columns over all rows that it takes.  4096 x 4096 bf16: 29 us forward, 42 backward (2.3, 2.4 TB/s; one row a workgroup at a time,
-// two joins of its waves each: latency, hidden by eight workgroups a CU).
+// two joins of its waves each: latency, hidden by eight workgroups a CU).  Rows that are no multiple of 4 are loaded by the element: 8192 x 8191
+// f32 592 us forward and backward (x 8188: 347; 19 of the backward pass's registers do not fit), in the form below, x 8193, 1092.
 constexpr int V = 4;
 
 template <bool WG> __device__ inline float row_sum(float s, int L, float *red)
@@ -636,7 +637,7 @@ template <typename T, int N> void go_n(const Plan &p, bool bwd, dim3 grid, hipSt
 {
     if constexpr (N <= 8) {
         if (p.kind == 0) return go_rows<T, N, false>(p, bwd, grid, st, a);
-        if constexpr (N > 1)
+        if constexpr (N > 2)      // (the workgroup form starts at 513 packs, three a thread)
             if (p.kind == 1) return go_rows<T, N, true>(p, bwd, grid, st, a);
     }
     if constexpr (N <= 16)
