@@ -12,7 +12,9 @@
 // this package's networks.  Bound by memory: the forward pass reads x (and residual) once and writes y once, the backward
 // pass reads x, dy (and residual where the activation needs z) once and writes dx (and dresidual) once; a row's values stay
 // in registers between its sums and its results.  Sums and statistics are fp32: a lane adds its own elements, then lanes
-// and waves are joined in a fixed order.  The variance is taken of (x - mean), not as a difference of large moments.  z is
+// and waves are joined in a fixed order.  The variance is taken of d = x - mean, not as a difference of large moments, and the mean of d,
+// the mean's own rounding, is taken off d (its sum rides on the join of the variance's): a constant row gives exactly the bias, and a mean far
+// larger than the spread costs the forward pass nothing.  The mean that the backward pass gets is that one rounded to fp32.  z is
 // formed again in the backward pass instead of being derived from the rounded y: 1 - y^2 of a half-precision y near 1 has
 // no correct digit.  The sums over rows (dweight, dbias) go through one partial row per workgroup and a second launch that
 // adds those in a fixed order: bit-for-bit reproducible, no atomics.
@@ -118,7 +120,7 @@ struct Args {
 // ---- rows: C contiguous --------------------------------------------------------------------------------------------------
 // A row belongs to L lanes (a power of two, at most one wave: no barrier, several short rows a wave) or, WG, to the whole
 // workgroup.  Lane l holds the elements V * (l + L * i) .. + V - 1, i < NV, in registers, and keeps the weights of its
-// columns over all rows that it takes.  4096 x 4096 bf16: 29 us forward, 42 backward (2.3, 2.4 TB/s; one row a workgroup at a time,
+// columns over all rows that it takes.  4096 x 4096 bf16: 30 us forward, 42 backward (2.2, 2.4 TB/s; one row a workgroup at a time,
 // two joins of its waves each: latency, hidden by eight workgroups a CU).  Rows that are no multiple of 4 are loaded by the element: 8192 x 8191
 // f32 592 us forward and backward (x 8188: 347; 19 of the backward pass's registers do not fit), in the form below, x 8193, 1092.
 constexpr int V = 4;
@@ -135,6 +137,32 @@ template <bool WG> __device__ inline float row_sum(float s, int L, float *red)
     return s;
 }
 
+// the same of two sums at once
+template <bool WG> __device__ inline void row_sums(float &s, float &q, int L, float *red)
+{
+    for (int o = (WG ? 64 : L) >> 1; o > 0; o >>= 1) {
+        s += __shfl_xor(s, o, 64);
+        q += __shfl_xor(q, o, 64);
+    }
+    if (WG) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) { red[threadIdx.x >> 6] = s; red[4 + (threadIdx.x >> 6)] = q; }
+        __syncthreads();
+        s = (red[0] + red[1]) + (red[2] + red[3]);
+        q = (red[4] + red[5]) + (red[6] + red[7]);
+    }
+}
+// sums of d and d^2 -> the correction of the mean, 1 / sqrt(variance + eps)
+// (inv = 1 / C: products, not divisions, which cost the widest maps a tenth of their time; what a product adds to the first mean is
+// corrected here with the rest of it)
+__device__ inline float correct(float &mean, float sd, float sq, float inv, float eps, float &rstd)
+{
+    const float by = sd * inv, var = (sq - sd * by) * inv;
+    rstd = 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + eps);      // (NaN stays NaN)
+    mean += by;
+    return by;
+}
+
 template <int NV> __device__ inline void row_vec(const void *p, int dtype, int l, int L, int C, float missing, float (&f)[NV][V])
 {
 #pragma unroll
@@ -148,7 +176,7 @@ template <int NV> __device__ inline void row_vec(const void *p, int dtype, int l
 
 template <typename T, int NV, bool WG, bool EVEN> __global__ __launch_bounds__(kThreads) void rows_fwd(Args a, int L)
 {
-    __shared__ float red[kThreads / 64];
+    __shared__ float red[2 * kThreads / 64];
     const int l = WG ? threadIdx.x : threadIdx.x & (L - 1), per = WG ? 1 : kThreads / L, C = a.C;
     const float inv = 1.0f / (float)C;
     float w[NV][V], b[NV][V];
@@ -164,29 +192,32 @@ template <typename T, int NV, bool WG, bool EVEN> __global__ __launch_bounds__(k
         if (a.res)
 #pragma unroll
             for (int i = 0; i < NV; ++i) e[i] = raw_row<T, V, EVEN>(reinterpret_cast<const T *>(a.res) + at, V * (l + L * i), C);
-        float f[NV][V], s = 0.0f, v = 0.0f;
+        float f[NV][V], s = 0.0f, v = 0.0f, d = 0.0f, rstd;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
 #pragma unroll
             for (int k = 0; k < V; ++k) f[i][k] = V * (l + L * i) + k < C ? to_f<T>(q[i].v[k]) : 0.0f;
             s += (f[i][0] + f[i][1]) + (f[i][2] + f[i][3]);
         }
-        const float mean = row_sum<WG>(s, L, red) * inv;
+        float mean = row_sum<WG>(s, L, red) * inv;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int k = 0; k < V; ++k) {
+                const bool in = V * (l + L * i) + k < C;
                 f[i][k] -= mean;
-                v += V * (l + L * i) + k < C ? f[i][k] * f[i][k] : 0.0f;
+                d += in ? f[i][k] : 0.0f;
+                v += in ? f[i][k] * f[i][k] : 0.0f;
             }
-        const float rstd = 1.0f / sqrtf(row_sum<WG>(v, L, red) * inv + a.eps);
+        row_sums<WG>(d, v, L, red);
+        const float by = correct(mean, d, v, inv, a.eps, rstd);
         if (!live) continue;
         if (l == 0 && a.mean) { a.mean[r] = mean; a.rstd[r] = rstd; }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
 #pragma unroll
             for (int k = 0; k < V; ++k)
-                f[i][k] = act(a.act, f[i][k] * rstd * w[i][k] + b[i][k] + (a.res ? to_f<T>(e[i].v[k]) : 0.0f));
+                f[i][k] = act(a.act, (f[i][k] - by) * rstd * w[i][k] + b[i][k] + (a.res ? to_f<T>(e[i].v[k]) : 0.0f));
             store_row<T, V, EVEN>(reinterpret_cast<T *>(a.y) + at, V * (l + L * i), C, f[i]);
         }
     }
@@ -280,7 +311,7 @@ template <typename T, int NV, bool WG, bool EVEN> __global__ __launch_bounds__(k
 // ---- maps: the channels of a position lie `inner` elements apart --------------------------------------------------------
 // A workgroup takes LX * P neighbouring positions (P per lane: 4 when inner is a multiple of 4, so that a lane's positions
 // are one load; else 1) and all channels: lane group g of G = 256 / LX holds the channels g, g + G, ... in registers.
-// 80 x 32 x 128 x 128 f32 with tanh: 84 us forward, 110 backward (4.0, 4.6 TB/s of a copy's 4.9).
+// 80 x 32 x 128 x 128 f32 with tanh: 81 us forward, 110 backward (4.1, 4.6 TB/s of a copy's 4.9).
 // A thread holds up to 64 values, one position at a time up to 16: 64 channels do not fit the register file (the backward pass spilled 789
 // registers), and 32 leave one wave a SIMD: 32 x 256 x 61 x 63 f32 takes 927 us forward and backward with up to 64, 396 with up to 32, 268 with
 // up to 16 (x 257: 1280, 578, 416).  Past 4096 channels, where a workgroup has one position, up to 32 are better than 16 with a
@@ -301,9 +332,46 @@ template <int P> __device__ inline void map_sum(float (&s)[P], int LX, float *re
         s[k] = (red[lx * P + k] + red[(LX + lx) * P + k]) + (red[(2 * LX + lx) * P + k] + red[(3 * LX + lx) * P + k]);
 }
 
+// Second sums of a tile's positions, of d = x - mean and d^2: by[k] what the mean is corrected by, rstd[k]; position j of the tile is
+// finished by thread j alone (all threads for themselves: 103 us instead of 81 for the map above) and, if asked for, stored.
+// red: the partial sums that the mean was made of, then room for 3 * 256.
+template <int P>
+__device__ inline void map_stats(const float (&d)[P], const float (&q)[P], float (&by)[P], float (&rstd)[P], int LX, float *red, float inv,
+                                 float eps, float *mean_out, float *rstd_out, long at, long rows)
+{
+    const int lx = threadIdx.x & (LX - 1), wave = threadIdx.x >> 6, j = threadIdx.x, n = LX * P;
+    float *rd = red + 256, *rq = red + 512, *out = red + 768;
+    float sd[P], sq[P];
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+        sd[k] = d[k];
+        sq[k] = q[k];
+        for (int o = 32; o >= LX; o >>= 1) {
+            sd[k] += __shfl_xor(sd[k], o, 64);
+            sq[k] += __shfl_xor(sq[k], o, 64);
+        }
+    }
+    if ((int)(threadIdx.x & 63) < LX)
+#pragma unroll
+        for (int k = 0; k < P; ++k) {
+            rd[wave * n + lx * P + k] = sd[k];
+            rq[wave * n + lx * P + k] = sq[k];
+        }
+    __syncthreads();
+    if (j < n) {
+        float mean = ((red[j] + red[n + j]) + (red[2 * n + j] + red[3 * n + j])) * inv, r;
+        out[j] = correct(mean, (rd[j] + rd[n + j]) + (rd[2 * n + j] + rd[3 * n + j]), (rq[j] + rq[n + j]) + (rq[2 * n + j] + rq[3 * n + j]), inv, eps, r);
+        out[64 + j] = r;
+        if (mean_out && at + j < rows) { mean_out[at + j] = mean; rstd_out[at + j] = r; }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < P; ++k) { by[k] = out[lx * P + k]; rstd[k] = out[64 + lx * P + k]; }
+}
+
 template <typename T, int NC, int P> __global__ __launch_bounds__(kThreads) void maps_fwd(Args a, int LX)
 {
-    __shared__ float red[4 * 64 * P];
+    __shared__ __attribute__((aligned(16))) float red[3 * 256 + 128];      // (a tile has at most 64 positions)
     const int lx = threadIdx.x & (LX - 1), g = threadIdx.x / LX, G = kThreads / LX, C = a.C;
     const float inv = 1.0f / (float)C;
     const long tile = (long)LX * P;
@@ -324,9 +392,9 @@ template <typename T, int NC, int P> __global__ __launch_bounds__(kThreads) void
         if (a.res)
 #pragma unroll
             for (int i = 0; i < NC; ++i) e[i] = raw<T, P>(reinterpret_cast<const T *>(a.res) + at + (g + G * i < C ? g + G * i : C - 1) * a.inner);
-        float f[NC][P], s[P], v[P];
+        float f[NC][P], s[P], v[P], d[P], by[P], rstd[P];
 #pragma unroll
-        for (int k = 0; k < P; ++k) s[k] = v[k] = 0.0f;
+        for (int k = 0; k < P; ++k) s[k] = v[k] = d[k] = 0.0f;
 #pragma unroll
         for (int i = 0; i < NC; ++i)
 #pragma unroll
@@ -342,19 +410,17 @@ template <typename T, int NC, int P> __global__ __launch_bounds__(kThreads) void
 #pragma unroll
             for (int k = 0; k < P; ++k) {
                 f[i][k] -= s[k];
+                d[k] += g + G * i < C ? f[i][k] : 0.0f;
                 v[k] += g + G * i < C ? f[i][k] * f[i][k] : 0.0f;
             }
-        map_sum<P>(v, LX, red);
-#pragma unroll
-        for (int k = 0; k < P; ++k) v[k] = 1.0f / sqrtf(v[k] * inv + a.eps);
+        map_stats<P>(d, v, by, rstd, LX, red, inv, a.eps, a.mean, a.rstd, t * tile, a.rows);
         if (!live) continue;
-        if (a.mean && g == 0) { store<float, P>(a.mean + pos, s); store<float, P>(a.rstd + pos, v); }
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
             const int c = g + G * i;
             if (c >= C) continue;
 #pragma unroll
-            for (int k = 0; k < P; ++k) f[i][k] = act(a.act, f[i][k] * v[k] * w[i] + b[i] + (a.res ? to_f<T>(e[i].v[k]) : 0.0f));
+            for (int k = 0; k < P; ++k) f[i][k] = act(a.act, (f[i][k] - by[k]) * rstd[k] * w[i] + b[i] + (a.res ? to_f<T>(e[i].v[k]) : 0.0f));
             store<T, P>(reinterpret_cast<T *>(a.y) + at + c * a.inner, f[i]);
         }
     }
@@ -362,7 +428,7 @@ template <typename T, int NC, int P> __global__ __launch_bounds__(kThreads) void
 
 template <typename T, int NC, int P> __global__ __launch_bounds__(kThreads) void maps_bwd(Args a, int LX)
 {
-    __shared__ float red[4 * 64 * P];
+    __shared__ float red[256];
     const int lx = threadIdx.x & (LX - 1), g = threadIdx.x / LX, G = kThreads / LX, C = a.C;
     const float inv = 1.0f / (float)C;
     const bool need_z = a.act != TEF_ACT_NONE, need_e = need_z && a.res;
@@ -459,17 +525,17 @@ template <typename T> __global__ __launch_bounds__(kThreads) void long_fwd(Args 
         const T *x = reinterpret_cast<const T *>(a.x) + at;
         double s = 0.0, q = 0.0;
         for (int c = threadIdx.x; c < a.C; c += kThreads) s += to_f<T>(x[(long)c * a.inner]);
-        const float mean = (float)(long_sum(s, red) / a.C);
+        const double mean = long_sum(s, red) / a.C;
         for (int c = threadIdx.x; c < a.C; c += kThreads) {
-            const float d = to_f<T>(x[(long)c * a.inner]) - mean;
+            const double d = to_f<T>(x[(long)c * a.inner]) - mean;
             q += d * d;
         }
         const float rstd = 1.0f / sqrtf((float)(long_sum(q, red) / a.C) + a.eps);
-        if (threadIdx.x == 0 && a.mean) { a.mean[r] = mean; a.rstd[r] = rstd; }
+        if (threadIdx.x == 0 && a.mean) { a.mean[r] = (float)mean; a.rstd[r] = rstd; }
         for (int c = threadIdx.x; c < a.C; c += kThreads) {
             const long off = at + (long)c * a.inner;
             const float e = a.res ? to_f<T>(reinterpret_cast<const T *>(a.res)[off]) : 0.0f;
-            const float z = (to_f<T>(reinterpret_cast<const T *>(a.x)[off]) - mean) * rstd * vec_at(a.v.w, a.v.dtype, c, 1.0f) +
+            const float z = (float)(to_f<T>(reinterpret_cast<const T *>(a.x)[off]) - mean) * rstd * vec_at(a.v.w, a.v.dtype, c, 1.0f) +
                             vec_at(a.v.b, a.v.dtype, c, 0.0f) + e;
             reinterpret_cast<T *>(a.y)[off] = from_f<T>(act(a.act, z));
         }
