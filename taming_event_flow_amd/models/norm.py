@@ -55,7 +55,7 @@ class _LayerNormFn(torch.autograd.Function):
         dtype = _DTYPES[x.dtype]
         d = _lib.NormDesc(n // inner if n else 0, inner if n else 1, C, dtype, dtype if vec is None else _DTYPES[vec.dtype], _lib.ACT[act], eps)
         # results are tensors of their own in `like`'s shape and order, no views: the caller may change them in place
-        y = torch.empty_strided(shape, like.stride(), dtype=x.dtype, device=x.device)
+        y = torch.empty_like(like)
         stats = torch.empty((2 * n,), dtype=torch.float32, device=x.device) if keep else None
         at = stats.data_ptr() if keep else None
         with torch.cuda.device_of(x):
@@ -130,7 +130,8 @@ def layer_norm(x, weight=None, bias=None, dim=1, eps=1e-5, activation=None, resi
         raise ValueError(f"layer_norm: residual {tuple(residual.shape)} {residual.dtype} on {residual.device} for an input "
                          f"{tuple(x.shape)} {x.dtype} on {x.device}")
     # (a parameter asks for gradients under no_grad too: what the backward pass needs is kept only where there will be one)
-    keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual))
+    keep = torch.is_grad_enabled() and (x.requires_grad or weight is not None and weight.requires_grad or bias is not None and bias.requires_grad
+                                        or residual is not None and residual.requires_grad)
     return _LayerNormFn.apply(x, weight, bias, residual, dim, float(eps), activation, keep)
 
 
