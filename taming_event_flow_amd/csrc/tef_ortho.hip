@@ -1181,6 +1181,7 @@ bool bounded(Poly &p)
     return true;
 }
 
+enum Form { TINY, SMALL, TILED, FORMS };
 struct Cut { int whole, splits; long items, joins; };
 struct Group {
     Mat m[kGroup];
@@ -1404,17 +1405,9 @@ int iterate(Group &g, const Poly &p, double eps, char *ws, const Step &st, hipSt
     return tef::check_launch("orthogonalisation");
 }
 
-bool within(const Group &g, int side, int length)
-{
-    for (int k = 0; k < g.n; ++k)
-        if (g.m[k].m > side || g.m[k].n > length) return false;
-    return true;
-}
-bool all_small(const Group &g) { return within(g, kTinySide, kTinyLong) || within(g, kSmallSide, kSmallLong); }
-
-// One workgroup a matrix when every matrix of the group is small enough: 27 us against the tiled launches' 71 for a single 64 x 18 one,
+// One workgroup a matrix for small ones: 27 us against the tiled launches' 71 for a single 64 x 18 one,
 // 81 against 94 at the limit of 64 x 320, 63 against 185 for 512 of 64 x 64.
-template <typename T> int small(const Group &g, const Poly &p, double eps, hipStream_t stream)
+template <typename T> int small(const Group &g, Form form, const Poly &p, double eps, hipStream_t stream)
 {
     const SmallPoly sp{(float)p.a, (float)(p.b / p.a), (float)(p.c / p.a), p.steps, p.first, p.grow_first, p.grow_rest, eps};
     for (int at = 0; at < g.n;) {
@@ -1428,7 +1421,7 @@ template <typename T> int small(const Group &g, const Poly &p, double eps, hipSt
             longest = longest > g.m[at].n ? longest : g.m[at].n;
         }
         const dim3 grid((unsigned)items), block(kThreads);
-        if (within(g, kTinySide, kTinyLong)) hipLaunchKernelGGL(ortho_tiny<T>, grid, block, 0, stream, list, sp);
+        if (form == TINY) hipLaunchKernelGGL(ortho_tiny<T>, grid, block, 0, stream, list, sp);
         else if (longest <= 64) hipLaunchKernelGGL((ortho_small<T, 2>), grid, block, 0, stream, list, sp);
         else if (longest <= 128) hipLaunchKernelGGL((ortho_small<T, 4>), grid, block, 0, stream, list, sp);
         else hipLaunchKernelGGL((ortho_small<T, 10>), grid, block, 0, stream, list, sp);
@@ -1444,48 +1437,60 @@ bool polynomial(Poly &p, int steps, double a, double b, double c, double eps, in
     return bounded(p);
 }
 
-bool group_of(Group &g, const tef_ortho_matrix *m, int at, int count)
+// What a matrix goes through, by its own size alone: its bits do not depend on the other matrices of the call.  (Tiles are planned for a
+// group, though: where a product is cut along k, and with it the order of its sums, depends on the tiled matrices beside it.)
+template <typename D> Form form_of(const D &d, bool step)
 {
-    g.n = count - at < kGroup ? count - at : kGroup;
-    for (int k = 0; k < g.n; ++k) {
-        const tef_ortho_matrix &d = m[at + k];
-        Mat &M = g.m[k];
-        if (!describe(M, d.rows, d.cols, d.batch)) return false;
-        if (d.src_ld < d.cols || d.dst_ld < d.cols) return tef::fail("orthogonalisation: row stride shorter than a row");
-        M.src = d.src; M.dst = d.dst;
-        M.src_ld = d.src_ld; M.dst_ld = d.dst_ld;
-        M.src_stride = d.src_stride; M.dst_stride = d.dst_stride;
-    }
-    plan(g);
+    const long m = d.rows < d.cols ? d.rows : d.cols, n = d.rows < d.cols ? d.cols : d.rows;
+    if (step) return TILED;
+    return m <= kTinySide && n <= kTinyLong ? TINY : m <= kSmallSide && n <= kSmallLong ? SMALL : TILED;
+}
+
+bool take(Mat &M, const tef_ortho_matrix &d)
+{
+    if (!describe(M, d.rows, d.cols, d.batch)) return false;
+    if (d.src_ld < d.cols || d.dst_ld < d.cols) return tef::fail("orthogonalisation: row stride shorter than a row");
+    M.src = d.src; M.dst = d.dst;
+    M.src_ld = d.src_ld; M.dst_ld = d.dst_ld;
+    M.src_stride = d.src_stride; M.dst_stride = d.dst_stride;
+    return true;
+}
+bool take(Mat &M, const tef_muon_matrix &d)
+{
+    if (!describe(M, d.rows, d.cols, 1)) return false;
+    if (d.offset < 0) return tef::fail("tef_muon_step: negative offset");
+    M.src = reinterpret_cast<const void *>(d.offset); M.dst = reinterpret_cast<void *>(d.offset);
+    M.src_ld = M.dst_ld = d.cols;
+    M.scale = d.scale;
     return true;
 }
 
-bool group_of(Group &g, const tef_muon_matrix *m, int at, int count)
+// the list's next matrices of one form, from number `at` on (g.n = 0: no more)
+template <typename D> bool next_group(Group &g, const D *m, int &at, int count, Form form, bool step)
 {
-    g.n = count - at < kGroup ? count - at : kGroup;
-    for (int k = 0; k < g.n; ++k) {
-        const tef_muon_matrix &d = m[at + k];
-        Mat &M = g.m[k];
-        if (!describe(M, d.rows, d.cols, 1)) return false;
-        if (d.offset < 0) return tef::fail("tef_muon_step: negative offset");
-        M.src = reinterpret_cast<const void *>(d.offset); M.dst = reinterpret_cast<void *>(d.offset);
-        M.src_ld = M.dst_ld = d.cols;
-        M.scale = d.scale;
-    }
-    plan(g);
+    g.n = 0;
+    g.bytes = 0;
+    for (; at < count && g.n < kGroup; ++at)
+        if (form_of(m[at], step) == form && !take(g.m[g.n++], m[at])) return false;
+    if (g.n && form == TILED) plan(g);
     return true;
 }
 
-// (one workgroup a matrix needs none; the optimiser's step does not go that way)
-template <typename D> size_t workspace_of(const D *m, int count, bool small_ones)
+template <typename T> int run(Group &g, Form form, const Poly &p, double eps, char *ws, hipStream_t stream)
+{
+    return form == TILED ? iterate<T, false>(g, p, eps, ws, Step{}, stream) : small<T>(g, form, p, eps, stream);
+}
+
+template <typename D> size_t workspace_of(const D *m, int count, bool step)
 {
     if (count < 0 || (count && !m)) return tef::fail("orthogonalisation: null matrix list"), 0;
     size_t most = 256;
     Group g;
-    for (int at = 0; at < count; at += kGroup) {
-        if (!group_of(g, m, at, count)) return 0;
-        if (!(small_ones && all_small(g)) && (size_t)g.bytes > most) most = (size_t)g.bytes;
-    }
+    for (int form = 0; form < FORMS; ++form)
+        for (int at = 0; at < count;) {
+            if (!next_group(g, m, at, count, (Form)form, step)) return 0;
+            if ((size_t)g.bytes > most) most = (size_t)g.bytes;
+        }
     return most;
 }
 
@@ -1493,7 +1498,7 @@ template <typename D> size_t workspace_of(const D *m, int count, bool small_ones
 
 extern "C" {
 
-size_t tef_orthogonalize_workspace_bytes(const tef_ortho_matrix *matrices, int count) { return workspace_of(matrices, count, true); }
+size_t tef_orthogonalize_workspace_bytes(const tef_ortho_matrix *matrices, int count) { return workspace_of(matrices, count, false); }
 
 int tef_orthogonalize(const tef_ortho_matrix *matrices, int count, int dtype, int steps, double a, double b, double c, double eps,
                       void *workspace, size_t workspace_bytes, void *stream)
@@ -1501,7 +1506,7 @@ int tef_orthogonalize(const tef_ortho_matrix *matrices, int count, int dtype, in
     Poly p;
     if (!polynomial(p, steps, a, b, c, eps, 2, 1)) return TEF_ERR_INVALID;
     if (dtype < TEF_F32 || dtype > TEF_BF16) return tef::fail("tef_orthogonalize: type"), TEF_ERR_INVALID;
-    const size_t need = workspace_of(matrices, count, true);
+    const size_t need = workspace_of(matrices, count, false);
     if (!need) return TEF_ERR_INVALID;
     if (count == 0) return 0;
     for (int k = 0; k < count; ++k)
@@ -1509,25 +1514,20 @@ int tef_orthogonalize(const tef_ortho_matrix *matrices, int count, int dtype, in
     if (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < need)
         return tef::fail("tef_orthogonalize: workspace too small or not 256-byte aligned"), TEF_ERR_WORKSPACE;
     Group g;
-    for (int at = 0; at < count; at += kGroup) {
-        if (!group_of(g, matrices, at, count)) return TEF_ERR_INVALID;
-        if (all_small(g)) {
-            const int rc = dtype == TEF_F32 ? small<float>(g, p, eps, (hipStream_t)stream)
-                         : dtype == TEF_F16 ? small<__half>(g, p, eps, (hipStream_t)stream)
-                                            : small<__hip_bfloat16>(g, p, eps, (hipStream_t)stream);
+    for (int f = 0; f < FORMS; ++f)
+        for (int at = 0; at < count;) {
+            const Form form = (Form)f;
+            if (!next_group(g, matrices, at, count, form, false)) return TEF_ERR_INVALID;
+            if (!g.n) break;
+            const int rc = dtype == TEF_F32 ? run<float>(g, form, p, eps, (char *)workspace, (hipStream_t)stream)
+                         : dtype == TEF_F16 ? run<__half>(g, form, p, eps, (char *)workspace, (hipStream_t)stream)
+                                            : run<__hip_bfloat16>(g, form, p, eps, (char *)workspace, (hipStream_t)stream);
             if (rc) return rc;
-            continue;
         }
-        const Step none{};
-        const int rc = dtype == TEF_F32 ? iterate<float, false>(g, p, eps, (char *)workspace, none, (hipStream_t)stream)
-                     : dtype == TEF_F16 ? iterate<__half, false>(g, p, eps, (char *)workspace, none, (hipStream_t)stream)
-                                        : iterate<__hip_bfloat16, false>(g, p, eps, (char *)workspace, none, (hipStream_t)stream);
-        if (rc) return rc;
-    }
     return 0;
 }
 
-size_t tef_muon_workspace_bytes(const tef_muon_matrix *matrices, int count) { return workspace_of(matrices, count, false); }
+size_t tef_muon_workspace_bytes(const tef_muon_matrix *matrices, int count) { return workspace_of(matrices, count, true); }
 
 int tef_muon_step(float *p, float *g, float *m, float *v, const tef_muon_matrix *matrices, int nmatrices, const tef_muon_vector *vectors,
                   int nvectors, const float *norm, const double *hp, const float *step, int nesterov, int steps, double a, double b,
@@ -1543,15 +1543,16 @@ int tef_muon_step(float *p, float *g, float *m, float *v, const tef_muon_matrix 
         total += vectors[k].size;
     }
     if (total > 0x3fffffff) return tef::fail("tef_muon_step: more than 2^30 vector elements"), TEF_ERR_INVALID;
-    const size_t need = workspace_of(matrices, nmatrices, false);
+    const size_t need = workspace_of(matrices, nmatrices, true);
     if (!need) return TEF_ERR_INVALID;
     if (nmatrices && (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < need))
         return tef::fail("tef_muon_step: workspace too small or not 256-byte aligned"), TEF_ERR_WORKSPACE;
     hipStream_t st = (hipStream_t)stream;
     const Step s{g, m, p, norm, hp, nesterov != 0};
     Group gr;
-    for (int at = 0; at < nmatrices; at += kGroup) {
-        if (!group_of(gr, matrices, at, nmatrices)) return TEF_ERR_INVALID;
+    for (int at = 0; at < nmatrices;) {
+        if (!next_group(gr, matrices, at, nmatrices, TILED, true)) return TEF_ERR_INVALID;
+        if (!gr.n) break;
         const int rc = iterate<float, true>(gr, poly, eps, (char *)workspace, s, st);
         if (rc) return rc;
     }

@@ -56,8 +56,9 @@ def _as_batch(t):
 def orthogonalize(update, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     """Newton-Schulz orthogonalisation: X = U / max(|U|, eps), then `steps` times X <- a X + (b A + c A A) X with A = X X^T (for a tall
     matrix X^T X), coefficients (a, b, c).  update: a matrix [rows, cols], a batch of them [..., rows, cols], or a list / tuple of such tensors
-    (any mix of shapes, one type, one device: all of them in the same launches); float32, float16 or bfloat16.  -> new tensor(s)
-    of the same shape and type.  The arithmetic is fp32-grade whatever the type.  A zero matrix gives zeros, a NaN or an
+    (any mix of shapes, one type, one device: matrices of one kind in the same launches); float32, float16 or bfloat16.  -> new tensor(s)
+    of the same shape and type.  The arithmetic is fp32-grade whatever the type.  A matrix of up to 64 x 320 has the same bits alone and in any
+    list; of larger ones the order of sums depends on the larger ones beside it.  A zero matrix gives zeros, a NaN or an
     infinity makes its own matrix NaN.  Not differentiable."""
     many = isinstance(update, (list, tuple))
     tensors = list(update) if many else [update]
