@@ -18,7 +18,7 @@
 // iteration in fp32, on gradients of rank m / 4 to m, segments of 2, 1, 1, 1 steps are 1.05 to 1.2 times as far from 64 bits
 // (1.4 below 64 rows), 3 + 2 steps 1.5 to 3.5 times.  orthogonalize() takes the former: 6 m^2 n + 4 m^3
 // multiply-adds (symmetric products at half) where the plain iteration takes 10 m^2 n + 5 m^3.  Small matrices take the same segments in
-// one workgroup; tiny ones go step by step, without planes.  The optimiser takes the latter, 3 m^2 n + 7 m^3: its update is scaled by the learning rate and added to fp32 parameters, whose own
+// one workgroup; those of up to 8 rows are iterated on the small side alone, in 64 bits, without planes.  The optimiser takes the latter, 3 m^2 n + 7 m^3: its update is scaled by the learning rate and added to fp32 parameters, whose own
 // rounding is as large as that error.
 //
 // Arithmetic.  fp32 matrix instructions run at 1/16 of the fp16 rate, so every operand is held as two fp16 planes, v = hi + lo
@@ -1057,70 +1057,207 @@ template <typename T, int LINES> __global__ __launch_bounds__(kThreads) void ort
     }
 }
 
-// ---- tiny matrices: m <= 8, X in fp32, sums in 64 bits -----------------------------------------------------------------------------
-// A matrix instruction would be idle for the most part, and with so few terms the planes' 22 bits show: X in LDS, one workgroup,
-// A's m^2 elements with up to 256 / m^2 threads each, then every thread its columns of a (X + B X).  Only X is rounded, once a step.
-// Largest distance from 64 bits over twelve gradients, here / in planes / the plain fp32 iteration: 2 x 3 1.2e-6 / 3.8e-6 / 1.2e-6,
-// 4 x 4 2.3e-6 / 8.6e-6 / 5.1e-6, 8 x 100 2.4e-6 / 5.1e-6 / 4.4e-6 (with fp32 sums 2.2e-6, 4.3e-6, 3.8e-6).  Time, here against in
-// planes: 25 us and 25 for 2 x 3, 26 and 33 for 8 x 100, 56 and 55 for 8 x 320, 132 and 103 at the limit of 8 x 960: taken for the
-// accuracy.  Bound by the latency of its passes over LDS and their barriers.
-constexpr int kTinySide = 8, kTinyLong = 960;
-template <typename T> __global__ __launch_bounds__(kThreads) void ortho_tiny(Small list, SmallPoly p)
+// ---- tiny matrices: m <= 8, sums and the iteration in 64 bits ------------------------------------------------------------------------
+// A matrix instruction would be idle for the most part, and with so few terms the planes' 22 bits show.  One pass over the matrix sums
+// A = X X^T (m (m + 1) / 2 sums a thread), the iteration runs on the small side alone (P = a I + b A + c A A, A' = P A P, Q' = P Q, 64 lanes
+// an 8 x 8 matrix), a second pass writes Q X: everything in 64 bits, rounded once at the end.  A' multiplies A's rounding by up to max|P|^2 a
+// step, so more steps than `run` (10^6 between them: 5 with the usual coefficients) are cut into segments of as many: X <- Q X is kept in
+// 64 bits, in LDS or the workspace, and A summed again.  Distance from an iteration in 64 bits on gradients of 2 x 3 to 8 x 8192: half a
+// step of fp32, where the plain fp32 iteration is 0.4 to 4.8e-6 off.
+// Up to kTinyOne columns a matrix is one workgroup's, in one launch (TINY); longer ones take a launch for each sum and one for the
+// result, in workgroups of kTinyPer columns and more, whose sums go through the workspace and are added up in order by every workgroup
+// of the next launch (THIN): 8 x 960 takes 27.8 us in one launch and 25.6 in two, 512 of 8 x 1000 40 and 47, 2 x 513 17 and 20.  2 x 3: 18 us a
+// call, kernel 6.0; 8 x 8192: 27, kernels 15.2 + 8.4; 8 x 200000: 52 (planes: 605).  Bound by latency, the long ones by 64-bit multiply-adds.
+constexpr int kTinySide = 8, kTinyPairs = kTinySide * (kTinySide + 1) / 2;
+constexpr long kTinyOne = 1024, kTinyPer = 512, kTinyParts = 128;
+enum { TINY_ALL = 0, TINY_ALL_SEGMENTS, TINY_SUMS, TINY_APPLY };
+struct TinyPoly { double a, b, c, eps; int steps, run, seg; };
+
+// a column of the matrix.  The optimiser's: the first pass moves the momentum.
+template <typename T, bool STEP, bool FIRST> __device__ inline void tiny_column(double (&x)[kTinySide], const Mat &M, const T *src, const Step &st, float clip, float mu, float w, long c)
 {
-    __shared__ float X[kTinySide * (kTinyLong + 1)];
-    __shared__ double A[kTinySide * kTinySide], B[kTinySide * kTinySide], red[4];
+#pragma unroll
+    for (int r = 0; r < kTinySide; ++r) {
+        x[r] = 0.0;
+        if (r >= M.m) continue;
+        const long off = M.tall ? c * M.src_ld + r : r * M.src_ld + c;
+        if constexpr (STEP) {
+            const long at = (long)M.src + off;
+            const float g = st.g[at] * clip;
+            float mm = st.m[at];
+            if (FIRST) {
+                mm = mm + w * (g - mm);
+                st.m[at] = mm;
+            }
+            x[r] = st.nesterov ? g + mu * (mm - g) : mm;
+        } else {
+            x[r] = to_f<T>(src[off]);
+        }
+    }
+}
+
+// NT: threads of a workgroup; with at most 64 columns one wave has all of them, and the same sums.
+template <typename T, bool STEP, int WHAT, int NT = kThreads> __global__ __launch_bounds__(NT) void ortho_tiny(Small list, TinyPoly p, char *ws, Step st)
+{
+    constexpr int S = kTinySide, WAVES = NT / 64;
+    constexpr bool ONE = WHAT == TINY_ALL || WHAT == TINY_ALL_SEGMENTS;
+    __shared__ double red[WAVES][kTinyPairs], A[S * S], W[S * S], V[S * S], Q[2][S * S], held[WHAT == TINY_ALL_SEGMENTS ? S * kTinyOne : 1];
     int k = 0;
     while (k + 1 < list.n && list.first[k + 1] <= (int)blockIdx.x) ++k;
     const Mat &M = list.m[k];
-    const int bi = blockIdx.x - list.first[k], cols = M.tall ? M.m : M.n, m = M.m, n = M.n, ld = n | 1, E = m * m;
-    const T *src = reinterpret_cast<const T *>(M.src) + bi * M.src_stride;
-    double s = 0.0;
-    for (int i = threadIdx.x; i < m * n; i += kThreads) {
-        const float v = to_f<T>(src[(long)(i / cols) * M.src_ld + i % cols]);
-        s += (double)v * v;
+    const int item = blockIdx.x - list.first[k], bi = item / M.parts, part = item % M.parts, m = M.m, pairs = m * (m + 1) / 2;
+    const int per = ((M.n + M.parts - 1) / M.parts + NT - 1) & ~(NT - 1), c0 = part * per, c1 = c0 + per < M.n ? c0 + per : M.n;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, e = lane;
+    const int r = e >> 3, c = e & 7, lo = r < c ? r : c, hi = r < c ? c : r, pair = hi * (hi + 1) / 2 + lo;
+    const float mu = STEP ? (float)st.hp[1] : 0.0f, clip = STEP ? clip_scale(st.norm, st.hp[3]) : 1.0f, w = STEP ? (float)(1.0 - st.hp[1]) : 0.0f;
+    const T *src = STEP ? nullptr : reinterpret_cast<const T *>(M.src) + bi * M.src_stride;
+    // the workspace of a batch element (THIN): two sets of the parts' sums, by the parity of the segment that they belong to, then X
+    double *sums = nullptr, *X = held;
+    if (!ONE) {
+        sums = reinterpret_cast<double *>(ws + M.part) + bi * (2l * M.parts * pairs + (long)m * M.n);
+        X = sums + 2l * M.parts * pairs;
     }
-    s = sqrt(block_sum(s, red));
-    const double mul = 1.0 / (s < p.eps ? p.eps : s);
-    for (int i = threadIdx.x; i < m * n; i += kThreads) {
-        const int r = i / cols, c = i % cols;
-        X[M.tall ? c * ld + r : r * ld + c] = (float)((double)to_f<T>(src[(long)r * M.src_ld + c]) * mul);
-    }
-    int per = 1;      // threads of an element of A
-    while (per < 64 && 2 * per * E <= kThreads) per <<= 1;
-    const int e = threadIdx.x / per, slice = threadIdx.x & (per - 1), i = e / m, j = e % m;
-    __syncthreads();
-    for (int step = 0; step < p.steps; ++step) {
-        double f = 0.0;
-        if (e < E)
-            for (int c = slice; c < n; c += per) f = fma((double)X[i * ld + c], (double)X[j * ld + c], f);
-        for (int o = per >> 1; o > 0; o >>= 1) f += __shfl_xor(f, o, 64);
-        if (e < E && slice == 0) A[e] = f;
-        __syncthreads();
-        if ((int)threadIdx.x < E) {
-            const int r = threadIdx.x / m, c = threadIdx.x % m;
-            double g = 0.0;
-            for (int x = 0; x < m; ++x) g = fma(A[r * m + x], A[x * m + c], g);
-            B[threadIdx.x] = p.b * A[threadIdx.x] + p.c * g;
+    auto column = [&](double (&x)[S], long col, bool source) {      // (what a thread reads of X it wrote itself)
+        if (source) return tiny_column<T, STEP, false>(x, M, src, st, clip, mu, w, col);
+#pragma unroll
+        for (int i = 0; i < S; ++i) x[i] = i < m ? X[(long)i * M.n + col] : 0.0;
+    };
+    double *q = Q[0], *spare = Q[1];
+    // this workgroup's sums of the products of X's rows, X <- Q X first (seg > 0)
+    auto sum = [&](int seg) {
+        double s[kTinyPairs];
+#pragma unroll
+        for (int i = 0; i < kTinyPairs; ++i) s[i] = 0.0;
+        for (int col = c0 + tid; col < c1; col += NT) {
+            double x[S];
+            if (seg == 0) {
+                tiny_column<T, STEP, true>(x, M, src, st, clip, mu, w, col);
+            } else {
+                double u[S];
+                column(u, col, seg == 1);
+#pragma unroll
+                for (int i = 0; i < S; ++i) {
+                    x[i] = 0.0;
+                    if (i >= m) continue;
+#pragma unroll
+                    for (int j = 0; j < S; ++j) x[i] = fma(q[i * S + j], u[j], x[i]);
+                    X[(long)i * M.n + col] = x[i];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < S; ++i)
+                if (i < m)
+#pragma unroll
+                    for (int j = 0; j <= i; ++j) s[i * (i + 1) / 2 + j] = fma(x[i], x[j], s[i * (i + 1) / 2 + j]);
         }
         __syncthreads();
-        for (int c = threadIdx.x; c < n; c += kThreads) {
-            double x[kTinySide];
+        if (c0 + wave * 64 >= c1) {      // (no column for this wave)
+            if (lane < pairs) red[wave][lane] = 0.0;
+        } else {
 #pragma unroll
-            for (int r = 0; r < kTinySide; ++r) x[r] = r < m ? (double)X[r * ld + c] : 0.0;
-            for (int r = 0; r < m; ++r) {
-                double g = X[r * ld + c];
+            for (int i = 0; i < kTinyPairs; ++i)
+                if (i < pairs) {
+                    for (int o = 32; o > 0; o >>= 1) s[i] += __shfl_xor(s[i], o, 64);
+                    if (lane == 0) red[wave][i] = s[i];
+                }
+        }
+        __syncthreads();
+    };
+    auto joined = [&](int i) {
+        if constexpr (WAVES == 1) return red[0][i];
+        else return (red[0][i] + red[1][i]) + (red[2][i] + red[3][i]);
+    };
+    auto times = [&](const double *L, const double *R) {      // (of matrices that commute: symmetric, so the upper triangle's value for both)
+        double f = 0.0;
 #pragma unroll
-                for (int q = 0; q < kTinySide; ++q)
-                    if (q < m) g = fma(B[r * m + q], x[q], g);
-                X[r * ld + c] = (float)(p.a * g);      // (b, c are over a)
+        for (int x = 0; x < S; ++x) f = fma(L[lo * S + x], R[x * S + hi], f);
+        return f;
+    };
+    // the steps of segment `seg` on the sums in `red`, into q: one wave's work, whose LDS accesses are done in the order that they are written in
+    auto in_order = [] { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); };
+    auto iterate = [&](int seg) {
+        const int begin = seg * p.run, end = begin + p.run < p.steps ? begin + p.run : p.steps;
+        if (wave == 0) {
+            A[e] = hi < m ? joined(pair) : 0.0;
+            double mul = 1.0;
+            if (seg == 0) {
+                in_order();
+                double norm = 0.0;
+                for (int i = 0; i < m; ++i) norm += A[i * S + i];
+                norm = sqrt(norm);
+                mul = 1.0 / (norm < p.eps ? p.eps : norm);      // (a NaN norm: NaN everywhere)
+                in_order();
+                A[e] = A[e] * mul * mul;
+            }
+            q[e] = r == c ? mul : 0.0;
+            in_order();
+            double *from = q, *to = spare;
+            for (int step = begin; step < end; ++step) {
+                W[e] = fma(p.c, times(A, A), fma(p.b, A[e], r == c ? p.a : 0.0));      // P
+                in_order();
+                to[e] = times(W, from);
+                if (step + 1 < end) {
+                    V[e] = times(A, W);
+                    in_order();
+                    A[e] = times(W, V);
+                }
+                in_order();
+                double *const was = from;
+                from = to;
+                to = was;
             }
         }
+        if ((end - begin) & 1) {
+            double *const was = q;
+            q = spare;
+            spare = was;
+        }
         __syncthreads();
+    };
+    const int segments = (p.steps + p.run - 1) / p.run;
+    if (ONE) {
+        for (int seg = 0; seg < (WHAT == TINY_ALL ? 1 : segments); ++seg) {
+            sum(seg);
+            iterate(seg);
+        }
+    } else {
+        if (p.seg > 0) {      // the segment before this launch's: its parts' sums, a quarter of them a wave
+            const int was = (p.seg - 1) & 1;
+            if (e < pairs) {
+                double s = 0.0;
+                for (int k = wave; k < M.parts; k += WAVES) s += sums[((long)was * M.parts + k) * pairs + e];
+                red[wave][e] = s;
+            }
+            __syncthreads();
+            iterate(p.seg - 1);
+        }
+        if (WHAT == TINY_SUMS) {
+            const int now = p.seg & 1;
+            sum(p.seg);
+            if (tid < pairs) sums[((long)now * M.parts + part) * pairs + tid] = joined(tid);
+            return;
+        }
     }
-    T *dst = reinterpret_cast<T *>(M.dst) + bi * M.dst_stride;
-    for (int q = threadIdx.x; q < m * n; q += kThreads) {
-        const int r = q / cols, c = q % cols;
-        dst[(long)r * M.dst_ld + c] = from_f<T>(X[M.tall ? c * ld + r : r * ld + c]);
+    const float keep = STEP ? (float)(1.0 - st.hp[0] * st.hp[2]) : 1.0f, go = STEP ? (float)(st.hp[0] * (double)M.scale) : 1.0f;
+    T *dst = STEP ? nullptr : reinterpret_cast<T *>(M.dst) + bi * M.dst_stride;
+    for (int col = c0 + tid; col < c1; col += NT) {
+        double x[S];
+        column(x, col, segments == 1);
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            if (i >= m) continue;
+            double f = 0.0;
+#pragma unroll
+            for (int j = 0; j < S; ++j) f = fma(q[i * S + j], x[j], f);
+            const long off = M.tall ? (long)col * M.dst_ld + i : i * M.dst_ld + col;
+            if constexpr (STEP) {
+                st.g[(long)M.src + off] = 0.0f;      // (the optimiser's rows are as far apart in both)
+                float *o = st.p + (long)M.dst + off;
+                *o = *o * keep - go * (float)f;
+            } else {
+                dst[off] = from_f<T>((float)f);
+            }
+        }
     }
 }
 
@@ -1154,34 +1291,63 @@ __global__ __launch_bounds__(kThreads) void muon_vectors(Ranges rg, float *p, fl
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------------------
-struct Poly { double a, b, c; int steps, first, rest, grow_first, grow_rest; };      // steps of the first segment and of the following ones; the powers of two X grows by in them
+struct Poly { double a, b, c; int steps, first, rest, grow_first, grow_rest; double most; };      // most: max|P| on the way; steps of the first segment and of the following ones; the powers of two X grows by in them
 
 // The bounds that the fixed scales rely on, for singular values that start anywhere in [0, 1]: X and A stay below 2^2 (s < 4 would
 // square to 16: 2^12 * 16 = 65536 overflows fp16), B and R below 15, and a segment's q below 2^6 (the exponents of X).
 bool bounded(Poly &p)
 {
     if (!(isfinite(p.a) && isfinite(p.b) && isfinite(p.c)) || fabs(p.a) < 1e-3) return tef::fail("orthogonalisation: the coefficients have to be finite, the first one not 0");
-    double first = 1.0, rest = 1.0;
-    for (int g = 0; g <= 512; ++g) {
-        double s = g / 512.0, q = 1.0, size = 1.0;
+    // 513 values s (0 among them: its q is 1); W at once, no branches between them: the host does this on every call
+    constexpr int W = 8;
+    const double a = p.a, b = p.b / p.a, c = p.c / p.a;
+    double first = 1.0, rest = 1.0, least[W], largest[W];
+    for (int w = 0; w < W; ++w) least[w] = largest[w] = 1.0;
+    for (int g = 1; g <= 512; g += W) {
+        double s[W], q[W], top[W], far[W], size = 1.0;
+        for (int w = 0; w < W; ++w) s[w] = (g + w) / 512.0, q[w] = 1.0;
         for (int k = 0, left = p.first; k < p.steps; ++k, --left) {
-            if (left == 0) { left = p.rest; q = size = 1.0; }
-            const double l = s * s, poly = 1.0 + (p.b * l + p.c * l * l) / p.a;
-            q *= poly;
-            size *= p.a;
-            s *= p.a * poly;
-            if (!(fabs(s) < 3.9 && fabs(poly - 1.0) < 15.0 && fabs(q - 1.0) < 15.0 && fabs(size) < 64.0 && fabs(size * q) < 64.0))
+            if (left == 0) {
+                left = p.rest;
+                size = 1.0;
+                for (int w = 0; w < W; ++w) q[w] = 1.0;
+            }
+            size *= a;
+            for (int w = 0; w < W; ++w) {
+                const double l = s[w] * s[w], poly = 1.0 + (b + c * l) * l;
+                q[w] *= poly;
+                s[w] *= a * poly;
+                least[w] = poly < least[w] ? poly : least[w];
+                largest[w] = poly > largest[w] ? poly : largest[w];
+                top[w] = fabs(s[w]);
+                far[w] = fabs(q[w] - 1.0);
+            }
+            double grown = 1.0;
+            int held = 1;
+            for (int w = 0; w < W; ++w) {
+                held &= (int)(top[w] < 3.9) & (int)(far[w] < 15.0);      // (not for NaN)
+                grown = fabs(q[w]) > grown ? fabs(q[w]) : grown;
+            }
+            grown *= fabs(size);
+            if (!held || !(grown < 64.0))
                 return tef::fail("orthogonalisation: these coefficients let the iteration grow past what it can hold (singular values below 3.9)");
             double &most = k < p.first ? first : rest;
-            most = fabs(size * q) > most ? fabs(size * q) : most;
+            most = grown > most ? grown : most;
         }
     }
+    double low = 1.0, high = 1.0;
+    for (int w = 0; w < W; ++w) {
+        low = least[w] < low ? least[w] : low;
+        high = largest[w] > high ? largest[w] : high;
+    }
+    if (high - 1.0 >= 15.0 || 1.0 - low >= 15.0) return tef::fail("orthogonalisation: these coefficients let the iteration grow past what it can hold (singular values below 3.9)");
+    p.most = fabs(a) * (high > -low ? high : -low);
     p.grow_first = (int)ceil(log2(first));
     p.grow_rest = (int)ceil(log2(rest));
     return true;
 }
 
-enum Form { TINY, SMALL, TILED, FORMS };
+enum Form { TINY, THIN, SMALL, TILED, FORMS };
 struct Cut { int whole, splits; long items, joins; };
 struct Group {
     Mat m[kGroup];
@@ -1405,26 +1571,70 @@ int iterate(Group &g, const Poly &p, double eps, char *ws, const Step &st, hipSt
     return tef::check_launch("orthogonalisation");
 }
 
-// One workgroup a matrix for small ones: 27 us against the tiled launches' 71 for a single 64 x 18 one,
-// 81 against 94 at the limit of 64 x 320, 63 against 185 for 512 of 64 x 64.
-template <typename T> int small(const Group &g, Form form, const Poly &p, double eps, hipStream_t stream)
+// The launches of up to kChunk matrices each: items(matrix) workgroups a matrix.  (Batches hold up to 2^20 matrices and a matrix's items are at
+// most 2^22, a launch holds up to 2^24 workgroups.)
+template <typename Items, typename Launch> void in_chunks(const Group &g, Items items, Launch launch)
 {
-    const SmallPoly sp{(float)p.a, (float)(p.b / p.a), (float)(p.c / p.a), p.steps, p.first, p.grow_first, p.grow_rest, eps};
     for (int at = 0; at < g.n;) {
         Small list;
-        int items = 0, longest = 0;
-        // (batches hold up to 2^20 matrices, a launch up to 2^24 workgroups)
-        for (list.n = 0; list.n < kChunk && at < g.n && items <= 0x700000; ++list.n, ++at) {
+        int total = 0, longest = 0;
+        for (list.n = 0; list.n < kChunk && at < g.n && total <= 0x700000; ++list.n, ++at) {
             list.m[list.n] = g.m[at];
-            list.first[list.n] = items;
-            items += g.m[at].batch;
+            list.first[list.n] = total;
+            total += (int)items(g.m[at]);
             longest = longest > g.m[at].n ? longest : g.m[at].n;
         }
-        const dim3 grid((unsigned)items), block(kThreads);
-        if (form == TINY) hipLaunchKernelGGL(ortho_tiny<T>, grid, block, 0, stream, list, sp);
-        else if (longest <= 64) hipLaunchKernelGGL((ortho_small<T, 2>), grid, block, 0, stream, list, sp);
+        launch(list, dim3((unsigned)total), longest);
+    }
+}
+
+// One workgroup a matrix for small ones: 27 us against the tiled launches' 71 for a single 64 x 18 one,
+// 81 against 94 at the limit of 64 x 320, 63 against 185 for 512 of 64 x 64.
+template <typename T> int small(const Group &g, const Poly &p, double eps, hipStream_t stream)
+{
+    const SmallPoly sp{(float)p.a, (float)(p.b / p.a), (float)(p.c / p.a), p.steps, p.first, p.grow_first, p.grow_rest, eps};
+    in_chunks(g, [](const Mat &M) { return M.batch; }, [&](const Small &list, dim3 grid, int longest) {
+        const dim3 block(kThreads);
+        if (longest <= 64) hipLaunchKernelGGL((ortho_small<T, 2>), grid, block, 0, stream, list, sp);
         else if (longest <= 128) hipLaunchKernelGGL((ortho_small<T, 4>), grid, block, 0, stream, list, sp);
         else hipLaunchKernelGGL((ortho_small<T, 10>), grid, block, 0, stream, list, sp);
+    });
+    return tef::check_launch("orthogonalisation");
+}
+
+void plan_thin(Group &g)
+{
+    long at = 0;
+    for (int k = 0; k < g.n; ++k) {
+        Mat &M = g.m[k];
+        const long most = (1l << 22) / M.batch;
+        long parts = (M.n + kTinyPer - 1) / kTinyPer;
+        parts = parts > kTinyParts ? kTinyParts : parts;
+        parts = parts > most ? most : parts;
+        M.parts = (int)parts;
+        M.part = at;
+        at += (M.batch * (parts * M.m * (M.m + 1) + (long)M.m * M.n) * 8 + 255) & ~255l;      // two sets of m (m + 1) / 2 sums; X
+    }
+    g.bytes = at;
+}
+template <typename T, bool STEP> int tiny(const Group &g, Form form, const Poly &p, double eps, char *ws, const Step &st, hipStream_t stream)
+{
+    // (rounding of 10^-16 stays below 10^-9 of A through a run: A' takes max|P|^2 of it a step)
+    const double most = p.most > 1.0 ? log(p.most) : 0.0;
+    const int run = most > 0.0 && 2.0 * most * p.steps > log(1e6) ? (int)fmax(1.0, floor(log(1e6) / (2.0 * most))) : p.steps;
+    TinyPoly tp{p.a, p.b, p.c, eps, p.steps, run, 0};
+    const dim3 block(kThreads);
+    const auto items = [](const Mat &M) { return M.batch * M.parts; };
+    if (form == TINY) {
+        in_chunks(g, items, [&](const Small &list, dim3 grid, int longest) {
+            if (run >= p.steps && longest <= 64) hipLaunchKernelGGL((ortho_tiny<T, STEP, TINY_ALL, 64>), grid, dim3(64), 0, stream, list, tp, ws, st);
+            else if (run >= p.steps) hipLaunchKernelGGL((ortho_tiny<T, STEP, TINY_ALL>), grid, block, 0, stream, list, tp, ws, st);
+            else hipLaunchKernelGGL((ortho_tiny<T, STEP, TINY_ALL_SEGMENTS>), grid, block, 0, stream, list, tp, ws, st);
+        });
+    } else {
+        for (; tp.seg * run < p.steps; ++tp.seg)
+            in_chunks(g, items, [&](const Small &list, dim3 grid, int) { hipLaunchKernelGGL((ortho_tiny<T, STEP, TINY_SUMS>), grid, block, 0, stream, list, tp, ws, st); });
+        in_chunks(g, items, [&](const Small &list, dim3 grid, int) { hipLaunchKernelGGL((ortho_tiny<T, STEP, TINY_APPLY>), grid, block, 0, stream, list, tp, ws, st); });
     }
     return tef::check_launch("orthogonalisation");
 }
@@ -1433,7 +1643,7 @@ bool polynomial(Poly &p, int steps, double a, double b, double c, double eps, in
 {
     if (steps < 1 || steps > kMaxSteps) return tef::fail("orthogonalisation: 1 to 32 steps");
     if (!(eps >= 1e-200 && eps < 1e30)) return tef::fail("orthogonalisation: eps must be positive (1e-200 at least: 1 / eps is formed)");
-    p = Poly{a, b, c, steps, first, rest, 0, 0};
+    p = Poly{a, b, c, steps, first, rest, 0, 0, 0.0};
     return bounded(p);
 }
 
@@ -1443,7 +1653,7 @@ template <typename D> Form form_of(const D &d, bool step)
 {
     const long m = d.rows < d.cols ? d.rows : d.cols, n = d.rows < d.cols ? d.cols : d.rows;
     if (step) return TILED;
-    return m <= kTinySide && n <= kTinyLong ? TINY : m <= kSmallSide && n <= kSmallLong ? SMALL : TILED;
+    return m <= kTinySide ? (n <= kTinyOne ? TINY : THIN) : m <= kSmallSide && n <= kSmallLong ? SMALL : TILED;
 }
 
 bool take(Mat &M, const tef_ortho_matrix &d)
@@ -1473,12 +1683,15 @@ template <typename D> bool next_group(Group &g, const D *m, int &at, int count, 
     for (; at < count && g.n < kGroup; ++at)
         if (form_of(m[at], step) == form && !take(g.m[g.n++], m[at])) return false;
     if (g.n && form == TILED) plan(g);
+    if (form == THIN) plan_thin(g);
+    if (form == TINY)
+        for (int k = 0; k < g.n; ++k) g.m[k].parts = 1;
     return true;
 }
 
 template <typename T> int run(Group &g, Form form, const Poly &p, double eps, char *ws, hipStream_t stream)
 {
-    return form == TILED ? iterate<T, false>(g, p, eps, ws, Step{}, stream) : small<T>(g, form, p, eps, stream);
+    return form == TILED ? iterate<T, false>(g, p, eps, ws, Step{}, stream) : form == SMALL ? small<T>(g, p, eps, stream) : tiny<T, false>(g, form, p, eps, ws, Step{}, stream);
 }
 
 template <typename D> size_t workspace_of(const D *m, int count, bool step)
