@@ -18,8 +18,10 @@
 // iteration in fp32, on gradients of rank m / 4 to m, segments of 2, 1, 1, 1 steps are 1.05 to 1.2 times as far from 64 bits
 // (1.4 below 64 rows), 3 + 2 steps 1.5 to 3.5 times.  orthogonalize() takes the former: 6 m^2 n + 4 m^3
 // multiply-adds (symmetric products at half) where the plain iteration takes 10 m^2 n + 5 m^3.  Small matrices take the same segments in
-// one workgroup; those of up to 8 rows are iterated on the small side alone, in 64 bits, without planes.  The optimiser takes the latter, 3 m^2 n + 7 m^3: its update is scaled by the learning rate and added to fp32 parameters, whose own
-// rounding is as large as that error.
+// one workgroup; those of up to 8 rows are iterated on the small side alone, in 64 bits, without planes.  The optimiser
+// takes the latter, 3 m^2 n + 7 m^3: on momenta as networks have them (rank m / 4 to m over noise, 9 to 512 rows) the rms distance of a step's
+// parameters from 64 bits is 0.97 to 1.21 times that of the plain iteration, the largest element's 0.7 to 1.7 times; segments of 2, 1, 1, 1
+// would make that 0.81 to 1.09 and 0.6 to 1.7 and the default network's step 1.25 ms instead of 0.92.
 //
 // Arithmetic.  fp32 matrix instructions run at 1/16 of the fp16 rate, so every operand is held as two fp16 planes, v = hi + lo
 // with hi = fp16(v), lo = fp16(v - hi) — 22 bits — and a product is hi hi + hi lo + lo hi with fp32 accumulation; the dropped lo lo
@@ -154,7 +156,8 @@ __device__ inline double block_sum(double s, double *red)
 
 // ---- the matrices' values ---------------------------------------------------------------------------------------------------
 // Orthogonalisation: the caller's matrix.  Optimiser step: the look-ahead of the momentum, u = g + mu (m' - g) (Nesterov) or m',
-// g the clipped gradient, m' = m + (1 - mu) (g - m); the first sweep writes m', the second one clears g.
+// g the clipped gradient, m' = m + (1 - mu) (g - m); the first sweep writes m', the second one clears g.  u is formed as mu m' + (1 - mu) g:
+// while the momentum is young g and mu (m' - g) nearly cancel (a tenth is left on the first step), and their roundings would be ten times u's own.
 struct Step {
     float *g, *m, *p;                  // flat buffers; a Mat's src / dst are element offsets into them
     const float *norm;
@@ -193,7 +196,7 @@ template <typename T, bool STEP> __global__ __launch_bounds__(kThreads) void ort
             float mm = st.m[off + i];
             mm = mm + w * (g - mm);
             st.m[off + i] = mm;
-            const float u = st.nesterov ? g + mu * (mm - g) : mm;
+            const float u = st.nesterov ? mu * mm + w * g : mm;
             s += (double)u * u;
         };
         long i = lo + 4l * threadIdx.x;
@@ -203,7 +206,7 @@ template <typename T, bool STEP> __global__ __launch_bounds__(kThreads) void ort
             for (int j = 0; j < 4; ++j) {
                 const float gc = g.v[j] * clip;
                 mm.v[j] = mm.v[j] + w * (gc - mm.v[j]);
-                const float u = st.nesterov ? gc + mu * (mm.v[j] - gc) : mm.v[j];
+                const float u = st.nesterov ? mu * mm.v[j] + w * gc : mm.v[j];
                 s += (double)u * u;
             }
             *reinterpret_cast<Pack<float, 4> *>(st.m + off + i) = mm;
@@ -264,14 +267,14 @@ template <typename T, bool STEP> __global__ __launch_bounds__(kThreads) void ort
         up = e[0] - kExpX;
     }
     const double mul = ldexp(1.0 / div, kExpX + up);
-    const float clip = STEP ? clip_scale(st.norm, st.hp[3]) : 1.0f, mu = STEP ? (float)st.hp[1] : 0.0f;
+    const float clip = STEP ? clip_scale(st.norm, st.hp[3]) : 1.0f, mu = STEP ? (float)st.hp[1] : 0.0f, w = STEP ? (float)(1.0 - st.hp[1]) : 0.0f;
     const T *src = reinterpret_cast<const T *>(M.src) + bi * M.src_stride;
     auto value = [&](long off) -> float {      // element `off` of the source
         if constexpr (STEP) {
             const long i = (long)M.src + off;
             const float g = st.g[i] * clip, mm = st.m[i];
             st.g[i] = 0.0f;
-            return st.nesterov ? g + mu * (mm - g) : mm;
+            return st.nesterov ? mu * mm + w * g : mm;
         } else {
             return to_f<T>(src[off]);
         }
@@ -297,7 +300,7 @@ template <typename T, bool STEP> __global__ __launch_bounds__(kThreads) void ort
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     const float gc = g.v[k] * clip;
-                    f[k] = st.nesterov ? gc + mu * (mm.v[k] - gc) : mm.v[k];
+                    f[k] = st.nesterov ? mu * mm.v[k] + w * gc : mm.v[k];
                     zero.v[k] = 0.0f;
                 }
                 *reinterpret_cast<Pack<float, 8> *>(st.g + at) = zero;
@@ -1066,15 +1069,16 @@ template <typename T, int LINES> __global__ __launch_bounds__(kThreads) void ort
 // step of fp32, where the plain fp32 iteration is 0.4 to 4.8e-6 off.
 // Up to kTinyOne columns a matrix is one workgroup's, in one launch (TINY); longer ones take a launch for each sum and one for the
 // result, in workgroups of kTinyPer columns and more, whose sums go through the workspace and are added up in order by every workgroup
-// of the next launch (THIN): 8 x 960 takes 27.8 us in one launch and 25.6 in two, 512 of 8 x 1000 40 and 47, 2 x 513 17 and 20.  2 x 3: 18 us a
-// call, kernel 6.0; 8 x 8192: 27, kernels 15.2 + 8.4; 8 x 200000: 52 (planes: 605).  Bound by latency, the long ones by 64-bit multiply-adds.
+// of the next launch (THIN): 8 x 960 takes 18.8 us in one launch and 20.4 in two, 8 x 1500 23.8 and 20.8, 512 of 8 x 1000 31.5 and 33.  2 x 3: 17
+// us a call, kernel 6.0; 8 x 8192: 20, kernels 7.3 + 9.0; 8 x 200000: 43 (planes: 605).  Bound by the call and by latency, the long ones by
+// 64-bit multiply-adds.
 constexpr int kTinySide = 8, kTinyPairs = kTinySide * (kTinySide + 1) / 2;
 constexpr long kTinyOne = 1024, kTinyPer = 512, kTinyParts = 128;
 enum { TINY_ALL = 0, TINY_ALL_SEGMENTS, TINY_SUMS, TINY_APPLY };
 struct TinyPoly { double a, b, c, eps; int steps, run, seg; };
 
 // a column of the matrix.  The optimiser's: the first pass moves the momentum.
-template <typename T, bool STEP, bool FIRST> __device__ inline void tiny_column(double (&x)[kTinySide], const Mat &M, const T *src, const Step &st, float clip, float mu, float w, long c)
+template <typename T, bool STEP, bool FIRST> __device__ inline void tiny_column(double (&x)[kTinySide], const Mat &M, const T *src, const Step &st, float clip, double mu, long c)
 {
 #pragma unroll
     for (int r = 0; r < kTinySide; ++r) {
@@ -1086,10 +1090,10 @@ template <typename T, bool STEP, bool FIRST> __device__ inline void tiny_column(
             const float g = st.g[at] * clip;
             float mm = st.m[at];
             if (FIRST) {
-                mm = mm + w * (g - mm);
+                mm = mm + (float)(1.0 - mu) * (g - mm);
                 st.m[at] = mm;
             }
-            x[r] = st.nesterov ? g + mu * (mm - g) : mm;
+            x[r] = st.nesterov ? mu * mm + (1.0 - mu) * g : mm;
         } else {
             x[r] = to_f<T>(src[off]);
         }
@@ -1109,7 +1113,8 @@ template <typename T, bool STEP, int WHAT, int NT = kThreads> __global__ __launc
     const int per = ((M.n + M.parts - 1) / M.parts + NT - 1) & ~(NT - 1), c0 = part * per, c1 = c0 + per < M.n ? c0 + per : M.n;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, e = lane;
     const int r = e >> 3, c = e & 7, lo = r < c ? r : c, hi = r < c ? c : r, pair = hi * (hi + 1) / 2 + lo;
-    const float mu = STEP ? (float)st.hp[1] : 0.0f, clip = STEP ? clip_scale(st.norm, st.hp[3]) : 1.0f, w = STEP ? (float)(1.0 - st.hp[1]) : 0.0f;
+    const double mu = STEP ? st.hp[1] : 0.0;
+    const float clip = STEP ? clip_scale(st.norm, st.hp[3]) : 1.0f;
     const T *src = STEP ? nullptr : reinterpret_cast<const T *>(M.src) + bi * M.src_stride;
     // the workspace of a batch element (THIN): two sets of the parts' sums, by the parity of the segment that they belong to, then X
     double *sums = nullptr, *X = held;
@@ -1118,7 +1123,7 @@ template <typename T, bool STEP, int WHAT, int NT = kThreads> __global__ __launc
         X = sums + 2l * M.parts * pairs;
     }
     auto column = [&](double (&x)[S], long col, bool source) {      // (what a thread reads of X it wrote itself)
-        if (source) return tiny_column<T, STEP, false>(x, M, src, st, clip, mu, w, col);
+        if (source) return tiny_column<T, STEP, false>(x, M, src, st, clip, mu, col);
 #pragma unroll
         for (int i = 0; i < S; ++i) x[i] = i < m ? X[(long)i * M.n + col] : 0.0;
     };
@@ -1131,7 +1136,7 @@ template <typename T, bool STEP, int WHAT, int NT = kThreads> __global__ __launc
         for (int col = c0 + tid; col < c1; col += NT) {
             double x[S];
             if (seg == 0) {
-                tiny_column<T, STEP, true>(x, M, src, st, clip, mu, w, col);
+                tiny_column<T, STEP, true>(x, M, src, st, clip, mu, col);
             } else {
                 double u[S];
                 column(u, col, seg == 1);
@@ -1153,13 +1158,24 @@ template <typename T, bool STEP, int WHAT, int NT = kThreads> __global__ __launc
         __syncthreads();
         if (c0 + wave * 64 >= c1) {      // (no column for this wave)
             if (lane < pairs) red[wave][lane] = 0.0;
-        } else {
+        } else if (m <= 4) {
 #pragma unroll
-            for (int i = 0; i < kTinyPairs; ++i)
+            for (int i = 0; i < 10; ++i)
                 if (i < pairs) {
                     for (int o = 32; o > 0; o >>= 1) s[i] += __shfl_xor(s[i], o, 64);
                     if (lane == 0) red[wave][i] = s[i];
                 }
+        } else {      // halving: a lane sends the half of its sums that it does not keep (63 exchanges instead of 216), lane i ends with sum i
+            double v[64];
+#pragma unroll
+            for (int i = 0; i < 64; ++i) v[i] = i < kTinyPairs ? s[i] : 0.0;
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) {
+                const bool upper = lane & o;
+#pragma unroll
+                for (int i = 0; i < o; ++i) v[i] = (upper ? v[i + o] : v[i]) + __shfl_xor(upper ? v[i] : v[i + o], o, 64);
+            }
+            if (lane < pairs) red[wave][lane] = v[0];
         }
         __syncthreads();
     };
@@ -1652,8 +1668,8 @@ bool polynomial(Poly &p, int steps, double a, double b, double c, double eps, in
 template <typename D> Form form_of(const D &d, bool step)
 {
     const long m = d.rows < d.cols ? d.rows : d.cols, n = d.rows < d.cols ? d.cols : d.rows;
-    if (step) return TILED;
-    return m <= kTinySide ? (n <= kTinyOne ? TINY : THIN) : m <= kSmallSide && n <= kSmallLong ? SMALL : TILED;
+    if (m <= kTinySide) return n <= kTinyOne ? TINY : THIN;
+    return !step && m <= kSmallSide && n <= kSmallLong ? SMALL : TILED;      // (the optimiser's momentum and parameters: tiny or tiles)
 }
 
 bool take(Mat &M, const tef_ortho_matrix &d)
@@ -1763,12 +1779,15 @@ int tef_muon_step(float *p, float *g, float *m, float *v, const tef_muon_matrix 
     hipStream_t st = (hipStream_t)stream;
     const Step s{g, m, p, norm, hp, nesterov != 0};
     Group gr;
-    for (int at = 0; at < nmatrices;) {
-        if (!next_group(gr, matrices, at, nmatrices, TILED, true)) return TEF_ERR_INVALID;
-        if (!gr.n) break;
-        const int rc = iterate<float, true>(gr, poly, eps, (char *)workspace, s, st);
-        if (rc) return rc;
-    }
+    for (int f = 0; f < FORMS; ++f)
+        for (int at = 0; at < nmatrices;) {
+            const Form form = (Form)f;
+            if (!next_group(gr, matrices, at, nmatrices, form, true)) return TEF_ERR_INVALID;
+            if (!gr.n) break;
+            const int rc = form == TILED ? iterate<float, true>(gr, poly, eps, (char *)workspace, s, st)
+                                         : tiny<float, true>(gr, form, poly, eps, (char *)workspace, s, st);
+            if (rc) return rc;
+        }
     long v0 = 0;
     for (int at = 0; at < nvectors; at += kRanges) {
         Ranges rg;
