@@ -566,8 +566,9 @@ int tef_layer_norm_backward(const tef_norm_desc *d, const void *x, const void *w
  * row's elements contiguous) X = U / max(|U|_F, eps), then `steps` times X <- a X + (b A + c A A) X with A = X X^T (X^T X for tall
  * ones: same result), written to dst (which may be src).  All matrices of a call go through the same launches.
  * src and dst have type `dtype` (TEF_F32 / F16 / BF16) and the alignment of their elements; the arithmetic is fp32-grade
- * whatever the type.  1 <= steps <= 32, 1e-200 <= eps < 1e30; a first coefficient of 0 and coefficients under which a singular value in
- * [0, 1] would leave |s| < 3.9 are refused.  The matrix list is read during the call only.  Workspace: 256-byte aligned, the caller's, of the size asked for with the same
+ * whatever the type.  1 <= steps <= 32, 1e-200 <= eps < 1e30.  With P(s) = a + b s^2 + c s^4, a coefficient a of 0, |P| / |a| past 16, the product
+ * of P over two neighbouring steps past 64 (|a| >= 8), and coefficients under which a singular value in [0, 1] would leave |s| < 3.9 are refused:
+ * by both entry points alike, and by tef_orthogonalize_check (0 or TEF_ERR_INVALID; nothing is launched).  The matrix list is read during the call only.  Workspace: 256-byte aligned, the caller's, of the size asked for with the same
  * list; two calls that may run at once need two. */
 typedef struct tef_ortho_matrix {
     const void *src;
@@ -580,6 +581,7 @@ typedef struct tef_ortho_matrix {
     long src_stride;
     long dst_stride;
 } tef_ortho_matrix;
+int tef_orthogonalize_check(int steps, double a, double b, double c, double eps);
 size_t tef_orthogonalize_workspace_bytes(const tef_ortho_matrix *matrices, int count);
 int tef_orthogonalize(const tef_ortho_matrix *matrices, int count, int dtype, int steps, double a, double b, double c, double eps,
                       void *workspace, size_t workspace_bytes, void *stream);

@@ -245,6 +245,7 @@ SIGNATURES = {
     "tef_layer_norm_forward": (ctypes.c_int, [ctypes.POINTER(NormDesc)] + [_fp] * 8),
     "tef_layer_norm_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(NormDesc)]),
     "tef_layer_norm_backward": (ctypes.c_int, [ctypes.POINTER(NormDesc)] + [_fp] * 12 + [ctypes.c_size_t, _fp]),
+    "tef_orthogonalize_check": (ctypes.c_int, [ctypes.c_int] + [ctypes.c_double] * 4),
     "tef_orthogonalize_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(OrthoMatrix), ctypes.c_int]),
     "tef_orthogonalize": (ctypes.c_int, [ctypes.POINTER(OrthoMatrix), ctypes.c_int, ctypes.c_int, ctypes.c_int] + [ctypes.c_double] * 4
                           + [_fp, ctypes.c_size_t, _fp]),

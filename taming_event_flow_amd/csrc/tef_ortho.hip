@@ -1346,7 +1346,7 @@ bool bounded(Poly &p)
             }
             grown *= fabs(size);
             if (!held || !(grown < 64.0))
-                return tef::fail("orthogonalisation: these coefficients let the iteration grow past what it can hold (singular values below 3.9)");
+                return tef::fail("orthogonalisation: these coefficients let the iteration grow past what it can hold (singular values below 3.9, their polynomial below 64 in two steps)");
             double &most = k < p.first ? first : rest;
             most = grown > most ? grown : most;
         }
@@ -1356,7 +1356,7 @@ bool bounded(Poly &p)
         low = least[w] < low ? least[w] : low;
         high = largest[w] > high ? largest[w] : high;
     }
-    if (high - 1.0 >= 15.0 || 1.0 - low >= 15.0) return tef::fail("orthogonalisation: these coefficients let the iteration grow past what it can hold (singular values below 3.9)");
+    if (high - 1.0 >= 15.0 || 1.0 - low >= 15.0) return tef::fail("orthogonalisation: these coefficients let the iteration grow past what it can hold (singular values below 3.9, their polynomial below 64 in two steps)");
     p.most = fabs(a) * (high > -low ? high : -low);
     p.grow_first = (int)ceil(log2(first));
     p.grow_rest = (int)ceil(log2(rest));
@@ -1727,6 +1727,12 @@ template <typename D> size_t workspace_of(const D *m, int count, bool step)
 
 extern "C" {
 
+int tef_orthogonalize_check(int steps, double a, double b, double c, double eps)
+{
+    Poly p;
+    return polynomial(p, steps, a, b, c, eps, 2, 1) ? 0 : TEF_ERR_INVALID;
+}
+
 size_t tef_orthogonalize_workspace_bytes(const tef_ortho_matrix *matrices, int count) { return workspace_of(matrices, count, false); }
 
 int tef_orthogonalize(const tef_ortho_matrix *matrices, int count, int dtype, int steps, double a, double b, double c, double eps,
@@ -1763,7 +1769,8 @@ int tef_muon_step(float *p, float *g, float *m, float *v, const tef_muon_matrix 
                   double c, double eps, void *workspace, size_t workspace_bytes, void *stream)
 {
     Poly poly;
-    if (!polynomial(poly, steps, a, b, c, eps, steps % 3 == 1 && steps > 1 ? 2 : 3, 3)) return TEF_ERR_INVALID;
+    // (segments of three steps where their q stays below 2^6: a below 4; else as orthogonalize, with the same refusals)
+    if (!polynomial(poly, steps, a, b, c, eps, steps % 3 == 1 && steps > 1 ? 2 : 3, 3) && !polynomial(poly, steps, a, b, c, eps, 2, 1)) return TEF_ERR_INVALID;
     if (!p || !g || !m || !norm || !hp || !step || nvectors < 0 || (nvectors && (!vectors || !v)))
         return tef::fail("tef_muon_step: null pointer"), TEF_ERR_INVALID;
     long total = 0;

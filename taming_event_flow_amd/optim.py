@@ -121,6 +121,8 @@ class FusedMuon(FusedAdam):
         if bucket.flat.dtype != torch.float32:
             raise TypeError(f"FusedMuon: float32 parameters (got {bucket.flat.dtype})")
         self._poly = _polynomial(steps, coefficients, eps)
+        if _lib.lib().tef_orthogonalize_check(*self._poly):      # (here, not in the first step, which would have been counted by then)
+            raise ValueError(_lib.lib().tef_last_error().decode())
         _lib.require_device_tensor(bucket.flat, "FusedMuon gradient bucket")
         self.nesterov = bool(nesterov)
         super().__init__(bucket, lr, betas=betas, eps=adam_eps)
