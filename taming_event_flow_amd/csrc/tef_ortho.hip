@@ -1404,7 +1404,7 @@ Cut cut_one(long tiles, long lines, int ts)
 
 // Tile sizes: 128 where the launch then still covers the 256 CUs, else 64 (a quarter of the work each, so that four times as many
 // workgroups share it).
-void plan(Group &g)
+bool plan(Group &g)
 {
     long chain128 = 0, apply128 = 0, steps128 = 0;
     for (int k = 0; k < g.n; ++k) {
@@ -1477,8 +1477,12 @@ void plan(Group &g)
         for (int w = 0; w < 2; ++w) g.chain[w] = Cut{0, 1, first[PH_CHAIN] * (w + 1), 0};
     }
     // (a launch holds less than 2^32 threads: 2^24 workgroups of 256, and a launch of two products has twice the items)
-    for (int f = 0; f < PHASES; ++f) g.grid[f] = first[f] > 0x7fffff ? -1 : (int)first[f];
     g.bytes = at;
+    for (int f = 0; f < PHASES; ++f) {
+        if (first[f] > 0x7fffff) return tef::fail("orthogonalisation: too many tiles for one launch");
+        g.grid[f] = (int)first[f];
+    }
+    return true;
 }
 
 bool describe(Mat &M, long rows, long cols, long batch)
@@ -1498,8 +1502,6 @@ bool describe(Mat &M, long rows, long cols, long batch)
 template <typename T, bool STEP>
 int iterate(Group &g, const Poly &p, double eps, char *ws, const Step &st, hipStream_t stream)
 {
-    for (int f = 0; f < PHASES; ++f)
-        if (g.grid[f] < 0) return tef::fail("orthogonalisation: too many tiles for one launch"), TEF_ERR_INVALID;
     Mat *table = reinterpret_cast<Mat *>(ws);
     const dim3 block(kThreads);
     for (int at = 0; at < g.n; at += kChunk) {
@@ -1698,7 +1700,7 @@ template <typename D> bool next_group(Group &g, const D *m, int &at, int count, 
     g.bytes = 0;
     for (; at < count && g.n < kGroup; ++at)
         if (form_of(m[at], step) == form && !take(g.m[g.n++], m[at])) return false;
-    if (g.n && form == TILED) plan(g);
+    if (g.n && form == TILED && !plan(g)) return false;
     if (form == THIN) plan_thin(g);
     if (form == TINY)
         for (int k = 0; k < g.n; ++k) g.m[k].parts = 1;
