@@ -118,6 +118,9 @@ class FusedMuon(FusedAdam):
             raise ValueError(f"momentum = {momentum}: in [0, 1)")
         if not (math.isfinite(lr) and lr >= 0.0 and math.isfinite(weight_decay) and weight_decay >= 0.0):
             raise ValueError(f"lr = {lr}, weight_decay = {weight_decay}: finite, not negative")
+        as_vector = {id(p) for p in vectors}
+        if as_vector - {id(p) for p in bucket.params}:
+            raise ValueError("vectors: parameters of the bucket (an entry is not one of them)")
         if bucket.flat.dtype != torch.float32:
             raise TypeError(f"FusedMuon: float32 parameters (got {bucket.flat.dtype})")
         self._poly = _polynomial(steps, coefficients, eps)
@@ -127,7 +130,6 @@ class FusedMuon(FusedAdam):
         self.nesterov = bool(nesterov)
         super().__init__(bucket, lr, betas=betas, eps=adam_eps)
         self.param_groups[0].update(momentum=float(momentum), weight_decay=float(weight_decay), adam_lr=None if adam_lr is None else float(adam_lr))
-        as_vector = {id(p) for p in vectors}
         matrices, ranges, at, nvec = [], [], 0, 0
         for p in bucket.params:
             n = p.numel()

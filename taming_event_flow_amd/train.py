@@ -241,6 +241,18 @@ def _held_by_a_graph(params):
     return held
 
 
+def _muon_arguments(model, config):
+    """FusedMuon's keyword arguments in an optimizer config; `vectors` holds names of parameters, or of modules for all of theirs."""
+    kw = {k: v for k, v in config.items() if k not in ("name", "lr", "capturable")}
+    vectors = []
+    for name in kw.pop("vectors", None) or ():
+        found = [p for n, p in model.named_parameters() if n == name or n.startswith(f"{name}.")]
+        if not found:
+            raise ValueError(f"optimizer: vectors: no parameter or module named {name!r}")
+        vectors += [p for p in found if p.requires_grad]
+    return dict(kw, vectors=vectors)
+
+
 class Trainer:
     """model + loss + optimiser wired like reference train_flow.py:60-70, plus the DP gradient bucket."""
 
@@ -275,8 +287,7 @@ class Trainer:
             self.optimizer = self.fused_opt
         elif config["optimizer"]["name"] == "Muon":
             # orthogonalised updates for the matrices, Adam for the vectors (optim.FusedMuon's keyword arguments in the config)
-            self.fused_opt = self.optimizer = FusedMuon(self.bucket, config["optimizer"]["lr"],
-                                                        **{k: config["optimizer"][k] for k in extra})
+            self.fused_opt = self.optimizer = FusedMuon(self.bucket, config["optimizer"]["lr"], **_muon_arguments(self.model, config["optimizer"]))
         else:
             self.optimizer = getattr(torch.optim, config["optimizer"]["name"])(self.model.parameters(), **opt_kwargs)
         self.last_loss = None

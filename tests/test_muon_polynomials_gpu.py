@@ -37,3 +37,26 @@ def test_steps(dev, abc, steps):  # noqa: F811
         want = q.double() - scale * o
         bound = scale * (8 * plain + (segments_floor(steps, abc) + 2e-6) * o.abs().max().item()) + 2.0 ** -23 * want.abs().max().item()
         assert (p.detach().double().cpu() - want).abs().max().item() <= bound, tuple(p.shape)
+
+
+def test_heads_left_to_adam_by_name(dev):  # noqa: F811
+    """A Trainer's config: `vectors: [arch.preds]` gives the prediction heads Adam (a first step of at most adam_lr), the rest orthogonalised ones."""
+    import copy
+
+    from taming_event_flow_amd import train
+
+    cfg = copy.deepcopy(train.DEFAULT_CONFIG)
+    cfg["data"]["passes_loss"] = 2
+    cfg["loader"].update(batch_size=1, resolution=[32, 32], max_num_grad_events=200)
+    cfg["model"].update(base_channels=8)
+    cfg["optimizer"] = dict(name="Muon", lr=0.5, adam_lr=1e-4, vectors=["arch.preds"])
+    torch.manual_seed(0)
+    tr = train.Trainer(cfg, dev)
+    src = train.SyntheticSequences(cfg, dev, 300, seq_len=10 ** 9)
+    before = {n: p.detach().clone() for n, p in tr.model.named_parameters()}
+    tr.step(src.next(), new_seq=True), tr.step(src.next())
+    moved = {n: (p.detach() - before[n]).abs().max().item() for n, p in tr.model.named_parameters()}
+    heads = [n for n in moved if ".preds." in n]
+    assert len(heads) == 8 and all(moved[n] <= 1.01e-4 for n in heads) and max(moved[n] for n in heads) > 0
+    assert any(v > 1e-2 for n, v in moved.items() if n not in heads)
+    tr.close()
