@@ -585,6 +585,20 @@ int tef_orthogonalize_check(int steps, double a, double b, double c, double eps)
 size_t tef_orthogonalize_workspace_bytes(const tef_ortho_matrix *matrices, int count);
 int tef_orthogonalize(const tef_ortho_matrix *matrices, int count, int dtype, int steps, double a, double b, double c, double eps,
                       void *workspace, size_t workspace_bytes, void *stream);
+/* What the matrix number `index` of a list would go through (nothing is launched): form 0 up to 8 rows in one workgroup, 1 up to 8 rows in
+ * several, 2 up to 64 x 320 in one workgroup, 3 tiles; of the latter the tile sides, workgroups and joins of the Gram product, of one and two
+ * m x m products, and the tile side of the last product.  optimiser: as tef_muon_step would (rows and cols count). */
+typedef struct tef_ortho_plan {
+    int form;
+    int gram_tile;
+    int gram_items;
+    int gram_joins;
+    int chain_tile;
+    int chain_items[2];
+    int chain_joins[2];
+    int apply_tile;
+} tef_ortho_plan;
+int tef_orthogonalize_plan(const tef_ortho_matrix *matrices, int count, int index, int optimiser, tef_ortho_plan *out);
 /* tef_muon_step: one optimiser step on flat fp32 buffers p (parameters), g (gradients), m (momentum), v (Adam's second moments of
  * the vectors only, packed in list order).  g is first scaled by min(1, max_norm / (norm + 1e-6)) (max_norm <= 0: not).
  * Matrices: m += (1 - momentum) (g - m); u = nesterov ? g + momentum (m - g) : m; p <- p (1 - lr weight_decay) - lr scale O(u),

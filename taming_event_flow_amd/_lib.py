@@ -105,6 +105,13 @@ class OrthoMatrix(ctypes.Structure):
                                                                             "dst_stride")]
 
 
+class OrthoPlan(ctypes.Structure):
+    """struct tef_ortho_plan (include/tef.h)"""
+
+    _fields_ = [("form", ctypes.c_int), ("gram_tile", ctypes.c_int), ("gram_items", ctypes.c_int), ("gram_joins", ctypes.c_int),
+                ("chain_tile", ctypes.c_int), ("chain_items", ctypes.c_int * 2), ("chain_joins", ctypes.c_int * 2), ("apply_tile", ctypes.c_int)]
+
+
 class MuonMatrix(ctypes.Structure):
     """struct tef_muon_matrix (include/tef.h)"""
 
@@ -249,6 +256,8 @@ SIGNATURES = {
     "tef_orthogonalize_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(OrthoMatrix), ctypes.c_int]),
     "tef_orthogonalize": (ctypes.c_int, [ctypes.POINTER(OrthoMatrix), ctypes.c_int, ctypes.c_int, ctypes.c_int] + [ctypes.c_double] * 4
                           + [_fp, ctypes.c_size_t, _fp]),
+    "tef_orthogonalize_plan": (ctypes.c_int, [ctypes.POINTER(OrthoMatrix), ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                              ctypes.POINTER(OrthoPlan)]),
     "tef_muon_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(MuonMatrix), ctypes.c_int]),
     "tef_muon_step": (ctypes.c_int, [_fp] * 4 + [ctypes.POINTER(MuonMatrix), ctypes.c_int, ctypes.POINTER(MuonVector), ctypes.c_int]
                       + [_fp] * 3 + [ctypes.c_int, ctypes.c_int] + [ctypes.c_double] * 4 + [_fp, ctypes.c_size_t, _fp]),

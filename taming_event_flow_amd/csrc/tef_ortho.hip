@@ -1764,6 +1764,24 @@ int tef_orthogonalize(const tef_ortho_matrix *matrices, int count, int dtype, in
     return 0;
 }
 
+int tef_orthogonalize_plan(const tef_ortho_matrix *matrices, int count, int index, int optimiser, tef_ortho_plan *out)
+{
+    if (!out || index < 0 || index >= count) return tef::fail("tef_orthogonalize_plan: no such matrix"), TEF_ERR_INVALID;
+    if (!workspace_of(matrices, count, optimiser != 0)) return TEF_ERR_INVALID;
+    memset(out, 0, sizeof(*out));
+    const Form form = form_of(matrices[index], optimiser != 0);
+    out->form = form;
+    if (form != TILED) return 0;
+    Group g;
+    for (int at = 0; at <= index;)
+        if (!next_group(g, matrices, at, count, form, optimiser != 0)) return TEF_ERR_INVALID;
+    out->gram_tile = g.ts_gram; out->gram_items = (int)g.gram.items; out->gram_joins = (int)g.gram.joins;
+    out->chain_tile = g.ts_chain;
+    for (int k = 0; k < 2; ++k) { out->chain_items[k] = (int)g.chain[k].items; out->chain_joins[k] = (int)g.chain[k].joins; }
+    out->apply_tile = g.ts_apply;
+    return 0;
+}
+
 size_t tef_muon_workspace_bytes(const tef_muon_matrix *matrices, int count) { return workspace_of(matrices, count, true); }
 
 int tef_muon_step(float *p, float *g, float *m, float *v, const tef_muon_matrix *matrices, int nmatrices, const tef_muon_vector *vectors,
