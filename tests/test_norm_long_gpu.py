@@ -43,3 +43,36 @@ def test_more_columns_than_a_launch_has_threads(dev):
     # g, s1 and u s2 with a few roundings each, u off by du in the last two; rstd relative
     bound = rstd * (8 * U * (d64.abs().max() + s1.abs() + 1.8 * s2.abs()) + du * (s2.abs() + d64.abs().mean())) + 8 * U * want.abs().max()
     assert ((dx - want).abs().max() <= bound).item()
+
+
+CASES = [((70001, 32768), lambda t: t[-3:]), ((300007, 8192), lambda t: t[-3:]), ((33, 1024, 256, 257), lambda t: t[-1:, :, -2:]),
+         ((33, 1024, 255, 257), lambda t: t[-1:, :, -2:]), ((5, 9000, 223, 223), lambda t: t[-1:, :, -1:])]
+
+
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_gradients_past_32_bits(dev, case):
+    """More than 2^31 elements, in the rows' and the maps' forms and the long one: every gradient at the last rows / positions, and those of the
+    vectors, to which only they contribute (the rest has a gradient of zero).  Bounds: test_norm_gpu.py."""
+    from test_norm_gpu import check, reference
+    from taming_event_flow_amd.models.norm import layer_norm
+
+    shape, tail = CASES[case]
+    C = shape[1]
+    assert torch.Size(shape).numel() > 2 ** 31
+    gen = torch.Generator(device=dev).manual_seed(case)
+    x, r, dy = (torch.zeros(shape, dtype=torch.bfloat16, device=dev) for _ in range(3))
+    parts = []
+    for t in (x, r, dy):
+        parts.append(torch.randn(tail(t).shape, generator=gen, device=dev).to(t.dtype))
+        tail(t).copy_(parts[-1])
+    w, b = torch.linspace(0.5, 1.5, C, device=dev), torch.linspace(-1, 1, C, device=dev)
+    leaves = [t.requires_grad_(True) for t in (x, w, b, r)]
+    y = layer_norm(x, w, b, activation="tanh", residual=r)
+    want, _, _ = reference(parts[0], w, b, parts[1], 1, 1e-5, "tanh", parts[2])
+    check("y", tail(y.detach()), want["y"])
+    grads = torch.autograd.grad(y, leaves, dy)
+    del y
+    for name, g in zip(("dx", "dw", "db", "dres"), grads):
+        check(name, tail(g) if g.dim() > 1 else g, want[name])
+    for g in (grads[0], grads[3]):
+        assert not g[0].any()
