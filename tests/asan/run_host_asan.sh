@@ -16,4 +16,4 @@ UB=$(dirname $RT)/libclang_rt.ubsan_standalone-x86_64.so
 # of its own, with redzones
 LD_PRELOAD=$RT:$STUB TEF_HIP_LIB=$LIB TEF_HIP_STUB=$STUB PYTHONMALLOC=malloc \
   ASAN_OPTIONS=detect_leaks=0:halt_on_error=1:abort_on_error=1:detect_odr_violation=0:protect_shadow_gap=0 \
-  UBSAN_OPTIONS=halt_on_error=1:print_stacktrace=1 python $ROOT/tests/asan/dry_run_driver.py "$@"
+  UBSAN_OPTIONS=halt_on_error=1:print_stacktrace=1 python $ROOT/tests/asan/${TEF_ASAN_DRIVER:-dry_run_driver}.py "$@"
