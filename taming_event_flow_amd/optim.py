@@ -92,7 +92,7 @@ def orthogonalize(update, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
             ws, at = _aligned(nbytes, first.device)
             _lib.check(lib.tef_orthogonalize(arr, len(descs), _DTYPES[first.dtype], steps, a, b, c, eps, at, nbytes, _lib.stream_ptr()),
                        "tef_orthogonalize")
-    return type(update)(out) if many else out[0]
+    return (out if isinstance(update, list) else tuple(out)) if many else out[0]      # (a named tuple's class takes no list)
 
 
 class FusedMuon(FusedAdam):

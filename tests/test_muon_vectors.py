@@ -18,6 +18,19 @@ def test_entries_that_are_no_parameters():
         optim.FusedMuon(bucket, 0.1, vectors=params[:1])
 
 
+def test_named_tuples_of_matrices(monkeypatch):
+    """A named tuple is a tuple: empty matrices need no device."""
+    from collections import namedtuple
+
+    from taming_event_flow_amd import optim
+
+    monkeypatch.setattr(optim._lib, "require_device_tensor", lambda t, name: t)
+    pair = namedtuple("pair", "a b")(torch.zeros(0, 3), torch.zeros(2, 0))
+    got = optim.orthogonalize(pair)
+    assert isinstance(got, tuple) and [tuple(t.shape) for t in got] == [(0, 3), (2, 0)]
+    assert isinstance(optim.orthogonalize(list(pair)), list)
+
+
 def test_names_in_a_config():
     from taming_event_flow_amd import train
 
