@@ -152,15 +152,21 @@ template <bool WG> __device__ inline void row_sums(float &s, float &q, int L, fl
         q = (red[4] + red[5]) + (red[6] + red[7]);
     }
 }
-// sums of d and d^2 -> the correction of the mean, 1 / sqrt(variance + eps)
+// 1 / sqrt(v), within a unit of its last bit: the error of the two roundings of 1.0f / sqrtf(v), r, taken off once.  (0, inf and NaN as they come.)
+__device__ inline float inverse_root(float v)
+{
+    const float r = 1.0f / sqrtf(v), h = v * r, low = fmaf(v, r, -h), off = fmaf(-h, r, 1.0f) - low * r;      // 1 - v r^2
+    return fabsf(off) < 1.0f ? fmaf(0.5f * r, off, r) : r;
+}
+// sums of d and d^2 -> 1 / sqrt(variance + eps), the correction of the mean times that (and the mean corrected): u = d rstd - by in one rounding
 // (inv = 1 / C: products, not divisions, which cost the widest maps a tenth of their time; what a product adds to the first mean is
 // corrected here with the rest of it)
 __device__ inline float correct(float &mean, float sd, float sq, float inv, float eps, float &rstd)
 {
     const float by = sd * inv, var = (sq - sd * by) * inv;
-    rstd = 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + eps);      // (NaN stays NaN)
+    rstd = inverse_root((var < 0.0f ? 0.0f : var) + eps);      // (NaN stays NaN)
     mean += by;
-    return by;
+    return by * rstd;
 }
 
 template <int NV> __device__ inline void row_vec(const void *p, int dtype, int l, int L, int C, float missing, float (&f)[NV][V])
@@ -217,7 +223,7 @@ template <typename T, int NV, bool WG, bool EVEN> __global__ __launch_bounds__(k
         for (int i = 0; i < NV; ++i) {
 #pragma unroll
             for (int k = 0; k < V; ++k)
-                f[i][k] = act(a.act, (f[i][k] - by) * rstd * w[i][k] + b[i][k] + (a.res ? to_f<T>(e[i].v[k]) : 0.0f));
+                f[i][k] = act(a.act, fmaf(fmaf(f[i][k], rstd, -by), w[i][k], b[i][k]) + (a.res ? to_f<T>(e[i].v[k]) : 0.0f));
             store_row<T, V, EVEN>(reinterpret_cast<T *>(a.y) + at, V * (l + L * i), C, f[i]);
         }
     }
@@ -260,7 +266,7 @@ template <typename T, int NV, bool WG, bool EVEN> __global__ __launch_bounds__(k
                 const bool in = live && V * (l + L * i) + k < C;
                 u[i][k] = in ? (to_f<T>(qx[i].v[k]) - mean) * rstd : 0.0f;
                 float g = in ? to_f<T>(qd[i].v[k]) : 0.0f;
-                if (need_z && in) g *= act_slope(a.act, u[i][k] * w[i][k] + b[i][k] + (need_e ? to_f<T>(qe[i].v[k]) : 0.0f));
+                if (need_z && in) g *= act_slope(a.act, fmaf(u[i][k], w[i][k], b[i][k]) + (need_e ? to_f<T>(qe[i].v[k]) : 0.0f));
                 e[k] = g;
                 dw[i][k] += g * u[i][k];
                 db[i][k] += g;
@@ -278,7 +284,7 @@ template <typename T, int NV, bool WG, bool EVEN> __global__ __launch_bounds__(k
         for (int i = 0; i < NV; ++i) {
             float e[V];
 #pragma unroll
-            for (int k = 0; k < V; ++k) e[k] = rstd * (h[i][k] - s1 - u[i][k] * s2);
+            for (int k = 0; k < V; ++k) e[k] = rstd * fmaf(-u[i][k], s2, h[i][k] - s1);
             store_row<T, V, EVEN>(reinterpret_cast<T *>(a.dx) + at, V * (l + L * i), C, e);
         }
     }
@@ -332,7 +338,7 @@ template <int P> __device__ inline void map_sum(float (&s)[P], int LX, float *re
         s[k] = (red[lx * P + k] + red[(LX + lx) * P + k]) + (red[(2 * LX + lx) * P + k] + red[(3 * LX + lx) * P + k]);
 }
 
-// Second sums of a tile's positions, of d = x - mean and d^2: by[k] what the mean is corrected by, rstd[k]; position j of the tile is
+// Second sums of a tile's positions, of d = x - mean and d^2: by[k] what the mean is corrected by, times rstd[k]; position j of the tile is
 // finished by thread j alone (all threads for themselves: 103 us instead of 81 for the map above) and, if asked for, stored.
 // red: the partial sums that the mean was made of, then room for 3 * 256.
 template <int P>
@@ -420,7 +426,7 @@ template <typename T, int NC, int P> __global__ __launch_bounds__(kThreads) void
             const int c = g + G * i;
             if (c >= C) continue;
 #pragma unroll
-            for (int k = 0; k < P; ++k) f[i][k] = act(a.act, (f[i][k] - by[k]) * rstd[k] * w[i] + b[i] + (a.res ? to_f<T>(e[i].v[k]) : 0.0f));
+            for (int k = 0; k < P; ++k) f[i][k] = act(a.act, fmaf(fmaf(f[i][k], rstd[k], -by[k]), w[i], b[i]) + (a.res ? to_f<T>(e[i].v[k]) : 0.0f));
             store<T, P>(reinterpret_cast<T *>(a.y) + at + c * a.inner, f[i]);
         }
     }
@@ -466,7 +472,7 @@ template <typename T, int NC, int P> __global__ __launch_bounds__(kThreads) void
             for (int k = 0; k < P; ++k) {
                 u[i][k] = in ? (to_f<T>(qx[i].v[k]) - mean.v[k]) * rstd.v[k] : 0.0f;
                 h[i][k] = in ? to_f<T>(qd[i].v[k]) : 0.0f;
-                if (need_z && in) h[i][k] *= act_slope(a.act, u[i][k] * w[i] + b[i] + (need_e ? to_f<T>(qe[i].v[k]) : 0.0f));
+                if (need_z && in) h[i][k] *= act_slope(a.act, fmaf(u[i][k], w[i], b[i]) + (need_e ? to_f<T>(qe[i].v[k]) : 0.0f));
             }
             if (a.dres && in) store<T, P>(reinterpret_cast<T *>(a.dres) + at + (g + G * i) * a.inner, h[i]);
 #pragma unroll
@@ -488,7 +494,7 @@ template <typename T, int NC, int P> __global__ __launch_bounds__(kThreads) void
             if (c >= C) continue;
             float e[P];
 #pragma unroll
-            for (int k = 0; k < P; ++k) e[k] = rstd.v[k] * (h[i][k] - s1[k] * inv - u[i][k] * (s2[k] * inv));
+            for (int k = 0; k < P; ++k) e[k] = rstd.v[k] * fmaf(-u[i][k], s2[k] * inv, fmaf(-inv, s1[k], h[i][k]));
             store<T, P>(reinterpret_cast<T *>(a.dx) + at + c * a.inner, e);
         }
     }
@@ -530,13 +536,13 @@ template <typename T> __global__ __launch_bounds__(kThreads) void long_fwd(Args 
             const double d = to_f<T>(x[(long)c * a.inner]) - mean;
             q += d * d;
         }
-        const float rstd = 1.0f / sqrtf((float)(long_sum(q, red) / a.C) + a.eps);
+        const float rstd = (float)(1.0 / sqrt(long_sum(q, red) / a.C + (double)a.eps));
         if (threadIdx.x == 0 && a.mean) { a.mean[r] = (float)mean; a.rstd[r] = rstd; }
         for (int c = threadIdx.x; c < a.C; c += kThreads) {
             const long off = at + (long)c * a.inner;
             const float e = a.res ? to_f<T>(reinterpret_cast<const T *>(a.res)[off]) : 0.0f;
-            const float z = (float)(to_f<T>(reinterpret_cast<const T *>(a.x)[off]) - mean) * rstd * vec_at(a.v.w, a.v.dtype, c, 1.0f) +
-                            vec_at(a.v.b, a.v.dtype, c, 0.0f) + e;
+            const float u = (float)(to_f<T>(reinterpret_cast<const T *>(a.x)[off]) - mean) * rstd;
+            const float z = fmaf(u, vec_at(a.v.w, a.v.dtype, c, 1.0f), vec_at(a.v.b, a.v.dtype, c, 0.0f)) + e;
             reinterpret_cast<T *>(a.y)[off] = from_f<T>(act(a.act, z));
         }
     }
@@ -548,7 +554,7 @@ template <typename T> __device__ inline float long_g(const Args &a, long off, in
     float g = to_f<T>(reinterpret_cast<const T *>(a.dy)[off]);
     if (a.act != TEF_ACT_NONE) {
         const float e = a.res ? to_f<T>(reinterpret_cast<const T *>(a.res)[off]) : 0.0f;
-        g *= act_slope(a.act, *u * vec_at(a.v.w, a.v.dtype, c, 1.0f) + vec_at(a.v.b, a.v.dtype, c, 0.0f) + e);
+        g *= act_slope(a.act, fmaf(*u, vec_at(a.v.w, a.v.dtype, c, 1.0f), vec_at(a.v.b, a.v.dtype, c, 0.0f)) + e);
     }
     return g;
 }
@@ -579,7 +585,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void long_bwd(Args 
         for (int c = threadIdx.x; c < a.C; c += kThreads) {
             const long off = at + (long)c * a.inner;
             const float h = long_g<T>(a, off, c, mean, rstd, &u) * vec_at(a.v.w, a.v.dtype, c, 1.0f);
-            reinterpret_cast<T *>(a.dx)[off] = from_f<T>(rstd * (h - s1 - u * s2));
+            reinterpret_cast<T *>(a.dx)[off] = from_f<T>(rstd * fmaf(-u, s2, h - s1));
         }
     }
 }

@@ -58,3 +58,35 @@ def test_far_offset(dev, shape):
     D = 100
     du = D * U * D * U * 6e4 / var.sqrt() + (2 * D + 8) * U * u.abs()
     assert ((y - u).abs() <= du + U * u.abs()).all()
+
+
+@pytest.mark.parametrize("shape", [(1, 512, 8, 8), (1, 64, 60, 80), (300, 200), (64, 4096), (3, 258, 31, 37), (4, 9000), (16, 70, 7, 9)])
+def test_no_further_from_64_bits_than_elementary_operations(dev, shape):
+    """The root mean square distance of y and dx from 64 bits, against the same formulas as elementary fp32 operations: a value here passes
+    through one rounding fewer (x - mean, its product with rstd less the correction, the product with the weight plus the bias)."""
+    from taming_event_flow_amd.models.norm import layer_norm
+
+    C, lane = shape[1], [1, -1] + [1] * (len(shape) - 2)
+    ours, plains = [0.0, 0.0], [0.0, 0.0]
+    for seed in range(3):
+        gen = torch.Generator(device=dev).manual_seed(seed)
+        x = torch.randn(shape, generator=gen, device=dev) * 2 + 0.3
+        w, b = 1 + 0.2 * torch.randn(C, generator=gen, device=dev), 0.1 * torch.randn(C, generator=gen, device=dev)
+        dy = torch.randn(shape, generator=gen, device=dev)
+
+        def formulas(x, w, b, dy):
+            w, b = w.view(lane), b.view(lane)
+            d = x - x.mean(1, keepdim=True)
+            rstd = 1 / ((d * d).mean(1, keepdim=True) + 1e-5).sqrt()
+            u, h = d * rstd, dy * w
+            return u * w + b, rstd * (h - h.mean(1, keepdim=True) - u * (h * u).mean(1, keepdim=True))
+
+        xl = x.clone().requires_grad_(True)
+        y = layer_norm(xl, w, b)
+        got = (y.detach(), torch.autograd.grad(y, xl, dy)[0])
+        want = formulas(x.double(), w.double(), b.double(), dy.double())
+        plain = formulas(x, w, b, dy)
+        for i in range(2):
+            ours[i] += (got[i] - want[i]).square().sum().item()
+            plains[i] += (plain[i] - want[i]).square().sum().item()
+    assert ours[0] <= plains[0] and ours[1] <= plains[1], [(a / p) ** 0.5 for a, p in zip(ours, plains)]
